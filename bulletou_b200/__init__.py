@@ -82,5 +82,9 @@ from .revive import (  # noqa: F401
     compensate_l1_revival_mean, revive_ft, revive_ft_units, revive_l1_selected, revive_l2, revive_l2_selected,
     saturated_units,
 )
+from .token_layers import (  # noqa: F401
+    DeviceMatrix, dropout, dropout_backward, embedding_backward, embedding_forward, int8_linear, int8_matmul,
+    int8_quantize_rows, router_backward, router_forward,
+)
 
 __version__ = "0.1.0"

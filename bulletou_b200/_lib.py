@@ -83,6 +83,12 @@ class RowExchange(ctypes.Structure):
                 ("slot_rows", Z), ("epoch", I), ("small_recv", U64 * 8), ("small_len", Z), ("small_flag_base", Z)]
 
 
+class Matrix(ctypes.Structure):
+    """BulletOuB200Matrix."""
+
+    _fields_ = [("data", P), ("type", I), ("rows", Z), ("cols", Z), ("row_stride", Z)]
+
+
 class LossSpec(ctypes.Structure):
     """BulletOuB200LossSpec."""
 
@@ -198,6 +204,14 @@ SIGNATURES: dict[str, list] = {
     "bulletou_b200_sfnn_integer_forward_device": [P, P, Z, Z] + [P] * 9,
     "bulletou_b200_teacher_prepare_device": [P, P, P, Z] + [P] * 7,
     "bulletou_b200_hcpe_to_psv_device": [P, P, Z, P, P, P],
+    "bulletou_b200_embedding_forward_device": [P, P, P, F, P],
+    "bulletou_b200_embedding_backward_device": [P, P, P, F, P],
+    "bulletou_b200_dropout_device": [P, P, P, F, U64, U64, P],
+    "bulletou_b200_router_forward_device": [P, P, F, I, P, P, P, P, P],
+    "bulletou_b200_router_backward_device": [P, P, P, P, P, P, F, I, P],
+    "bulletou_b200_int8_quantize_rows_device": [P, P, P, P],
+    "bulletou_b200_int8_matmul_device": [P, P, P, P, P, P, P],
+    "bulletou_b200_int8_linear_device": [P, P, P, P, P, P],
     "bulletou_b200_validation_metrics_device": [P, P, P, P, Z, P, P],
     "bulletou_cuda_cpp_sfnn_validation_stats": [P] * 7 + [Z] * 4,
     "bulletou_cuda_cpp_sfnn_unit_stats": [P] * 7 + [Z] * 5,

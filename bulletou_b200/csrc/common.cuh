@@ -127,6 +127,9 @@ enum ScratchSlot : int {
     kScratchSfnnHeavy = 26,     // SFNN FT rows: segment plan and partial sums of heavy rows
     kScratchHcpe = 27,          // HCPE -> PackedSfenValue: uncompacted records, valid flags, scan
     kScratchValidation = 28,    // validation metrics: per-CTA partials
+    kScratchEmbedding = 29,     // embedding gradient: sorted tokens, partial rows
+    kScratchRouter = 30,        // router: per-CTA probability sums and counts
+    kScratchInt8 = 31,          // 8-bit product: quantised rows, their scales, repacked weights
 };
 
 int ok();

@@ -566,6 +566,102 @@ int bulletou_b200_validation_metrics_device(BulletOuCudaCppContext* ctx, const B
 int bulletou_b200_hcpe_to_psv_device(BulletOuCudaCppContext* ctx, const BulletOuCudaCppI32Buffer* hcpe,
     size_t n_records, BulletOuCudaCppI32Buffer* psv, BulletOuCudaCppI32Buffer* count, BulletOuCudaCppI32Buffer* valid);
 
+/* ---- token layers: a learned LayerStack router ----
+ * The operators of a token model over feature rows whose logits choose the
+ * LayerStack: lookup with scaling and its gradient, dropout, routing with a
+ * balance loss, and the 8-bit product that evaluates a dense layer.  They work
+ * on matrices in device memory of the context's device, on the context's
+ * stream, and allocate nothing but context scratch, which only grows (so a
+ * call whose sizes were seen before can be captured in a graph).  All sums are
+ * held in f32 or in integers; for the same inputs the results are the same
+ * bits from call to call. */
+#define BULLETOU_B200_TYPE_F32 0
+#define BULLETOU_B200_TYPE_BF16 1
+#define BULLETOU_B200_TYPE_I8 2
+#define BULLETOU_B200_TYPE_I32 3
+
+/* rows x cols elements; element (r, c) at data + (r * row_stride + c) elements.
+ * A vector of n is 1 x n.  row_stride counts only where rows > 1, and is then
+ * at least cols.  The memory belongs to the caller. */
+typedef struct BulletOuB200Matrix {
+    void* data;
+    int type;           /* BULLETOU_B200_TYPE_* */
+    size_t rows;
+    size_t cols;
+    size_t row_stride;  /* in elements */
+} BulletOuB200Matrix;
+
+/* out[n][:] = scale * table[token n][:], tokens in row-major order.  A token
+ * outside the table (-1: padding) gives a row of zeros.  table and out: f32 or
+ * bf16 each; tokens: i32 with rows * cols = out's rows. */
+int bulletou_b200_embedding_forward_device(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix* table,
+    const BulletOuB200Matrix* tokens, float scale, const BulletOuB200Matrix* out);
+
+/* table_gradients[v][:] = scale * sum of out_gradients[n][:] over the tokens n
+ * that name row v, in an order that the tokens alone fix; rows that none names
+ * are zeroed.  f32 or bf16 each; the sums are f32. */
+int bulletou_b200_embedding_backward_device(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix* tokens,
+    const BulletOuB200Matrix* out_gradients, float scale, const BulletOuB200Matrix* table_gradients);
+
+/* out = x * [kept] / (1 - p) (+ residual, optional), x, residual and out of one
+ * type, f32 or bf16.  The mask is never stored: element i (row-major) is lane
+ * i % 8 (16 bits, low half first) of the Philox4x32-10 block with the counter
+ * (i / 8, offset) and the key seed, and is kept where the lane is not below
+ * round(p * 65536); p is that multiple of 1 / 65536.  The gradient of x is the
+ * same call on the gradient of out.  A dropped element is 0 whatever x holds
+ * there.  out may be x or residual itself. */
+int bulletou_b200_dropout_device(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix* x,
+    const BulletOuB200Matrix* residual, float probability, unsigned long long seed, unsigned long long offset,
+    const BulletOuB200Matrix* out);
+
+#define BULLETOU_B200_ROUTER_MAX_EXPERTS 512
+#define BULLETOU_B200_ROUTER_MAX_TOP_K 8
+
+/* p = softmax(logits row); experts [rows][k] = the k largest logits' indexes,
+ * largest first, the lowest index first among equals; gates [rows][k] = p
+ * there, with normalize_gates divided by their sum.  k = the columns of
+ * experts.  A logit of -inf is never chosen; where fewer than k are left the
+ * slots hold expert -1 and gate 0, so a row of -inf chooses nothing and counts
+ * nowhere.  A row with NaN or +inf chooses nothing and makes the mean
+ * probabilities and the loss NaN.
+ * counts [experts + 1] = choices of each expert, then the rows that are alive
+ * (a finite largest logit); mean_probabilities[e] = sum of p over the rows /
+ * alive rows; loss = balance * experts * sum_e (counts[e] / all choices) *
+ * mean_probabilities[e]: `balance` where all experts are used alike. */
+int bulletou_b200_router_forward_device(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix* logits, float balance,
+    int normalize_gates, const BulletOuB200Matrix* experts, const BulletOuB200Matrix* gates,
+    const BulletOuB200Matrix* counts, const BulletOuB200Matrix* mean_probabilities, const BulletOuB200Matrix* loss);
+
+/* logit_gradients of the forward's gates and loss: gate_gradients [rows][k]
+ * (optional) is the gradient of gates, loss_gradient [1] (optional) that of
+ * loss; the counts are constants.  experts and counts are the forward's. */
+int bulletou_b200_router_backward_device(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix* logits,
+    const BulletOuB200Matrix* experts, const BulletOuB200Matrix* counts, const BulletOuB200Matrix* gate_gradients,
+    const BulletOuB200Matrix* loss_gradient, float balance, int normalize_gates,
+    const BulletOuB200Matrix* logit_gradients);
+
+/* Inner size at which a sum of 8-bit products could leave 32 bits. */
+#define BULLETOU_B200_INT8_MAX_INNER 131072
+
+/* Row by row: m = max |x|, q = round-to-even(x * (127 * (1 / m))), scales =
+ * m * (1 / 127), each operation rounded to f32.  A row with m < 2^-100 gives
+ * zeros and scale 0; a row with an infinity or a NaN gives zeros and scale
+ * NaN.  x: f32 or bf16; q: i8, same extents; scales: f32 [rows]. */
+int bulletou_b200_int8_quantize_rows_device(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix* x,
+    const BulletOuB200Matrix* q, const BulletOuB200Matrix* scales);
+
+/* out[m][n] = (sum_k q[m][k] * weights[n][k]) * (scales[m] * weight_scales[n])
+ * (+ bias[n], optional), the sum exact in 32-bit integers.  q, weights: i8;
+ * scales, weight_scales, bias: f32; out: f32 or bf16. */
+int bulletou_b200_int8_matmul_device(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix* q,
+    const BulletOuB200Matrix* scales, const BulletOuB200Matrix* weights, const BulletOuB200Matrix* weight_scales,
+    const BulletOuB200Matrix* bias, const BulletOuB200Matrix* out);
+
+/* The two above in one call: x is quantised row by row into context scratch. */
+int bulletou_b200_int8_linear_device(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix* x,
+    const BulletOuB200Matrix* weights, const BulletOuB200Matrix* weight_scales, const BulletOuB200Matrix* bias,
+    const BulletOuB200Matrix* out);
+
 #ifdef __cplusplus
 }
 #endif
