@@ -8,12 +8,18 @@
 #include <algorithm>
 #include <cmath>
 
-#include "device_matrix.cuh"
+#include "int8_linear.cuh"
 
 namespace bou {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr float kSmallest = 0x1p-100f;  // rows below it are zeros: 1 / m and 127 / m stay finite
+
+__device__ __forceinline__ float row_factor(float top) { return 127.0f * __frcp_rn(top); }
+__device__ __forceinline__ float row_scale(float top) { return top * (1.0f / 127.0f); }
+__device__ __forceinline__ int quantised(float x, float factor) { return __float2int_rn(x * factor); }
 
 // ------------------------------------------------------------------ quantisation
 struct QuantizeArgs {
@@ -22,83 +28,265 @@ struct QuantizeArgs {
     int8_t* q;
     size_t q_stride;
     float* scales;
-    int cols, padded_cols;  // columns [cols, padded_cols) of q are zeroed
+    int rows, cols;
+    int padded_cols;  // columns [cols, padded_cols) of q are zeroed
+    bool x_vector;    // 16-byte aligned rows of x
+    bool q_vector;    // 16-byte aligned rows of q, padded_cols a multiple of 16
 };
 
-// CTA per row.
+constexpr int kGroup = 16;  // columns that a thread takes together: a 16-byte store of q
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeArgs a) {
-    __shared__ float warp_top[kThreads / 32];
-    const T* x = static_cast<const T*>(a.x) + blockIdx.x * a.x_stride;
-    int8_t* q = a.q + blockIdx.x * a.q_stride;
-    float top = 0.0f;
-    bool bad = false;
-    for (int c = threadIdx.x; c < a.cols; c += kThreads) {
-        const float v = fabsf(to_f32(x[c]));
-        bad |= !(v < INFINITY);
-        top = fmaxf(top, v);
-    }
-    bad = __syncthreads_or(bad);
+__device__ __forceinline__ void load_group(const T* x, int c, int cols, bool vector, float* v) {
+    if (vector && c + kGroup <= cols) {
+        constexpr int kVec = 16 / sizeof(T);
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
-    __syncthreads();
-    for (int w = 0; w < kThreads / 32; ++w) top = fmaxf(top, warp_top[w]);
-    const bool some = !bad && top >= 0x1p-100f;
-    const float inverse = some ? 127.0f * __frcp_rn(top) : 0.0f;
-    for (int c = threadIdx.x; c < a.padded_cols; c += kThreads)
-        q[c] = c < a.cols && some ? static_cast<int8_t>(__float2int_rn(to_f32(x[c]) * inverse)) : 0;
-    if (threadIdx.x == 0) a.scales[blockIdx.x] = bad ? NAN : some ? top * (1.0f / 127.0f) : 0.0f;
+        for (int i = 0; i < kGroup; i += kVec) {
+            const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(x + c + i));
+            const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) v[i + j] = to_f32(e[j]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) v[i] = c + i < cols ? to_f32(x[c + i]) : 0.0f;
+    }
 }
 
-// ------------------------------------------------------------------ product
-struct ProductArgs {
-    const int8_t* q;
-    const int8_t* w;
-    size_t q_stride, w_stride;
-    const float* scales;
-    const float* w_scales;
-    const float* bias;
-    void* out;
-    size_t out_stride;
-    int m, n, k;
+__device__ __forceinline__ void store_group(const QuantizeArgs& a, int8_t* q, int c, const float* v, float factor, bool some) {
+    int8_t b[kGroup];
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) b[i] = static_cast<int8_t>(some ? quantised(v[i], factor) : 0);
+    if (a.q_vector) {
+        uint4 packed;
+        uint32_t* w = reinterpret_cast<uint32_t*>(&packed);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            w[i] = static_cast<uint8_t>(b[4 * i]) | static_cast<uint32_t>(static_cast<uint8_t>(b[4 * i + 1])) << 8 |
+                   static_cast<uint32_t>(static_cast<uint8_t>(b[4 * i + 2])) << 16 |
+                   static_cast<uint32_t>(static_cast<uint8_t>(b[4 * i + 3])) << 24;
+        *reinterpret_cast<uint4*>(q + c) = packed;
+    } else {
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i)
+            if (c + i < a.padded_cols) q[c + i] = b[i];
+    }
+}
+
+// kRowThreads threads for each row, which holds its values in registers
+// between the maximum and the rounding: x is read once.  Rows longer than
+// 2 * kGroup * kRowThreads (only with kRowThreads == kThreads) read the rest
+// again, from L2.
+template <typename T, int kRowThreads>
+__global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeArgs a) {
+    constexpr int kHeld = 2, kRowWarps = kRowThreads / 32;
+    __shared__ float warp_top[kWarps];
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int in_row = threadIdx.x % kRowThreads;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / kRowThreads) + threadIdx.x / kRowThreads;
+    const bool live = row < a.rows;
+    const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.x_stride;
+    float held[kHeld][kGroup];
+    float top = 0.0f;  // NaN and infinities become +inf here
+    auto take = [&](const float* v) {
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) {
+            const float m = fabsf(v[i]);
+            top = fmaxf(top, m == m ? m : INFINITY);
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+        const int c = (in_row + j * kRowThreads) * kGroup;
+        if (live && c < a.cols) {
+            load_group(x, c, a.cols, a.x_vector, held[j]);
+            take(held[j]);
+        }
+    }
+    for (int c = (in_row + kHeld * kRowThreads) * kGroup; live && c < a.cols; c += kRowThreads * kGroup) {
+        float v[kGroup];
+        load_group(x, c, a.cols, a.x_vector, v);
+        take(v);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if (kRowWarps > 1) {
+        if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
+        __syncthreads();
+        const int first = (threadIdx.x >> 5) / kRowWarps * kRowWarps;
+#pragma unroll
+        for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, warp_top[first + w]);
+    }
+    if (!live) return;
+    const bool some = top >= kSmallest && top < INFINITY;
+    const float factor = some ? row_factor(top) : 0.0f;
+    int8_t* q = a.q + row * a.q_stride;
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+        const int c = (in_row + j * kRowThreads) * kGroup;
+        if (c < a.padded_cols) store_group(a, q, c, held[j], factor, some && c < a.cols);
+    }
+    for (int c = (in_row + kHeld * kRowThreads) * kGroup; c < a.padded_cols; c += kRowThreads * kGroup) {
+        float v[kGroup];
+        load_group(x, c, a.cols, a.x_vector, v);
+        store_group(a, q, c, v, factor, some);
+    }
+    if (in_row == 0) a.scales[row] = top == INFINITY ? NAN : some ? row_scale(top) : 0.0f;
+}
+
+// Rows of bytes into rows that start on 16 bytes, for the TMA.
+__global__ void __launch_bounds__(kThreads) repack_kernel(const int8_t* src, size_t src_stride, int8_t* dst,
+                                                          size_t dst_stride, int rows, int cols) {
+    const int words = (cols + 3) / 4;
+    const size_t n = static_cast<size_t>(rows) * words;
+    for (size_t i = static_cast<size_t>(blockIdx.x) * kThreads + threadIdx.x; i < n;
+         i += static_cast<size_t>(gridDim.x) * kThreads) {
+        const size_t r = i / words;
+        const int c = static_cast<int>(i - r * words) * 4;
+        const int8_t* s = src + r * src_stride + c;
+        uint32_t w = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c + j < cols) w |= static_cast<uint32_t>(static_cast<uint8_t>(s[j])) << (8 * j);
+        *reinterpret_cast<uint32_t*>(dst + r * dst_stride + c) = w;
+    }
+}
+
+// ------------------------------------------------------------------ few rows
+// For up to kFewRows rows the weights' bytes are what counts: every warp takes
+// output channels one after the other, 16 bytes of a channel for each lane at
+// a time, against the rows' 8-bit values in shared memory.  Each CTA quantises
+// the rows itself (they are a few KB from L2), so the layer is one launch, and
+// the first channel's weights are on their way meanwhile.
+constexpr int kFewRows = 4;
+constexpr size_t kFewRowsBytes = 48 * 1024;  // shared memory for the rows
+
+struct FewRowsArgs {
+    ProductArgs p;
+    bool quantise;  // the rows are x; otherwise p.q and p.scales
+    const void* x;
+    size_t x_stride;
+    bool w_vector;  // 16-byte aligned rows of w
 };
 
-constexpr int kTileM = 64, kTileN = 64, kTileK = 64;
+// 16 bytes of a weight row from column c on, zeros beyond its end.
+__device__ __forceinline__ uint4 load_weights(const int8_t* w, int c, int cols, bool vector) {
+    if (vector && c + 16 <= cols) return __ldg(reinterpret_cast<const uint4*>(w + c));
+    uint4 packed = make_uint4(0, 0, 0, 0);
+    uint32_t* word = reinterpret_cast<uint32_t*>(&packed);
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+        if (c + j < cols) word[j >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(w[c + j])) << (8 * (j & 3));
+    return packed;
+}
 
-// A 64 x 64 tile of the output, 4 x 4 results for each thread.
-template <typename Out>
-__global__ void __launch_bounds__(kThreads) product_kernel(const ProductArgs a) {
-    __shared__ int sq[kTileK / 4][kTileM + 1], sw[kTileK / 4][kTileN + 1];
-    const int m0 = blockIdx.y * kTileM, n0 = blockIdx.x * kTileN;
-    const int tm = (threadIdx.x >> 4) * 4, tn = (threadIdx.x & 15) * 4;
-    int acc[4][4] = {};
-    for (int k0 = 0; k0 < a.k; k0 += kTileK) {
-        for (int i = threadIdx.x; i < kTileM * kTileK; i += kThreads) {
-            const int r = i / kTileK, c = i % kTileK;
-            const bool k_in = k0 + c < a.k;
-            reinterpret_cast<int8_t*>(&sq[c / 4][r])[c % 4] =
-                k_in && m0 + r < a.m ? a.q[static_cast<size_t>(m0 + r) * a.q_stride + k0 + c] : 0;
-            reinterpret_cast<int8_t*>(&sw[c / 4][r])[c % 4] =
-                k_in && n0 + r < a.n ? a.w[static_cast<size_t>(n0 + r) * a.w_stride + k0 + c] : 0;
-        }
-        __syncthreads();
+template <typename T, typename Out, int kRows>
+__global__ void __launch_bounds__(kThreads) few_rows_kernel(const FewRowsArgs a) {
+    extern __shared__ uint4 shared_rows[];  // [kRows][pitch] bytes
+    __shared__ float tops[kWarps][kRows];
+    constexpr int kAhead = 4;
+    const ProductArgs& p = a.p;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int pitch = (p.k + 15) / 16 * 16;
+    int8_t* const rows = reinterpret_cast<int8_t*>(shared_rows);
+    int64_t n = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+    const int64_t first_end = static_cast<int64_t>(blockIdx.x + 1) * kWarps;
+    uint4 ahead[kAhead];
 #pragma unroll
-        for (int c = 0; c < kTileK / 4; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(sq[c][tm + i], sw[c][tn + j], acc[i][j]);
-        __syncthreads();
+    for (int i = 0; i < kAhead; ++i) {
+        const int c = (i * 32 + lane) * 16;
+        ahead[i] = n < p.n && c < p.k ? load_weights(p.w + n * p.w_stride, c, p.k, a.w_vector) : make_uint4(0, 0, 0, 0);
     }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int m = m0 + tm + i, n = n0 + tn + j;
-            if (m >= a.m || n >= a.n) continue;
-            float y = static_cast<float>(acc[i][j]) * (a.scales[m] * a.w_scales[n]);
-            if (a.bias != nullptr) y += a.bias[n];
-            static_cast<Out*>(a.out)[static_cast<size_t>(m) * a.out_stride + n] = from_f32<Out>(y);
+    float scale[kRows];
+    if (a.quantise) {
+        const T* x = static_cast<const T*>(a.x);
+        float top[kRows];
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            top[r] = 0.0f;
+            if (r < p.m)
+                for (int c = threadIdx.x; c < p.k; c += kThreads) {
+                    const float m = fabsf(to_f32(x[r * a.x_stride + c]));
+                    top[r] = fmaxf(top[r], m == m ? m : INFINITY);
+                }
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], d));
+            if (lane == 0) tops[warp][r] = top[r];
         }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) top[r] = fmaxf(top[r], tops[w][r]);
+            const bool some = top[r] >= kSmallest && top[r] < INFINITY;
+            const float factor = some ? row_factor(top[r]) : 0.0f;
+            scale[r] = top[r] == INFINITY ? NAN : some ? row_scale(top[r]) : 0.0f;
+            for (int c = threadIdx.x; c < pitch; c += kThreads)
+                rows[r * pitch + c] = static_cast<int8_t>(
+                    some && r < p.m && c < p.k ? quantised(to_f32(x[r * a.x_stride + c]), factor) : 0);
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            scale[r] = r < p.m ? p.scales[r] : 0.0f;
+            for (int c = threadIdx.x; c < pitch; c += kThreads)
+                rows[r * pitch + c] = r < p.m && c < p.k ? p.q[r * p.q_stride + c] : 0;
+        }
+    }
+    __syncthreads();
+    for (; n < p.n; n += static_cast<int64_t>(gridDim.x) * kWarps) {
+        const int8_t* w = p.w + n * p.w_stride;
+        int sum[kRows] = {};
+        auto take = [&](const uint4& v, int c) {
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) {
+                const int4 q = *reinterpret_cast<const int4*>(rows + r * pitch + c);
+                sum[r] = __dp4a(static_cast<int>(v.x), q.x, sum[r]);
+                sum[r] = __dp4a(static_cast<int>(v.y), q.y, sum[r]);
+                sum[r] = __dp4a(static_cast<int>(v.z), q.z, sum[r]);
+                sum[r] = __dp4a(static_cast<int>(v.w), q.w, sum[r]);
+            }
+        };
+        for (int c0 = lane * 16; c0 < p.k; c0 += kAhead * 512) {
+            uint4 v[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int c = c0 + i * 512;
+                const bool first = n < first_end && c0 == lane * 16;
+                v[i] = first ? ahead[i] : c < p.k ? load_weights(w, c, p.k, a.w_vector) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+                if (c0 + i * 512 < p.k) take(v[i], c0 + i * 512);
+        }
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], d);
+        if (lane == 0) {
+            const float ws = p.w_scales[n], b = p.bias != nullptr ? p.bias[n] : 0.0f;
+#pragma unroll
+            for (int r = 0; r < kRows; ++r)
+                if (r < p.m)
+                    static_cast<Out*>(p.out)[r * p.out_stride + n] = from_f32<Out>(int8_result(sum[r], scale[r], ws, b));
+        }
+    }
+}
+
+// ------------------------------------------------------------------ host
+size_t padded(size_t n, size_t to) { return (n + to - 1) / to * to; }
+
+template <typename T>
+void launch_quantize(BulletOuCudaCppContext* ctx, const QuantizeArgs& a) {
+    const int cols = std::max(a.cols, a.padded_cols);
+    auto grid = [&](int row_threads) {
+        const int per = kThreads / row_threads;
+        return static_cast<unsigned>((static_cast<int64_t>(a.rows) + per - 1) / per);
+    };
+    if (cols <= 32 * 32) quantize_kernel<T, 32><<<grid(32), kThreads, 0, ctx->stream>>>(a);
+    else if (cols <= 64 * 32) quantize_kernel<T, 64><<<grid(64), kThreads, 0, ctx->stream>>>(a);
+    else if (cols <= 128 * 32) quantize_kernel<T, 128><<<grid(128), kThreads, 0, ctx->stream>>>(a);
+    else quantize_kernel<T, 256><<<grid(256), kThreads, 0, ctx->stream>>>(a);
 }
 
 int quantize(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix& x, int8_t* q, size_t q_stride, int padded_cols,
@@ -109,25 +297,89 @@ int quantize(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix& x, int8_t* q
     a.q = q;
     a.q_stride = q_stride;
     a.scales = scales;
+    a.rows = static_cast<int>(x.rows);
     a.cols = static_cast<int>(x.cols);
     a.padded_cols = padded_cols;
-    const int grid = static_cast<int>(x.rows);
-    if (x.type == BULLETOU_B200_TYPE_F32)
-        quantize_kernel<float><<<grid, kThreads, 0, ctx->stream>>>(a);
-    else
-        quantize_kernel<__nv_bfloat16><<<grid, kThreads, 0, ctx->stream>>>(a);
+    a.x_vector = rows_aligned(x, 16);
+    a.q_vector = padded_cols % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 && (x.rows <= 1 || q_stride % 16 == 0);
+    if (x.type == BULLETOU_B200_TYPE_F32) launch_quantize<float>(ctx, a);
+    else launch_quantize<__nv_bfloat16>(ctx, a);
     return check_launch("int8 quantise launch");
 }
 
-int product(BulletOuCudaCppContext* ctx, const ProductArgs& a, int out_type) {
-    const unsigned gm = (a.m + kTileM - 1) / kTileM;
-    if (gm > 65535u) return fail_messagef("int8 product: %d rows are not supported", a.m);
-    const dim3 grid((a.n + kTileN - 1) / kTileN, gm);
-    if (out_type == BULLETOU_B200_TYPE_F32)
-        product_kernel<float><<<grid, kThreads, 0, ctx->stream>>>(a);
-    else
-        product_kernel<__nv_bfloat16><<<grid, kThreads, 0, ctx->stream>>>(a);
-    return check_launch("int8 product launch");
+// Whether TMA can read these rows as they are.
+bool tma_rows(const void* data, size_t rows, size_t stride) {
+    return reinterpret_cast<uintptr_t>(data) % 16 == 0 && (rows <= 1 || stride % 16 == 0);
+}
+
+int repack(BulletOuCudaCppContext* ctx, const int8_t* src, size_t stride, int8_t* dst, size_t dst_stride, int rows, int cols) {
+    const size_t words = static_cast<size_t>(rows) * ((cols + 3) / 4);
+    const int grid = static_cast<int>(std::min<size_t>((words + kThreads - 1) / kThreads, static_cast<size_t>(ctx->sm_count) * 8));
+    repack_kernel<<<grid, kThreads, 0, ctx->stream>>>(src, stride, dst, dst_stride, rows, cols);
+    return check_launch("int8 repack launch");
+}
+
+template <typename T, typename Out>
+void launch_few_rows(BulletOuCudaCppContext* ctx, const FewRowsArgs& a) {
+    const int grid = std::min((a.p.n + kWarps - 1) / kWarps, ctx->sm_count * 4);
+    const size_t row = padded(a.p.k, 16);
+    if (a.p.m <= 1) few_rows_kernel<T, Out, 1><<<grid, kThreads, row, ctx->stream>>>(a);
+    else if (a.p.m <= 2) few_rows_kernel<T, Out, 2><<<grid, kThreads, 2 * row, ctx->stream>>>(a);
+    else few_rows_kernel<T, Out, kFewRows><<<grid, kThreads, kFewRows * row, ctx->stream>>>(a);
+}
+
+template <typename T>
+int few_rows(BulletOuCudaCppContext* ctx, const FewRowsArgs& a, int out_type) {
+    if (out_type == BULLETOU_B200_TYPE_F32) launch_few_rows<T, float>(ctx, a);
+    else launch_few_rows<T, __nv_bfloat16>(ctx, a);
+    return check_launch("int8 few-rows product launch");
+}
+
+// The product of `p`, of x's quantised rows where x is given (p.q and p.scales
+// are then filled in here).
+int product(BulletOuCudaCppContext* ctx, ProductArgs p, const BulletOuB200Matrix* x, int out_type) {
+    if (p.m <= kFewRows && kFewRows * padded(p.k, 16) <= kFewRowsBytes) {
+        FewRowsArgs a{};
+        a.p = p;
+        a.w_vector = tma_rows(p.w, p.n, p.w_stride);
+        if (x != nullptr) {
+            a.quantise = true;
+            a.x = x->data;
+            a.x_stride = x->row_stride;
+        }
+        if (x != nullptr && x->type == BULLETOU_B200_TYPE_BF16) return few_rows<__nv_bfloat16>(ctx, a, out_type);
+        return few_rows<float>(ctx, a, out_type);
+    }
+    const size_t pitch = std::max<size_t>(padded(p.k, 16), 16);
+    const bool own_q = x != nullptr || p.k == 0 || !tma_rows(p.q, p.m, p.q_stride);
+    const bool own_w = p.k == 0 || !tma_rows(p.w, p.n, p.w_stride);
+    const size_t scale_bytes = padded(static_cast<size_t>(p.m) * sizeof(float), 256);
+    const size_t q_bytes = own_q ? padded(p.m * pitch, 256) : 0;
+    void* scratch = nullptr;
+    if (scratch_slot(ctx, kScratchInt8, scale_bytes + q_bytes + (own_w ? p.n * pitch : 0), &scratch, "cudaMalloc int8 rows") != 0)
+        return -1;
+    float* const scales = static_cast<float*>(scratch);
+    int8_t* const q = static_cast<int8_t*>(scratch) + scale_bytes;
+    int8_t* const w = q + q_bytes;
+    if (own_w) {
+        if (p.k > 0 && repack(ctx, p.w, p.w_stride, w, pitch, p.n, p.k) != 0) return -1;
+        p.w = w;
+        p.w_stride = pitch;
+    }
+    if (x != nullptr) {
+        if (quantize(ctx, *x, q, pitch, static_cast<int>(pitch), scales) != 0) return -1;
+        p.scales = scales;
+    } else if (own_q && p.k > 0 && repack(ctx, p.q, p.q_stride, q, pitch, p.m, p.k) != 0) {
+        return -1;
+    }
+    if (own_q) {
+        p.q = q;
+        p.q_stride = pitch;
+    }
+    // a single row's stride is the caller's and may be anything
+    if (p.m == 1) p.q_stride = pitch;
+    if (p.n == 1) p.w_stride = pitch;
+    return launch_int8_mma(ctx, p, out_type, x != nullptr);
 }
 
 // The weight side's checks, shared by the two products.
@@ -200,7 +452,7 @@ int bulletou_b200_int8_matmul_device(BulletOuCudaCppContext* ctx, const BulletOu
     a.q = static_cast<const int8_t*>(q->data);
     a.q_stride = q->row_stride;
     a.scales = static_cast<const float*>(scales->data);
-    return product(ctx, a, out->type) != 0 ? -1 : ok();
+    return product(ctx, a, nullptr, out->type) != 0 ? -1 : ok();
 }
 
 int bulletou_b200_int8_linear_device(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix* x,
@@ -211,16 +463,7 @@ int bulletou_b200_int8_linear_device(BulletOuCudaCppContext* ctx, const BulletOu
         return -1;
     ProductArgs a = product_args(*weights, *weight_scales, bias, *out);
     if (a.m == 0 || a.n == 0) return ok();
-    a.q_stride = (static_cast<size_t>(a.k) + 15) / 16 * 16;
-    const size_t scale_bytes = (static_cast<size_t>(a.m) * sizeof(float) + 255) / 256 * 256;
-    void* p = nullptr;
-    if (scratch_slot(ctx, kScratchInt8, scale_bytes + a.m * a.q_stride, &p, "cudaMalloc int8 rows") != 0) return -1;
-    float* const scales = static_cast<float*>(p);
-    int8_t* const q = static_cast<int8_t*>(p) + scale_bytes;
-    a.scales = scales;
-    a.q = q;
-    if (quantize(ctx, *x, q, a.q_stride, static_cast<int>(a.q_stride), scales) != 0) return -1;
-    return product(ctx, a, out->type) != 0 ? -1 : ok();
+    return product(ctx, a, x, out->type) != 0 ? -1 : ok();
 }
 
 }  // extern "C"

@@ -1,0 +1,524 @@
+// The 8-bit product on the 5th-generation tensor cores (sm_100a):
+// tcgen05.mma.kind::i8, 8-bit operands from shared memory, 32-bit integer sums
+// in TMEM, so that every order of summation gives the same bits.
+//
+// Both operands are rows of k (K-major): a stage holds 128 bytes of k of each
+// row of the tile, loaded by TMA with 128-byte swizzle, and takes four MMAs of
+// 32 k.  Rows and k beyond the matrices are filled with zeros by the TMA.
+//
+// int8_pair_kernel, for large products: two CTAs of a cluster share a 256 x 256
+// tile (cta_group::2).  Each loads 128 rows of q and 128 of w -- half of what
+// two single CTAs would load for the same products, and what L2 can deliver
+// per SM is the limit of a 128 x 256 tile.  Persistent; the 512 TMEM columns
+// hold two accumulators, so a tile's epilogue runs under the next tile's MMAs.
+//
+// int8_tile_kernel, where there are too few 256 x 256 tiles for the SMs: one
+// 128 x TN tile for each CTA, with k cut over a cluster of up to four CTAs; the
+// partial integer sums meet through distributed shared memory.
+//
+// Every wait on an mbarrier is bounded (2 s); where one runs out the CTA's
+// remaining results are NaN.  No multicast loads.
+#include <algorithm>
+
+#include "int8_linear.cuh"
+#include "tensor_core.cuh"
+
+namespace bou {
+namespace {
+
+constexpr int kTileM = 128;                 // rows of q for each CTA (MMA M of one CTA)
+constexpr int kTileK = 128;                 // bytes of k in a stage: one swizzle atom
+constexpr uint32_t kABytes = kTileM * kTileK;
+constexpr int kStagePad = 4;                // floats between staged rows: 16-byte accesses without bank conflicts
+
+// Instruction descriptor, kind::i8: D s32 [4,6) = 2, A s8 [7,10) = 1, B s8
+// [10,13) = 1, both K-major, N >> 3 [17,23), M >> 4 [24,29).
+constexpr uint32_t int8_idesc(int m, int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n) >> 3 << 17) |
+           (static_cast<uint32_t>(m) >> 4 << 24);
+}
+
+// K-major with 128-byte swizzle: groups of 8 rows are 1024 bytes apart.
+__device__ __forceinline__ uint64_t k_major_desc(uint32_t addr) { return smem_desc(addr, 16u, 1024u); }
+
+template <int kGroup>
+__device__ __forceinline__ void mma_i8(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (kGroup == 1)
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+            " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(tmem),
+            "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+            " tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}" ::"r"(tmem),
+            "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
+}
+
+__device__ __forceinline__ void commit_one(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// Arrives on the barrier at this offset in both CTAs of the pair.
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int ld_cluster(uint32_t addr) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+// The load's bytes are counted on the barrier of the pair's first CTA.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
+        "[%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void wait_for_quantise() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// A warp writes 32 rows x 32 columns, one row in each lane: through shared
+// memory, so that the global stores cover whole rows of the block.
+template <typename Out>
+__device__ __forceinline__ void store_block(float* stage, const float* v, const ProductArgs& a, int row0, int col0,
+                                            bool vector_ok) {
+    constexpr int kCols = 32, kPitch = kCols + kStagePad;
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int c = 0; c < kCols; c += 4)
+        *reinterpret_cast<float4*>(stage + lane * kPitch + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+    __syncwarp();
+    Out* const out = static_cast<Out*>(a.out);
+    if (vector_ok && col0 + kCols <= a.n) {
+        constexpr int kVec = 16 / sizeof(Out);       // values of a 16-byte store
+        constexpr int kLanes = kCols / kVec;         // lanes of a row
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += 32 / kLanes) {
+            const int r = r0 + lane / kLanes, c = lane % kLanes * kVec;
+            if (row0 + r >= a.m) continue;
+            const float* src = stage + r * kPitch + c;
+            uint4 packed;
+            if constexpr (sizeof(Out) == 4) {
+                packed = *reinterpret_cast<const uint4*>(src);
+            } else {
+                uint32_t* p = reinterpret_cast<uint32_t*>(&packed);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const __nv_bfloat162 b = __floats2bfloat162_rn(src[2 * i], src[2 * i + 1]);
+                    p[i] = *reinterpret_cast<const uint32_t*>(&b);
+                }
+            }
+            *reinterpret_cast<uint4*>(out + static_cast<size_t>(row0 + r) * a.out_stride + col0 + c) = packed;
+        }
+    } else if (col0 + lane < a.n) {
+        for (int r = 0; r < 32 && row0 + r < a.m; ++r)
+            out[static_cast<size_t>(row0 + r) * a.out_stride + col0 + lane] = from_f32<Out>(stage[r * kPitch + lane]);
+    }
+    __syncwarp();
+}
+
+// ------------------------------------------------------------------ one tile for each CTA
+template <int TN>
+struct TileShape {
+    static constexpr uint32_t kStageBytes = kABytes + TN * kTileK;
+    static constexpr int kStages = TN == 64 ? 4 : 3;  // 96 KB: two CTAs on an SM
+    static constexpr int kThreads = 128;
+    static constexpr uint32_t kSmem = kStages * kStageBytes + 4 * 32 * (32 + kStagePad) * 4 + 2 * TN * 4 + 256 + 1024;
+};
+
+// `splits` CTAs of a cluster share a tile and cut k; the grid is their tiles,
+// the columns' tiles first.
+template <int TN, typename Out>
+__global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ CUtensorMap map_q,
+                                                        const __grid_constant__ CUtensorMap map_w, const ProductArgs a,
+                                                        int splits, bool vector_ok) {
+    using S = TileShape<TN>;
+    extern __shared__ uint8_t raw[];
+    const uint32_t raw_addr = smem_u32(raw);
+    const uint32_t base = (raw_addr + 1023u) & ~1023u;  // swizzle atoms
+    uint8_t* const stages = raw + (base - raw_addr);
+    float* const staging = reinterpret_cast<float*>(stages + S::kStages * S::kStageBytes);
+    float* const col_scale = staging + 4 * 32 * (32 + kStagePad);
+    float* const col_bias = col_scale + TN;
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(col_bias + TN);  // full, empty, done
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S::kStages + 1);
+    const uint32_t full = smem_u32(bars), empty = full + 8 * S::kStages, done = empty + 8 * S::kStages;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    const int rank = splits > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int tile = blockIdx.x / splits;
+    const int tiles_n = (a.n + TN - 1) / TN;
+    const int row0 = tile / tiles_n * kTileM, col0 = tile % tiles_n * TN;
+    const int blocks = (a.k + kTileK - 1) / kTileK;
+    const int share = (blocks + splits - 1) / splits;
+    const int k0 = min(blocks, rank * share), count = min(blocks, k0 + share) - k0;
+
+    if (tid == 0) {
+        for (int s = 0; s < S::kStages; ++s) {
+            mbar_init(full + 8 * s, 1);
+            mbar_init(empty + 8 * s, 1);
+        }
+        mbar_init(done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(static_cast<uint32_t>(TN))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    for (int c = tid; c < TN; c += S::kThreads) {
+        const bool in = col0 + c < a.n;
+        col_scale[c] = in ? a.w_scales[col0 + c] : 0.0f;
+        col_bias[c] = in && a.bias != nullptr ? a.bias[col0 + c] : 0.0f;
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0 && lane == 0) {
+        // the weights of the first stages come while the rows are still being quantised
+        const int ahead = min(count, S::kStages);
+        for (int i = 0; i < ahead; ++i) {
+            mbar_expect_tx(full + 8 * i, S::kStageBytes);
+            tma_load_2d(base + i * S::kStageBytes + kABytes, &map_w, (k0 + i) * kTileK, col0, full + 8 * i);
+        }
+        wait_for_quantise();
+        for (int i = 0; i < ahead; ++i) tma_load_2d(base + i * S::kStageBytes, &map_q, (k0 + i) * kTileK, row0, full + 8 * i);
+        for (int i = ahead; i < count; ++i) {
+            const int s = i % S::kStages;
+            if (!mbar_wait(empty + 8 * s, (i / S::kStages - 1) & 1)) break;
+            mbar_expect_tx(full + 8 * s, S::kStageBytes);
+            tma_load_2d(base + s * S::kStageBytes, &map_q, (k0 + i) * kTileK, row0, full + 8 * s);
+            tma_load_2d(base + s * S::kStageBytes + kABytes, &map_w, (k0 + i) * kTileK, col0, full + 8 * s);
+        }
+    } else if (warp == 1 && lane == 0) {
+        bool good = true;
+        for (int i = 0; i < count && good; ++i) {
+            const int s = i % S::kStages;
+            good = mbar_wait(full + 8 * s, (i / S::kStages) & 1);
+            if (!good) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t qa = base + s * S::kStageBytes, wa = qa + kABytes;
+#pragma unroll
+            for (int j = 0; j < kTileK / 32; ++j)
+                mma_i8<1>(tmem, k_major_desc(qa + 32 * j), k_major_desc(wa + 32 * j), int8_idesc(kTileM, TN),
+                          (i | j) != 0 ? 1u : 0u);
+            commit_one(empty + 8 * s);
+        }
+        if (good && count > 0) commit_one(done);
+    }
+    __syncwarp();
+    const bool good = count == 0 || mbar_wait(done, 0);
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    wait_for_quantise();  // the scales
+    float* const stage = staging + warp * 32 * (32 + kStagePad);
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    if (splits == 1) {
+        const int row = row0 + warp * 32 + lane;
+        const float row_scale = row < a.m ? (good ? a.scales[row] : NAN) : 0.0f;
+#pragma unroll 1
+        for (int c0 = 0; c0 < TN && col0 + c0 < a.n; c0 += 32) {
+            uint32_t sum[32];
+            float v[32];
+            tmem_ld32(lanes + c0, sum);
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+                v[c] = int8_result(count > 0 ? static_cast<int>(sum[c]) : 0, row_scale, col_scale[c0 + c], col_bias[c0 + c]);
+            store_block<Out>(stage, v, a, row0 + warp * 32, col0 + c0, vector_ok);
+        }
+    } else {
+        // partial sums as [column][row], over the stages that are no longer needed
+        int* const part = reinterpret_cast<int*>(stages);
+#pragma unroll 1
+        for (int c0 = 0; c0 < TN; c0 += 32) {
+            uint32_t sum[32];
+            tmem_ld32(lanes + c0, sum);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) part[(c0 + c) * kTileM + warp * 32 + lane] = count > 0 ? static_cast<int>(sum[c]) : 0;
+        }
+        int* const failed = reinterpret_cast<int*>(tmem_slot + 1);
+        if (tid == 0) *failed = 0;
+        __syncthreads();
+        if (!good) *failed = 1;
+        cluster_sync();
+        // the tile's 4 row groups x TN / 32 column groups, dealt out over the cluster's warps
+        const uint32_t mine = smem_u32(part), flag = smem_u32(failed);
+        for (int job = rank * 4 + warp; job < 4 * (TN / 32); job += 4 * splits) {
+            const int group = job & 3, c0 = (job >> 2) * 32;
+            const int row = row0 + group * 32 + lane;
+            if (row0 + group * 32 >= a.m || col0 + c0 >= a.n) continue;
+            int sum[32] = {};
+            bool broken = false;
+            for (int r = 0; r < splits; ++r) {
+                const uint32_t from = map_rank(mine, r);
+                broken |= ld_cluster(map_rank(flag, r)) != 0;
+#pragma unroll
+                for (int c = 0; c < 32; ++c) sum[c] += ld_cluster(from + ((c0 + c) * kTileM + group * 32 + lane) * 4);
+            }
+            const float row_scale = row < a.m ? (broken ? NAN : a.scales[row]) : 0.0f;
+            float v[32];
+#pragma unroll
+            for (int c = 0; c < 32; ++c) v[c] = int8_result(sum[c], row_scale, col_scale[c0 + c], col_bias[c0 + c]);
+            store_block<Out>(stage, v, a, row0 + group * 32, col0 + c0, vector_ok);
+        }
+        cluster_sync();  // no CTA leaves while another reads its sums
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (!good && tid == 0)  // copies in flight end before the memory is given back
+        for (int s = 0; s < min(count, S::kStages); ++s) mbar_wait(full + 8 * s, ((count - 1 - s) / S::kStages) & 1);
+    __syncthreads();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(static_cast<uint32_t>(TN))
+                     : "memory");
+}
+
+// ------------------------------------------------------------------ a pair of CTAs on 256 x 256 tiles
+constexpr int kPairN = 256;
+constexpr int kPairStages = 6;
+constexpr uint32_t kPairStageBytes = 2 * kABytes;  // 128 rows of q, 128 rows of w
+constexpr int kPairThreads = 192;                  // TMA, MMA, 4 x epilogue
+constexpr int kGroupM = 8;                         // tiles of rows that run next to one another, for L2
+constexpr uint32_t kPairSmem = kPairStages * kPairStageBytes + 4 * 32 * (32 + kStagePad) * 4 + 2 * kPairN * 4 + 256 + 1024;
+
+template <typename Out>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    int8_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_w,
+                     const ProductArgs a, bool vector_ok) {
+    extern __shared__ uint8_t raw[];
+    const uint32_t raw_addr = smem_u32(raw);
+    const uint32_t base = (raw_addr + 1023u) & ~1023u;
+    uint8_t* const stages = raw + (base - raw_addr);
+    float* const staging = reinterpret_cast<float*>(stages + kPairStages * kPairStageBytes);
+    float* const col_scale = staging + 4 * 32 * (32 + kStagePad);
+    float* const col_bias = col_scale + kPairN;
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(col_bias + kPairN);
+    const uint32_t full = smem_u32(bars), empty = full + 8 * kPairStages, tile_full = empty + 8 * kPairStages,
+                   tile_empty = tile_full + 16;
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kPairStages + 4);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = cluster_rank();
+
+    if (tid == 0) {
+        for (int s = 0; s < kPairStages; ++s) {
+            mbar_init(full + 8 * s, 1);
+            mbar_init(empty + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(tile_full + 8 * b, 1);
+            mbar_init(tile_empty + 8 * b, 8);  // 4 epilogue warps in each CTA
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(2u * kPairN)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    wait_for_quantise();
+
+    const int tiles_m = (a.m + 2 * kTileM - 1) / (2 * kTileM), tiles_n = (a.n + kPairN - 1) / kPairN;
+    const int tiles = tiles_m * tiles_n;
+    const int blocks = (a.k + kTileK - 1) / kTileK;
+    auto place = [&](int t, int& row0, int& col0) {
+        const int group = t / (kGroupM * tiles_n);
+        const int first = group * kGroupM, height = min(kGroupM, tiles_m - first);
+        const int in = t - group * kGroupM * tiles_n;
+        row0 = (first + in % height) * 2 * kTileM + static_cast<int>(rank) * kTileM;
+        col0 = in / height * kPairN;
+    };
+    const int first_tile = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+    if (warp == 0 && lane == 0) {
+        int i = 0;
+        bool good = true;
+        for (int t = first_tile; t < tiles && good; t += step) {
+            int row0, col0;
+            place(t, row0, col0);
+            for (int kb = 0; kb < blocks; ++kb, ++i) {
+                const int s = i % kPairStages;
+                if (i >= kPairStages && !(good = mbar_wait(empty + 8 * s, (i / kPairStages - 1) & 1))) break;
+                if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * kPairStageBytes);
+                const uint32_t bar = map_rank(full + 8 * s, 0), dst = base + s * kPairStageBytes;
+                tma_load_pair(dst, &map_q, kb * kTileK, row0, bar);
+                tma_load_pair(dst + kABytes, &map_w, kb * kTileK, col0 + static_cast<int>(rank) * kTileM, bar);
+            }
+        }
+        // without a failure every copy was consumed; after one the last of each stage is waited for
+        if (!good && rank == 0)
+            for (int j = max(0, i - kPairStages); j < i; ++j) mbar_wait(full + 8 * (j % kPairStages), (j / kPairStages) & 1);
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        int i = 0;
+        bool good = true;
+        for (int t = first_tile, n = 0; t < tiles && good; t += step, ++n) {
+            const int b = n & 1;
+            if (n >= 2 && !(good = mbar_wait(tile_empty + 8 * b, (n / 2 - 1) & 1))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (int kb = 0; kb < blocks; ++kb, ++i) {
+                const int s = i % kPairStages;
+                if (!(good = mbar_wait(full + 8 * s, (i / kPairStages) & 1))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t qa = base + s * kPairStageBytes, wa = qa + kABytes;
+#pragma unroll
+                for (int j = 0; j < kTileK / 32; ++j)
+                    mma_i8<2>(tmem + b * kPairN, k_major_desc(qa + 32 * j), k_major_desc(wa + 32 * j),
+                              int8_idesc(2 * kTileM, kPairN), (kb | j) != 0 ? 1u : 0u);
+                commit_pair(empty + 8 * s);
+            }
+            if (good) commit_pair(tile_full + 8 * b);
+        }
+    } else if (warp >= 2) {
+        const int quarter = warp & 3;  // the TMEM lanes this warp may read
+        float* const stage = staging + quarter * 32 * (32 + kStagePad);
+        bool good = true;
+        for (int t = first_tile, n = 0; t < tiles; t += step, ++n) {
+            const int b = n & 1;
+            int row0, col0;
+            place(t, row0, col0);
+            asm volatile("bar.sync 1, 128;" ::: "memory");  // the last tile's scales are read
+            for (int c = tid - 64; c < kPairN; c += 128) {
+                const bool in = col0 + c < a.n;
+                col_scale[c] = in ? a.w_scales[col0 + c] : 0.0f;
+                col_bias[c] = in && a.bias != nullptr ? a.bias[col0 + c] : 0.0f;
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            const int row = row0 + quarter * 32 + lane;
+            good = good && mbar_wait(tile_full + 8 * b, (n / 2) & 1);
+            good = __all_sync(0xffffffffu, good);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const float row_scale = row < a.m ? (good ? a.scales[row] : NAN) : 0.0f;
+            const uint32_t lanes = tmem + b * kPairN + (static_cast<uint32_t>(quarter * 32) << 16);
+#pragma unroll 1
+            for (int c0 = 0; c0 < kPairN && col0 + c0 < a.n; c0 += 32) {
+                uint32_t sum[32];
+                float v[32];
+                tmem_ld32(lanes + c0, sum);
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                    v[c] = int8_result(static_cast<int>(sum[c]), row_scale, col_scale[c0 + c], col_bias[c0 + c]);
+                store_block<Out>(stage, v, a, row0 + quarter * 32, col0 + c0, vector_ok);
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0)
+                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                                 map_rank(tile_empty + 8 * b, 0))
+                             : "memory");
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    cluster_sync();  // neither CTA leaves while the other's copies, MMAs or arrivals reach it
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2u * kPairN) : "memory");
+}
+
+// ------------------------------------------------------------------ host
+// rows x k bytes in boxes of box_rows x 128 bytes.
+int operand_map(CUtensorMap* map, const int8_t* data, int rows, int k, size_t stride, int box_rows) {
+    const EncodeTiled fn = encode_tiled();
+    if (fn == nullptr) return fail_message("cuTensorMapEncodeTiled is unavailable");
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride)};
+    const cuuint32_t box[2] = {kTileK, static_cast<cuuint32_t>(box_rows)};
+    const cuuint32_t estride[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(data), dims, strides, box, estride,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail_messagef("cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+    return 0;
+}
+
+template <typename Kernel, typename... Args>
+int launch(BulletOuCudaCppContext* ctx, Kernel kernel, int grid, int threads, size_t smem, int cluster, bool early,
+           Args... args) {
+    cudaError_t st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (st != cudaSuccess) return fail("cudaFuncSetAttribute int8 product", st);
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = smem;
+    config.stream = ctx->stream;
+    cudaLaunchAttribute attrs[2];
+    config.attrs = attrs;
+    if (cluster > 1) {
+        attrs[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attrs[config.numAttrs++].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
+    }
+    if (early) {
+        attrs[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attrs[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    st = cudaLaunchKernelEx(&config, kernel, args...);
+    return st != cudaSuccess ? fail("int8 product launch", st) : 0;
+}
+
+template <int TN, typename Out>
+int launch_tiles(BulletOuCudaCppContext* ctx, const ProductArgs& a, bool vector_ok, bool early) {
+    const int64_t tiles = static_cast<int64_t>((a.m + kTileM - 1) / kTileM) * ((a.n + TN - 1) / TN);
+    const int blocks = (a.k + kTileK - 1) / kTileK;
+    int splits = 1;
+    while (splits < 4 && tiles * splits * 2 <= ctx->sm_count && blocks >= 4 * splits) splits *= 2;
+    if (tiles * splits > INT32_MAX) return fail_messagef("int8 product: %d x %d results are too many", a.m, a.n);
+    CUtensorMap q, w;
+    if (operand_map(&q, a.q, a.m, a.k, a.q_stride, kTileM) != 0 || operand_map(&w, a.w, a.n, a.k, a.w_stride, TN) != 0)
+        return -1;
+    return launch(ctx, int8_tile_kernel<TN, Out>, static_cast<int>(tiles * splits), 128, TileShape<TN>::kSmem, splits,
+                  early, q, w, a, splits, vector_ok);
+}
+
+template <typename Out>
+int launch_pairs(BulletOuCudaCppContext* ctx, const ProductArgs& a, int tiles, bool vector_ok, bool early) {
+    CUtensorMap q, w;
+    if (operand_map(&q, a.q, a.m, a.k, a.q_stride, kTileM) != 0 || operand_map(&w, a.w, a.n, a.k, a.w_stride, kTileM) != 0)
+        return -1;
+    const int grid = 2 * std::min(tiles, ctx->sm_count / 2);
+    return launch(ctx, int8_pair_kernel<Out>, grid, kPairThreads, kPairSmem, 2, early, q, w, a, vector_ok);
+}
+
+template <typename Out>
+int launch_typed(BulletOuCudaCppContext* ctx, const ProductArgs& a, bool early) {
+    const bool vector_ok = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && (a.m <= 1 || a.out_stride * sizeof(Out) % 16 == 0);
+    const int64_t pairs = static_cast<int64_t>((a.m + 255) / 256) * ((a.n + 255) / 256);
+    if (pairs >= ctx->sm_count / 2 && pairs <= INT32_MAX)
+        return launch_pairs<Out>(ctx, a, static_cast<int>(pairs), vector_ok, early);
+    const int64_t wide = static_cast<int64_t>((a.m + 127) / 128) * ((a.n + 127) / 128);
+    return wide >= ctx->sm_count ? launch_tiles<128, Out>(ctx, a, vector_ok, early)
+                                 : launch_tiles<64, Out>(ctx, a, vector_ok, early);
+}
+
+}  // namespace
+
+int launch_int8_mma(BulletOuCudaCppContext* ctx, const ProductArgs& a, int out_type, bool after_quantise) {
+    return out_type == BULLETOU_B200_TYPE_F32 ? launch_typed<float>(ctx, a, after_quantise)
+                                              : launch_typed<__nv_bfloat16>(ctx, a, after_quantise);
+}
+
+}  // namespace bou

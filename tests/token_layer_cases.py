@@ -126,7 +126,7 @@ def quantize_rows(x):
 
 def int8_product(q, scales, w, w_scales, bias):
     """The product, and the magnitude its roundings scale with."""
-    acc = q.astype(np.int64) @ w.astype(np.int64).T
+    acc = q.astype(np.float64) @ w.astype(np.float64).T  # exact: below 2^53
     y = acc * scales.astype(np.float64)[:, None] * w_scales.astype(np.float64)
     size = np.abs(y)
     if bias is not None:
