@@ -3,24 +3,21 @@
 //   out[n] = scale * table[t_n]            (zeros where t_n is outside the table)
 //   table_gradients[v] = scale * sum over n with t_n = v of out_gradients[n]
 //
-// The gradient sorts the tokens (stable, so each row's entries keep their
-// order) and sums the rows of equal tokens in that order: no floating atomics,
-// the same bits from call to call.  The sort is a least-significant-digit
-// radix sort of (token, position) with tokens outside the table as the largest
-// key.
+// Both are bound by the rows' bytes.  The lookup is one pass with several rows
+// in flight for each warp.  The gradient sorts the tokens (stable, so each
+// row's entries keep their order) and then sums runs of equal tokens in that
+// order: no floating atomics, the same bits from call to call, every row of
+// out_gradients read once and every row of the table written once.
 #include <algorithm>
 
 #include "device_matrix.cuh"
+#include "token_launch.cuh"
 
 namespace bou {
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMaxDigitBits = 9;
-constexpr int kMaxBins = 1 << kMaxDigitBits;
-constexpr int kTile = 2048;  // keys of one CTA
-constexpr int kKeysPerWarp = kTile / kWarps;
 
 // Tokens in row-major order; those outside [0, vocab) become vocab.
 struct Tokens {
@@ -40,6 +37,54 @@ struct Tokens {
     }
 };
 
+// kUnit elements that are loaded or stored together: 16 bytes of the narrower
+// type where the rows allow it, else one element.
+template <typename T, int kUnit>
+__device__ __forceinline__ void load_unit(const T* p, float* v) {
+    if constexpr (kUnit == 1) {
+        v[0] = to_f32(*p);
+    } else {
+        constexpr int kWords = kUnit * sizeof(T) / 4;
+        uint32_t raw[kWords];
+        if constexpr (kWords == 2) {
+            const uint2 u = *reinterpret_cast<const uint2*>(p);
+            raw[0] = u.x, raw[1] = u.y;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4) {
+                const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p) + 4 * i);
+                raw[i] = u.x, raw[i + 1] = u.y, raw[i + 2] = u.z, raw[i + 3] = u.w;
+            }
+        }
+        const T* e = reinterpret_cast<const T*>(raw);
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i) v[i] = to_f32(e[i]);
+    }
+}
+template <typename T, int kUnit>
+__device__ __forceinline__ void store_unit(T* p, const float* v) {
+    if constexpr (kUnit == 1) {
+        *p = from_f32<T>(v[0]);
+    } else {
+        constexpr int kWords = kUnit * sizeof(T) / 4;
+        uint32_t raw[kWords];
+        T* e = reinterpret_cast<T*>(raw);
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i) e[i] = from_f32<T>(v[i]);
+        if constexpr (kWords == 2) {
+            __stcs(reinterpret_cast<uint2*>(p), make_uint2(raw[0], raw[1]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4)
+                __stcs(reinterpret_cast<uint4*>(reinterpret_cast<char*>(p) + 4 * i),
+                       make_uint4(raw[i], raw[i + 1], raw[i + 2], raw[i + 3]));
+        }
+    }
+}
+// The vector unit of a pair of types: 8 bf16 or 4 f32 fill 16 bytes.
+template <typename A, typename B>
+constexpr int kVectorUnit = sizeof(A) == 2 && sizeof(B) == 2 ? 8 : 4;
+
 // ------------------------------------------------------------------ lookup
 struct LookupArgs {
     Tokens tokens;
@@ -50,21 +95,55 @@ struct LookupArgs {
     float scale;
 };
 
-template <typename In, typename Out>
-__global__ void __launch_bounds__(kThreads) lookup_kernel(const LookupArgs a) {
-    const size_t n = static_cast<size_t>(a.tokens.n) * a.width;
-    for (size_t i = static_cast<size_t>(blockIdx.x) * kThreads + threadIdx.x; i < n;
-         i += static_cast<size_t>(gridDim.x) * kThreads) {
-        const int row = static_cast<int>(i / a.width);
-        const int col = static_cast<int>(i - static_cast<size_t>(row) * a.width);
-        const int t = a.tokens(row);
-        float v = 0.0f;
-        if (t < a.tokens.vocab) v = to_f32(static_cast<const In*>(a.table)[t * a.table_stride + col]) * a.scale;
-        static_cast<Out*>(a.out)[row * a.out_stride + col] = from_f32<Out>(v);
+// A group of 2^k lanes, enough for a row's units, takes kRows rows at a time, so
+// that kRows loads of each lane are in flight behind the kRows tokens.  The
+// stores stream past L2, which keeps the table.
+template <typename In, typename Out, int kUnit>
+__global__ void __launch_bounds__(kThreads) lookup_kernel(const LookupArgs a, int group) {
+    constexpr int kRows = 4;
+    const int lane = threadIdx.x & (group - 1);
+    const int units = a.width / kUnit;
+    const int64_t groups = static_cast<int64_t>(gridDim.x) * (kThreads / group);
+    const int64_t first = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / group;
+    for (int64_t r0 = first; r0 < a.tokens.n; r0 += groups * kRows) {
+        int token[kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const int64_t r = r0 + i * groups;
+            token[i] = r < a.tokens.n ? a.tokens(static_cast<int>(r)) : a.tokens.vocab;
+        }
+        for (int u = lane; u < units; u += group) {
+            float v[kRows][kUnit];
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                if (token[i] < a.tokens.vocab) {
+                    load_unit<In, kUnit>(static_cast<const In*>(a.table) + token[i] * a.table_stride + u * kUnit, v[i]);
+#pragma unroll
+                    for (int j = 0; j < kUnit; ++j) v[i][j] *= a.scale;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < kUnit; ++j) v[i][j] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                const int64_t r = r0 + i * groups;
+                if (r < a.tokens.n)
+                    store_unit<Out, kUnit>(static_cast<Out*>(a.out) + r * a.out_stride + u * kUnit, v[i]);
+            }
+        }
     }
 }
 
 // ------------------------------------------------------------------ sort
+// Least-significant-digit radix sort of (token, position), tokens outside the
+// table as the largest key.  Digits of up to 11 bits: fewer passes save three
+// launches each, which is what a sort of 10^5 tokens costs, and 2048 counters
+// for each of 8 warps still fit the shared memory twice.
+constexpr int kMaxDigitBits = 11;
+constexpr int kMaxBins = 1 << kMaxDigitBits;
+constexpr int kMaxTile = 2048;
+
 struct SortPass {
     Tokens tokens;           // keys of the first pass
     const int* keys_in;      // null: the tokens themselves, at positions 0..n-1
@@ -74,16 +153,19 @@ struct SortPass {
     int* counts;             // [bins][tiles], turned into starts inside a bin
     int* totals;             // [bins]
     int n, tiles, shift, bins;
+    int tile;                // keys of one CTA, a multiple of 32 * kWarps
     __device__ __forceinline__ int key(int i) const { return keys_in != nullptr ? keys_in[i] : tokens(i); }
     __device__ __forceinline__ int digit(int k) const { return (k >> shift) & (bins - 1); }
 };
 
 __global__ void __launch_bounds__(kThreads) sort_count_kernel(const SortPass s) {
     __shared__ int count[kMaxBins];
+    let_next_start();
+    wait_for_previous();
     for (int b = threadIdx.x; b < s.bins; b += kThreads) count[b] = 0;
     __syncthreads();
-    const int first = blockIdx.x * kTile;
-    for (int i = first + threadIdx.x; i < min(s.n, first + kTile); i += kThreads) atomicAdd(count + s.digit(s.key(i)), 1);
+    const int first = blockIdx.x * s.tile;
+    for (int i = first + threadIdx.x; i < min(s.n, first + s.tile); i += kThreads) atomicAdd(count + s.digit(s.key(i)), 1);
     __syncthreads();
     for (int b = threadIdx.x; b < s.bins; b += kThreads) s.counts[static_cast<size_t>(b) * s.tiles + blockIdx.x] = count[b];
 }
@@ -112,6 +194,8 @@ __device__ __forceinline__ int block_exclusive(int v, int* warp_sums, int* total
 // CTA per bin: where each tile's keys of the bin start inside the bin.
 __global__ void __launch_bounds__(kThreads) sort_scan_kernel(const SortPass s) {
     __shared__ int warp_sums[kWarps];
+    let_next_start();
+    wait_for_previous();
     int* counts = s.counts + static_cast<size_t>(blockIdx.x) * s.tiles;
     int run = 0;
     for (int t0 = 0; t0 < s.tiles; t0 += kThreads) {
@@ -128,14 +212,18 @@ __global__ void __launch_bounds__(kThreads) sort_scan_kernel(const SortPass s) {
 // of its bin, its tile's start in the bin, the keys of earlier warps and steps,
 // and its rank among the equal digits of its warp's step.
 __global__ void __launch_bounds__(kThreads) sort_scatter_kernel(const SortPass s) {
-    __shared__ int place[kWarps][kMaxBins];
+    extern __shared__ int places[];  // [kWarps][bins]
     __shared__ int warp_sums[kWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int i = threadIdx.x; i < kWarps * kMaxBins; i += kThreads) place[0][i] = 0;
+    int* const place = places + warp * s.bins;
+    let_next_start();
+    for (int i = threadIdx.x; i < kWarps * s.bins; i += kThreads) places[i] = 0;
     __syncthreads();
-    const int first = blockIdx.x * kTile + warp * kKeysPerWarp;
-    const int end = min(s.n, first + kKeysPerWarp);
-    for (int i = first + lane; i < end; i += 32) atomicAdd(&place[warp][s.digit(s.key(i))], 1);
+    wait_for_previous();
+    const int per_warp = s.tile / kWarps;
+    const int first = blockIdx.x * s.tile + warp * per_warp;
+    const int end = min(s.n, first + per_warp);
+    for (int i = first + lane; i < end; i += 32) atomicAdd(place + s.digit(s.key(i)), 1);
     __syncthreads();
     int run = 0;
     for (int b0 = 0; b0 < s.bins; b0 += kThreads) {
@@ -146,8 +234,8 @@ __global__ void __launch_bounds__(kThreads) sort_scatter_kernel(const SortPass s
         if (b < s.bins) {
             at += s.counts[static_cast<size_t>(b) * s.tiles + blockIdx.x];
             for (int w = 0; w < kWarps; ++w) {
-                const int c = place[w][b];
-                place[w][b] = at;
+                const int c = places[w * s.bins + b];
+                places[w * s.bins + b] = at;
                 at += c;
             }
         }
@@ -160,28 +248,38 @@ __global__ void __launch_bounds__(kThreads) sort_scatter_kernel(const SortPass s
             const int k = s.key(i);
             const int d = s.digit(k);
             const unsigned peers = __match_any_sync(active, d);
-            const int start = place[warp][d];
+            const int start = place[d];
             const int at = start + __popc(peers & ((1u << lane) - 1));
             s.keys_out[at] = k;
             s.positions_out[at] = s.positions_in != nullptr ? s.positions_in[i] : i;
             __syncwarp(active);  // every lane has read `start`
-            if (lane == 31 - __clz(peers)) place[warp][d] = start + __popc(peers);
+            if (lane == 31 - __clz(peers)) place[d] = start + __popc(peers);
         }
         __syncwarp();
     }
 }
 
 // ------------------------------------------------------------------ gradient
+// The sorted entries are cut into chunks of equal length, so that a token that
+// half of the entries name costs no more than the others.  A group of lanes
+// sums its chunk's runs of equal tokens in order.  A run inside the chunk is a
+// row's gradient and is written; a run that goes on beyond the chunk leaves a
+// partial row, and joined_rows_kernel adds those up in the order of the chunks.
 struct GradientArgs {
     const int* keys;       // sorted
     const int* positions;
-    int n;
+    int n, chunk, chunks;
     const void* grad;
     void* out;
     int vocab, width;
     size_t grad_stride, out_stride;
     float scale;
+    float* heads;          // [chunks][width]: the chunk's first run, begun before it
+    float* tails;          // [chunks][width]: the run that begins in the chunk and goes on after it
+    int row_blocks;        // CTAs that write the rows no token names
 };
+
+constexpr int kEmptyRows = 128;  // table rows of one such CTA
 
 // First place in the sorted keys whose key is not below `v`.
 __device__ __forceinline__ int lower_bound(const int* keys, int n, int v) {
@@ -194,18 +292,181 @@ __device__ __forceinline__ int lower_bound(const int* keys, int n, int v) {
     return lo;
 }
 
-// CTA per table row: its entries summed in order, a thread per column.
-template <typename In, typename Out>
-__global__ void __launch_bounds__(kThreads) gradient_kernel(const GradientArgs a) {
-    __shared__ int range[2];
-    const int v = blockIdx.x;
-    if (threadIdx.x < 2) range[threadIdx.x] = lower_bound(a.keys, a.n, v + threadIdx.x);
+template <typename Out, int kUnit>
+__device__ void write_empty_rows(const GradientArgs& a, int block) {
+    __shared__ int empty[kEmptyRows];
+    const int64_t v0 = static_cast<int64_t>(block) * kEmptyRows;
+    if (threadIdx.x < kEmptyRows) {
+        const int64_t v = v0 + threadIdx.x;
+        bool none = false;
+        if (v < a.vocab) {
+            const int at = lower_bound(a.keys, a.n, static_cast<int>(v));
+            none = at == a.n || a.keys[at] != v;
+        }
+        empty[threadIdx.x] = none;
+    }
     __syncthreads();
-    for (int c = threadIdx.x; c < a.width; c += kThreads) {
-        float sum = 0.0f;
-        for (int i = range[0]; i < range[1]; ++i)
-            sum += to_f32(static_cast<const In*>(a.grad)[a.positions[i] * a.grad_stride + c]);
-        static_cast<Out*>(a.out)[v * a.out_stride + c] = from_f32<Out>(sum * a.scale);
+    const float zeros[kUnit] = {};
+    for (int r = threadIdx.x >> 5; r < kEmptyRows; r += kWarps) {
+        if (!empty[r]) continue;
+        Out* out = static_cast<Out*>(a.out) + (v0 + r) * a.out_stride;
+        for (int u = threadIdx.x & 31; u < a.width / kUnit; u += 32) store_unit<Out, kUnit>(out + u * kUnit, zeros);
+    }
+}
+
+// kLanes lanes hold kUnits units of a row each; blockIdx.y cuts wider rows.
+template <typename In, typename Out, int kUnit, int kLanes, int kUnits>
+__global__ void __launch_bounds__(kThreads) gradient_kernel(const GradientArgs a) {
+    constexpr int kBatch = kUnit * kUnits > 8 ? 4 : 8;  // rows in flight
+    let_next_start();
+    wait_for_previous();
+    if (static_cast<int>(blockIdx.x) < a.row_blocks) {
+        if (blockIdx.y == 0) write_empty_rows<Out, kUnit>(a, blockIdx.x);
+        return;
+    }
+    const int c = (blockIdx.x - a.row_blocks) * (kThreads / kLanes) + threadIdx.x / kLanes;
+    if (c >= a.chunks) return;
+    const int lane = threadIdx.x & (kLanes - 1);
+    const int units = a.width / kUnit;
+    const int u0 = blockIdx.y * kLanes * kUnits + lane;
+    const int begin = c * a.chunk, end = min(a.n, begin + a.chunk);
+    const int before = begin > 0 ? a.keys[begin - 1] : -1, after = end < a.n ? a.keys[end] : -1;
+    float sum[kUnits][kUnit] = {};
+    int current = a.keys[begin];
+    bool from_before = current == before;
+    auto flush = [&](bool goes_on) {
+        if (current < a.vocab) {
+            float* part = from_before ? a.heads : goes_on ? a.tails : nullptr;
+#pragma unroll
+            for (int k = 0; k < kUnits; ++k) {
+                const int u = u0 + k * kLanes;
+                if (u >= units) continue;
+                if (part != nullptr) {
+#pragma unroll
+                    for (int j = 0; j < kUnit; ++j) part[static_cast<size_t>(c) * a.width + u * kUnit + j] = sum[k][j];
+                } else {
+                    float v[kUnit];
+#pragma unroll
+                    for (int j = 0; j < kUnit; ++j) v[j] = sum[k][j] * a.scale;
+                    store_unit<Out, kUnit>(static_cast<Out*>(a.out) + current * a.out_stride + u * kUnit, v);
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k)
+#pragma unroll
+            for (int j = 0; j < kUnit; ++j) sum[k][j] = 0.0f;
+    };
+    int key[kBatch], position[kBatch];
+    auto fetch = [&](int i0) {
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const bool in = i0 + b < end;
+            key[b] = in ? a.keys[i0 + b] : a.vocab;
+            position[b] = in ? a.positions[i0 + b] : 0;
+        }
+    };
+    fetch(begin);
+    for (int i0 = begin; i0 < end; i0 += kBatch) {
+        float v[kBatch][kUnits][kUnit];
+        int k_now[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            k_now[b] = key[b];
+            const In* row = static_cast<const In*>(a.grad) + position[b] * a.grad_stride;
+#pragma unroll
+            for (int k = 0; k < kUnits; ++k) {
+                const int u = u0 + k * kLanes;
+                if (key[b] < a.vocab && u < units) {
+                    load_unit<In, kUnit>(row + u * kUnit, v[b][k]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < kUnit; ++j) v[b][k][j] = 0.0f;
+                }
+            }
+        }
+        fetch(i0 + kBatch);
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            if (i0 + b >= end) break;
+            if (k_now[b] != current) {
+                flush(false);
+                current = k_now[b];
+                from_before = false;
+            }
+#pragma unroll
+            for (int k = 0; k < kUnits; ++k)
+#pragma unroll
+                for (int j = 0; j < kUnit; ++j) sum[k][j] += v[b][k][j];
+        }
+    }
+    flush(current == after);
+}
+
+// CTA for kWarps chunks: the rows whose run begins in a chunk and goes on after
+// it.  Runs over up to kShortRun more chunks take a warp each; longer ones are
+// shared by the CTA's warps, each a run of consecutive chunks, and joined in
+// that order.
+template <typename Out>
+__global__ void __launch_bounds__(kThreads) joined_rows_kernel(const GradientArgs a) {
+    constexpr int kShortRun = 16;
+    __shared__ int first_key[kWarps], more[kWarps];  // of each chunk's tail run: its row, the chunks after it
+    __shared__ float part[kWarps][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    wait_for_previous();
+    const int c0 = blockIdx.x * kWarps;
+    if (threadIdx.x < kWarps) {
+        const int c = c0 + threadIdx.x;
+        int row = -1, count = 0;
+        if (c + 1 < a.chunks) {
+            const int begin = c * a.chunk, last = begin + a.chunk - 1;
+            const int k = a.keys[last];
+            const bool begun_here = !(begin > 0 && a.keys[begin] == k && a.keys[begin - 1] == k);
+            if (k < a.vocab && a.keys[last + 1] == k && begun_here) {
+                row = k;
+                // the chunk that holds the run's last entry
+                count = (lower_bound(a.keys, a.n, k + 1) - 1) / a.chunk - c;
+            }
+        }
+        first_key[threadIdx.x] = row;
+        more[threadIdx.x] = count;
+    }
+    __syncthreads();
+    auto sum_heads = [&](int first, int count, int column) {
+        float s = 0.0f;
+        int i = 0;
+        for (; i + 8 <= count; i += 8) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = a.heads[static_cast<size_t>(first + i + j) * a.width + column];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s += v[j];
+        }
+        for (; i < count; ++i) s += a.heads[static_cast<size_t>(first + i) * a.width + column];
+        return s;
+    };
+    if (first_key[warp] >= 0 && more[warp] <= kShortRun) {
+        const int c = c0 + warp;
+        for (int column = lane; column < a.width; column += 32) {
+            const float s = a.tails[static_cast<size_t>(c) * a.width + column] + sum_heads(c + 1, more[warp], column);
+            static_cast<Out*>(a.out)[first_key[warp] * a.out_stride + column] = from_f32<Out>(s * a.scale);
+        }
+    }
+    for (int w = 0; w < kWarps; ++w) {
+        if (first_key[w] < 0 || more[w] <= kShortRun) continue;
+        const int c = c0 + w, share = (more[w] + kWarps - 1) / kWarps;
+        const int first = min(more[w], warp * share), count = min(more[w], first + share) - first;
+        for (int base = 0; base < a.width; base += 32) {
+            const int column = base + lane;
+            part[warp][lane] = column < a.width ? sum_heads(c + 1 + first, count, column) : 0.0f;
+            __syncthreads();
+            if (warp == 0 && column < a.width) {
+                float s = a.tails[static_cast<size_t>(c) * a.width + column];
+                for (int x = 0; x < kWarps; ++x) s += part[x][lane];
+                static_cast<Out*>(a.out)[first_key[w] * a.out_stride + column] = from_f32<Out>(s * a.scale);
+            }
+            __syncthreads();
+        }
     }
 }
 
@@ -221,47 +482,141 @@ Tokens tokens_of(const BulletOuB200Matrix& m, size_t vocab) {
 
 int validate_tokens(const BulletOuB200Matrix* tokens, const char* name) {
     if (validate_matrix(tokens, kTypeI32, name) != 0) return -1;
-    if (tokens->rows * tokens->cols >= static_cast<size_t>(INT32_MAX) - kTile)
+    if (tokens->rows * tokens->cols >= static_cast<size_t>(INT32_MAX) - kMaxTile)
         return fail_messagef("%s: too many tokens (%zu)", name, tokens->rows * tokens->cols);
     return 0;
 }
 
-// Sorts the tokens into context scratch.
-int sort_tokens(BulletOuCudaCppContext* ctx, const Tokens& tokens, const int** keys, const int** positions) {
-    const int n = tokens.n;
-    const int tiles = (n + kTile - 1) / kTile;
+// How the sort's and the gradient's scratch is laid out.
+struct GradientPlan {
+    int tile, tiles, passes, digit_bits;
+    int lanes, units, unit;   // shape of gradient_kernel
+    int chunk, chunks;
+    size_t row, counts, width;
+    size_t words() const { return 4 * row + kMaxBins + counts + 2 * static_cast<size_t>(chunks) * width; }
+};
+
+GradientPlan plan_gradient(const BulletOuCudaCppContext* ctx, int n, int vocab, int width, int vector_unit, bool vector) {
+    GradientPlan p{};
     int bits = 1;
-    while (static_cast<int64_t>(tokens.vocab) >> bits != 0) ++bits;
-    const int passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
-    const int digit_bits = (bits + passes - 1) / passes;
-    const int bins = 1 << digit_bits;
-    const size_t row = (static_cast<size_t>(n) + 63) / 64 * 64;
-    const size_t counts = static_cast<size_t>(bins) * tiles;
-    void* p = nullptr;
-    if (scratch_slot(ctx, kScratchEmbedding, (4 * row + counts + kMaxBins) * sizeof(int), &p,
-                     "cudaMalloc embedding sort") != 0)
-        return -1;
-    int* const base = static_cast<int*>(p);
+    while (static_cast<int64_t>(vocab) >> bits != 0) ++bits;
+    p.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
+    p.digit_bits = (bits + p.passes - 1) / p.passes;
+    p.tile = n >= kMaxTile * ctx->sm_count ? kMaxTile : kMaxTile / 2;  // a CTA for every SM while there are tokens enough
+    p.tiles = (n + p.tile - 1) / p.tile;
+    p.row = (static_cast<size_t>(n) + 63) / 64 * 64;
+    p.counts = (static_cast<size_t>(1) << p.digit_bits) * p.tiles;
+    p.width = width;
+    p.unit = vector ? vector_unit : 1;
+    const int units = width / p.unit;
+    p.lanes = units <= 4 ? 4 : units <= 8 ? 8 : units <= 16 ? 16 : 32;
+    // 8 values for each lane, so that 8 rows in flight fit the registers
+    p.units = std::min(8 / p.unit, (units + p.lanes - 1) / p.lanes);
+    p.units = p.units >= 8 ? 8 : p.units >= 4 ? 4 : p.units >= 2 ? 2 : 1;
+    // Chunks long enough that the two partial rows of each cost little, short
+    // enough that every SM has its 64 warps.
+    const int64_t groups = static_cast<int64_t>(ctx->sm_count) * 64 * 32 / p.lanes;
+    p.chunk = 128;
+    while (p.chunk > 16 && n / p.chunk < groups) p.chunk /= 2;
+    p.chunks = (n + p.chunk - 1) / p.chunk;
+    return p;
+}
+
+// Sorts the tokens into the scratch at `base`.
+int sort_tokens(BulletOuCudaCppContext* ctx, const Tokens& tokens, const GradientPlan& plan, int* base, GradientArgs* out) {
     SortPass s{};
     s.tokens = tokens;
-    s.n = n;
-    s.tiles = tiles;
-    s.bins = bins;
-    s.totals = base + 4 * row;
+    s.n = tokens.n;
+    s.tile = plan.tile;
+    s.tiles = plan.tiles;
+    s.bins = 1 << plan.digit_bits;
+    s.totals = base + 4 * plan.row;
     s.counts = s.totals + kMaxBins;
-    for (int pass = 0; pass < passes; ++pass) {
-        s.shift = pass * digit_bits;
-        s.keys_out = base + (pass & 1) * 2 * row;
-        s.positions_out = s.keys_out + row;
-        sort_count_kernel<<<tiles, kThreads, 0, ctx->stream>>>(s);
-        sort_scan_kernel<<<bins, kThreads, 0, ctx->stream>>>(s);
-        sort_scatter_kernel<<<tiles, kThreads, 0, ctx->stream>>>(s);
+    for (int pass = 0; pass < plan.passes; ++pass) {
+        s.shift = pass * plan.digit_bits;
+        s.keys_out = base + (pass & 1) * 2 * plan.row;
+        s.positions_out = s.keys_out + plan.row;
+        LaunchShape shape{dim3(plan.tiles), kThreads};
+        shape.chained = pass > 0;
+        if (launch_kernel(ctx, "embedding sort launch", sort_count_kernel, shape, s) != 0) return -1;
+        shape.chained = true;
+        shape.grid = dim3(s.bins);
+        if (launch_kernel(ctx, "embedding sort launch", sort_scan_kernel, shape, s) != 0) return -1;
+        shape.grid = dim3(plan.tiles);
+        shape.smem = static_cast<size_t>(kWarps) * s.bins * sizeof(int);
+        if (launch_kernel(ctx, "embedding sort launch", sort_scatter_kernel, shape, s) != 0) return -1;
         s.keys_in = s.keys_out;
         s.positions_in = s.positions_out;
     }
-    *keys = s.keys_in;
-    *positions = s.positions_in;
-    return check_launch("embedding sort launch");
+    out->keys = s.keys_in;
+    out->positions = s.positions_in;
+    return 0;
+}
+
+template <typename In, typename Out, int kUnit, int kLanes, int kUnits>
+int launch_gradient(BulletOuCudaCppContext* ctx, const GradientArgs& a) {
+    const int per_block = kThreads / kLanes;
+    const int64_t blocks = static_cast<int64_t>(a.row_blocks) + (a.chunks + per_block - 1) / per_block;
+    if (blocks > INT32_MAX) return fail_message("embedding gradient: too many tokens and rows");
+    LaunchShape shape{dim3(static_cast<unsigned>(blocks), (a.width / kUnit + kLanes * kUnits - 1) / (kLanes * kUnits)), kThreads};
+    shape.chained = a.n > 0;
+    if (launch_kernel(ctx, "embedding gradient launch", gradient_kernel<In, Out, kUnit, kLanes, kUnits>, shape, a) != 0) return -1;
+    if (a.chunks <= 1) return 0;
+    LaunchShape join{dim3((a.chunks + kWarps - 1) / kWarps), kThreads};
+    join.chained = true;
+    return launch_kernel(ctx, "embedding gradient join launch", joined_rows_kernel<Out>, join, a);
+}
+
+template <typename In, typename Out, int kUnit>
+int launch_gradient_unit(BulletOuCudaCppContext* ctx, const GradientArgs& a, const GradientPlan& p) {
+    if (p.lanes == 4) return launch_gradient<In, Out, kUnit, 4, 1>(ctx, a);
+    if (p.lanes == 8) return launch_gradient<In, Out, kUnit, 8, 1>(ctx, a);
+    if (p.lanes == 16) return launch_gradient<In, Out, kUnit, 16, 1>(ctx, a);
+    if constexpr (kUnit == 1) {
+        if (p.units == 8) return launch_gradient<In, Out, 1, 32, 8>(ctx, a);
+        if (p.units == 4) return launch_gradient<In, Out, 1, 32, 4>(ctx, a);
+    }
+    if constexpr (kUnit <= 4) {
+        if (p.units == 2) return launch_gradient<In, Out, kUnit, 32, 2>(ctx, a);
+    }
+    return launch_gradient<In, Out, kUnit, 32, 1>(ctx, a);
+}
+
+template <typename In, typename Out>
+int gradient(BulletOuCudaCppContext* ctx, const Tokens& t, GradientArgs a, bool vector) {
+    const GradientPlan p = plan_gradient(ctx, t.n, t.vocab, a.width, kVectorUnit<In, Out>, vector);
+    if (t.n > 0) {
+        void* scratch = nullptr;
+        if (scratch_slot(ctx, kScratchEmbedding, p.words() * sizeof(int), &scratch, "cudaMalloc embedding gradient") != 0) return -1;
+        int* const base = static_cast<int*>(scratch);
+        a.heads = reinterpret_cast<float*>(base + 4 * p.row + kMaxBins + p.counts);
+        a.tails = a.heads + static_cast<size_t>(p.chunks) * p.width;
+        if (sort_tokens(ctx, t, p, base, &a) != 0) return -1;
+    }
+    a.chunk = p.chunk;
+    a.chunks = p.chunks;
+    a.row_blocks = (a.vocab + kEmptyRows - 1) / kEmptyRows;
+    return vector ? launch_gradient_unit<In, Out, kVectorUnit<In, Out>>(ctx, a, p) : launch_gradient_unit<In, Out, 1>(ctx, a, p);
+}
+
+// Whether rows of `width` can be taken in vector units.
+template <typename A, typename B>
+bool vector_rows(const BulletOuB200Matrix& a, const BulletOuB200Matrix& b) {
+    constexpr int kUnit = kVectorUnit<A, B>;
+    return a.cols % kUnit == 0 && rows_aligned(a, std::min<size_t>(16, kUnit * sizeof(A))) &&
+           rows_aligned(b, std::min<size_t>(16, kUnit * sizeof(B)));
+}
+
+template <typename In, typename Out>
+int lookup(BulletOuCudaCppContext* ctx, const LookupArgs& a, const BulletOuB200Matrix& table, const BulletOuB200Matrix& out) {
+    const bool vector = vector_rows<In, Out>(table, out);
+    const int units = a.width / (vector ? kVectorUnit<In, Out> : 1);
+    int group = 1;
+    while (group < 32 && group < units) group *= 2;
+    const int64_t blocks = (static_cast<int64_t>(a.tokens.n) * group + kThreads - 1) / kThreads;
+    const LaunchShape shape{dim3(static_cast<unsigned>(std::min<int64_t>(blocks, ctx->sm_count * 8))), kThreads};
+    if (vector) return launch_kernel(ctx, "embedding lookup launch", lookup_kernel<In, Out, kVectorUnit<In, Out>>, shape, a, group);
+    return launch_kernel(ctx, "embedding lookup launch", lookup_kernel<In, Out, 1>, shape, a, group);
 }
 
 }  // namespace
@@ -289,15 +644,11 @@ int bulletou_b200_embedding_forward_device(BulletOuCudaCppContext* ctx, const Bu
     a.table_stride = table->row_stride;
     a.out_stride = out->row_stride;
     a.scale = scale;
-    const size_t blocks = (static_cast<size_t>(a.tokens.n) * a.width + kThreads - 1) / kThreads;
-    const int grid = static_cast<int>(std::min<size_t>(blocks, static_cast<size_t>(ctx->sm_count) * 8));
     const bool in16 = table->type == BULLETOU_B200_TYPE_BF16, out16 = out->type == BULLETOU_B200_TYPE_BF16;
     using B = __nv_bfloat16;
-    if (in16 && out16) lookup_kernel<B, B><<<grid, kThreads, 0, ctx->stream>>>(a);
-    else if (in16) lookup_kernel<B, float><<<grid, kThreads, 0, ctx->stream>>>(a);
-    else if (out16) lookup_kernel<float, B><<<grid, kThreads, 0, ctx->stream>>>(a);
-    else lookup_kernel<float, float><<<grid, kThreads, 0, ctx->stream>>>(a);
-    return check_launch("embedding lookup launch") != 0 ? -1 : ok();
+    const int rc = in16 ? (out16 ? lookup<B, B>(ctx, a, *table, *out) : lookup<B, float>(ctx, a, *table, *out))
+                        : (out16 ? lookup<float, B>(ctx, a, *table, *out) : lookup<float, float>(ctx, a, *table, *out));
+    return rc != 0 ? rc : ok();
 }
 
 int bulletou_b200_embedding_backward_device(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix* tokens,
@@ -314,7 +665,6 @@ int bulletou_b200_embedding_backward_device(BulletOuCudaCppContext* ctx, const B
     GradientArgs a{};
     const Tokens t = tokens_of(*tokens, table_gradients->rows);
     a.n = t.n;
-    if (t.n > 0 && sort_tokens(ctx, t, &a.keys, &a.positions) != 0) return -1;
     a.grad = out_gradients->data;
     a.out = table_gradients->data;
     a.vocab = t.vocab;
@@ -325,11 +675,10 @@ int bulletou_b200_embedding_backward_device(BulletOuCudaCppContext* ctx, const B
     const bool in16 = out_gradients->type == BULLETOU_B200_TYPE_BF16;
     const bool out16 = table_gradients->type == BULLETOU_B200_TYPE_BF16;
     using B = __nv_bfloat16;
-    if (in16 && out16) gradient_kernel<B, B><<<a.vocab, kThreads, 0, ctx->stream>>>(a);
-    else if (in16) gradient_kernel<B, float><<<a.vocab, kThreads, 0, ctx->stream>>>(a);
-    else if (out16) gradient_kernel<float, B><<<a.vocab, kThreads, 0, ctx->stream>>>(a);
-    else gradient_kernel<float, float><<<a.vocab, kThreads, 0, ctx->stream>>>(a);
-    return check_launch("embedding gradient launch") != 0 ? -1 : ok();
+    const BulletOuB200Matrix &g = *out_gradients, &o = *table_gradients;
+    const int rc = in16 ? (out16 ? gradient<B, B>(ctx, t, a, vector_rows<B, B>(g, o)) : gradient<B, float>(ctx, t, a, vector_rows<B, float>(g, o)))
+                        : (out16 ? gradient<float, B>(ctx, t, a, vector_rows<float, B>(g, o)) : gradient<float, float>(ctx, t, a, vector_rows<float, float>(g, o)));
+    return rc != 0 ? rc : ok();
 }
 
 }  // extern "C"

@@ -9,6 +9,7 @@
 #include <cmath>
 
 #include "int8_linear.cuh"
+#include "token_launch.cuh"
 
 namespace bou {
 namespace {
@@ -81,7 +82,7 @@ template <typename T, int kRowThreads>
 __global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeArgs a) {
     constexpr int kHeld = 2, kRowWarps = kRowThreads / 32;
     __shared__ float warp_top[kWarps];
-    asm volatile("griddepcontrol.launch_dependents;");
+    let_next_start();
     const int in_row = threadIdx.x % kRowThreads;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / kRowThreads) + threadIdx.x / kRowThreads;
     const bool live = row < a.rows;

@@ -22,6 +22,7 @@
 
 #include "int8_linear.cuh"
 #include "tensor_core.cuh"
+#include "token_launch.cuh"
 
 namespace bou {
 namespace {
@@ -94,7 +95,6 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
         : "memory");
 }
-__device__ __forceinline__ void wait_for_quantise() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // A warp writes 32 rows x 32 columns, one row in each lane: through shared
 // memory, so that the global stores cover whole rows of the block.
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ 
             mbar_expect_tx(full + 8 * i, S::kStageBytes);
             tma_load_2d(base + i * S::kStageBytes + kABytes, &map_w, (k0 + i) * kTileK, col0, full + 8 * i);
         }
-        wait_for_quantise();
+        wait_for_previous();
         for (int i = 0; i < ahead; ++i) tma_load_2d(base + i * S::kStageBytes, &map_q, (k0 + i) * kTileK, row0, full + 8 * i);
         for (int i = ahead; i < count; ++i) {
             const int s = i % S::kStages;
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ 
     __syncwarp();
     const bool good = count == 0 || mbar_wait(done, 0);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    wait_for_quantise();  // the scales
+    wait_for_previous();  // the scales
     float* const stage = staging + warp * 32 * (32 + kStagePad);
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
     if (splits == 1) {
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
-    wait_for_quantise();
+    wait_for_previous();
 
     const int tiles_m = (a.m + 2 * kTileM - 1) / (2 * kTileM), tiles_n = (a.n + kPairN - 1) / kPairN;
     const int tiles = tiles_m * tiles_n;
@@ -441,11 +441,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 }
 
 // ------------------------------------------------------------------ host
-// rows x k bytes in boxes of box_rows x 128 bytes.
+// rows x k bytes in boxes of box_rows x 128 bytes.  (With k = 0 nothing is
+// loaded, but a map has no empty dimension.)
 int operand_map(CUtensorMap* map, const int8_t* data, int rows, int k, size_t stride, int box_rows) {
     const EncodeTiled fn = encode_tiled();
     if (fn == nullptr) return fail_message("cuTensorMapEncodeTiled is unavailable");
-    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(std::max(k, 1)), static_cast<cuuint64_t>(rows)};
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride)};
     const cuuint32_t box[2] = {kTileK, static_cast<cuuint32_t>(box_rows)};
     const cuuint32_t estride[2] = {1, 1};
@@ -454,30 +455,6 @@ int operand_map(CUtensorMap* map, const int8_t* data, int rows, int k, size_t st
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail_messagef("cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
     return 0;
-}
-
-template <typename Kernel, typename... Args>
-int launch(BulletOuCudaCppContext* ctx, Kernel kernel, int grid, int threads, size_t smem, int cluster, bool early,
-           Args... args) {
-    cudaError_t st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (st != cudaSuccess) return fail("cudaFuncSetAttribute int8 product", st);
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(grid);
-    config.blockDim = dim3(threads);
-    config.dynamicSmemBytes = smem;
-    config.stream = ctx->stream;
-    cudaLaunchAttribute attrs[2];
-    config.attrs = attrs;
-    if (cluster > 1) {
-        attrs[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        attrs[config.numAttrs++].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
-    }
-    if (early) {
-        attrs[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attrs[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-    }
-    st = cudaLaunchKernelEx(&config, kernel, args...);
-    return st != cudaSuccess ? fail("int8 product launch", st) : 0;
 }
 
 template <int TN, typename Out>
@@ -490,8 +467,8 @@ int launch_tiles(BulletOuCudaCppContext* ctx, const ProductArgs& a, bool vector_
     CUtensorMap q, w;
     if (operand_map(&q, a.q, a.m, a.k, a.q_stride, kTileM) != 0 || operand_map(&w, a.w, a.n, a.k, a.w_stride, TN) != 0)
         return -1;
-    return launch(ctx, int8_tile_kernel<TN, Out>, static_cast<int>(tiles * splits), 128, TileShape<TN>::kSmem, splits,
-                  early, q, w, a, splits, vector_ok);
+    const LaunchShape shape{dim3(static_cast<unsigned>(tiles * splits)), TileShape<TN>::kThreads, TileShape<TN>::kSmem, splits, early};
+    return launch_kernel(ctx, "int8 product launch", int8_tile_kernel<TN, Out>, shape, q, w, a, splits, vector_ok);
 }
 
 template <typename Out>
@@ -499,8 +476,8 @@ int launch_pairs(BulletOuCudaCppContext* ctx, const ProductArgs& a, int tiles, b
     CUtensorMap q, w;
     if (operand_map(&q, a.q, a.m, a.k, a.q_stride, kTileM) != 0 || operand_map(&w, a.w, a.n, a.k, a.w_stride, kTileM) != 0)
         return -1;
-    const int grid = 2 * std::min(tiles, ctx->sm_count / 2);
-    return launch(ctx, int8_pair_kernel<Out>, grid, kPairThreads, kPairSmem, 2, early, q, w, a, vector_ok);
+    const LaunchShape shape{dim3(2 * std::min(tiles, ctx->sm_count / 2)), kPairThreads, kPairSmem, 2, early};
+    return launch_kernel(ctx, "int8 product launch", int8_pair_kernel<Out>, shape, q, w, a, vector_ok);
 }
 
 template <typename Out>
