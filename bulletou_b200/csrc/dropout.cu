@@ -11,6 +11,7 @@
 #include <cmath>
 
 #include "device_matrix.cuh"
+#include "token_launch.cuh"
 
 namespace bou {
 namespace {
@@ -42,36 +43,143 @@ struct DropoutArgs {
     const void* residual;
     void* out;
     size_t n;                         // elements
-    uint32_t cols;
+    size_t cols;
     size_t x_stride, residual_stride, out_stride;
     uint2 key, offset;
     uint32_t threshold;               // dropped below; 65536: everything
     float factor;
 };
 
-// A thread takes the eight elements of one block.
+__device__ __forceinline__ bool kept(const Philox& r, int j, uint32_t threshold) {
+    return ((r.w[j >> 1] >> (16 * (j & 1))) & 0xffffu) >= threshold;
+}
+
+// Eight neighbouring elements as 16 bytes of bf16 or 32 bytes of f32.
+template <typename T>
+struct Eight;
+template <>
+struct Eight<float> {
+    uint32_t raw[8];
+    __device__ __forceinline__ void load(const float* p) {
+        asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(raw[0]), "=r"(raw[1]), "=r"(raw[2]), "=r"(raw[3]), "=r"(raw[4]), "=r"(raw[5]), "=r"(raw[6]),
+                       "=r"(raw[7])
+                     : "l"(p));
+    }
+    __device__ __forceinline__ void store(float* p) const {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(raw[0]), "r"(raw[1]),
+                     "r"(raw[2]), "r"(raw[3]), "r"(raw[4]), "r"(raw[5]), "r"(raw[6]), "r"(raw[7])
+                     : "memory");
+    }
+    __device__ __forceinline__ float get(int j) const { return __uint_as_float(raw[j]); }
+    __device__ __forceinline__ void set(int j, float v) { raw[j] = __float_as_uint(v); }
+};
+template <>
+struct Eight<__nv_bfloat16> {
+    __nv_bfloat16 e[8];
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+        *reinterpret_cast<uint4*>(e) = __ldcs(reinterpret_cast<const uint4*>(p));
+    }
+    __device__ __forceinline__ void store(__nv_bfloat16* p) const {
+        __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(e));
+    }
+    __device__ __forceinline__ float get(int j) const { return __bfloat162float(e[j]); }
+    __device__ __forceinline__ void set(int j, float v) { e[j] = __float2bfloat16_rn(v); }
+};
+
+// Rows whose eights are aligned (or one flat vector as a single row): a thread
+// takes the eight elements of one block, kBlocks of them in flight.
+template <typename T, bool kResidual>
+__global__ void __launch_bounds__(kThreads) dropout_vector_kernel(const DropoutArgs a) {
+    constexpr int kBlocks = 2;
+    const size_t blocks = a.n / kLanes, step = static_cast<size_t>(gridDim.x) * kThreads;
+    const bool flat = a.cols == a.n;
+    for (size_t b0 = static_cast<size_t>(blockIdx.x) * kThreads + threadIdx.x; b0 < blocks; b0 += step * kBlocks) {
+        Eight<T> x[kBlocks], r[kBlocks];
+        size_t row[kBlocks], col[kBlocks];
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+            const size_t e = (b0 + i * step) * kLanes;
+            row[i] = flat ? 0 : e / a.cols;
+            col[i] = e - row[i] * a.cols;
+            if (b0 + i * step < blocks) {
+                x[i].load(static_cast<const T*>(a.x) + row[i] * a.x_stride + col[i]);
+                if (kResidual) r[i].load(static_cast<const T*>(a.residual) + row[i] * a.residual_stride + col[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+            const size_t b = b0 + i * step;
+            if (b >= blocks) break;
+            const Philox random = philox_block(b, a.offset, a.key);
+            Eight<T> y;
+#pragma unroll
+            for (int j = 0; j < kLanes; ++j) {
+                const float v = kept(random, j, a.threshold) ? x[i].get(j) : 0.0f;
+                y.set(j, kResidual ? __fmaf_rn(v, a.factor, r[i].get(j)) : v * a.factor);
+            }
+            y.store(static_cast<T*>(a.out) + row[i] * a.out_stride + col[i]);
+        }
+    }
+    // the last elements of a flat vector
+    if (blockIdx.x == 0 && threadIdx.x < a.n - blocks * kLanes) {
+        const size_t e = blocks * kLanes + threadIdx.x;
+        const Philox random = philox_block(blocks, a.offset, a.key);
+        const float v = kept(random, threadIdx.x, a.threshold) ? to_f32(static_cast<const T*>(a.x)[e]) : 0.0f;
+        static_cast<T*>(a.out)[e] = from_f32<T>(kResidual ? __fmaf_rn(v, a.factor, to_f32(static_cast<const T*>(a.residual)[e]))
+                                                          : v * a.factor);
+    }
+}
+
+// Any strides and alignment: a warp takes 32 blocks, that is 256 elements in
+// row-major order.  Each lane computes one block's eight decisions; the
+// elements are then read and written 32 neighbours at a time, each lane asking
+// the lane that holds its element's block.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(const DropoutArgs a) {
+    const int lane = threadIdx.x & 31;
     const size_t blocks = (a.n + kLanes - 1) / kLanes;
-    for (size_t b = static_cast<size_t>(blockIdx.x) * kThreads + threadIdx.x; b < blocks;
-         b += static_cast<size_t>(gridDim.x) * kThreads) {
-        const Philox r = philox_block(b, a.offset, a.key);
-        size_t row = b * kLanes / a.cols;
-        uint32_t col = static_cast<uint32_t>(b * kLanes - row * a.cols);
+    const size_t row_step = 32 / a.cols, col_step = 32 % a.cols;
+    for (size_t b0 = static_cast<size_t>(blockIdx.x) * kThreads + (threadIdx.x & ~31); b0 < blocks;
+         b0 += static_cast<size_t>(gridDim.x) * kThreads) {
+        const Philox random = philox_block(b0 + lane, a.offset, a.key);
+        uint32_t mask = 0;
+#pragma unroll
+        for (int j = 0; j < kLanes; ++j) mask |= kept(random, j, a.threshold) ? 1u << j : 0u;
+        size_t row = (b0 * kLanes + lane) / a.cols, col = b0 * kLanes + lane - row * a.cols;
+        float x[kLanes], r[kLanes];
+        size_t at[kLanes];
 #pragma unroll
         for (int j = 0; j < kLanes; ++j) {
-            if (b * kLanes + j >= a.n) break;
-            const uint32_t u = (r.w[j >> 1] >> (16 * (j & 1))) & 0xffffu;
-            const bool kept = u >= a.threshold;
-            float y = kept ? to_f32(static_cast<const T*>(a.x)[row * a.x_stride + col]) * a.factor : 0.0f;
-            if (a.residual != nullptr) y += to_f32(static_cast<const T*>(a.residual)[row * a.residual_stride + col]);
-            static_cast<T*>(a.out)[row * a.out_stride + col] = from_f32<T>(y);
-            if (++col == a.cols) {
-                col = 0;
+            const bool in = b0 * kLanes + j * 32 + lane < a.n;
+            at[j] = row * a.out_stride + col;
+            x[j] = in ? to_f32(static_cast<const T*>(a.x)[row * a.x_stride + col]) : 0.0f;
+            r[j] = in && a.residual != nullptr ? to_f32(static_cast<const T*>(a.residual)[row * a.residual_stride + col]) : 0.0f;
+            row += row_step;
+            col += col_step;
+            if (col >= a.cols) {
+                col -= a.cols;
                 ++row;
             }
         }
+#pragma unroll
+        for (int j = 0; j < kLanes; ++j) {
+            const uint32_t theirs = __shfl_sync(0xffffffffu, mask, j * 4 + (lane >> 3));
+            const float v = (theirs >> (lane & 7)) & 1u ? x[j] : 0.0f;
+            if (b0 * kLanes + j * 32 + lane < a.n)
+                static_cast<T*>(a.out)[at[j]] = from_f32<T>(a.residual != nullptr ? __fmaf_rn(v, a.factor, r[j]) : v * a.factor);
+        }
     }
+}
+
+template <typename T>
+int launch_dropout(BulletOuCudaCppContext* ctx, DropoutArgs a, bool vector) {
+    const int64_t per_cta = static_cast<int64_t>(kThreads) * kLanes;
+    const int64_t ctas = (static_cast<int64_t>(a.n) + per_cta - 1) / per_cta;
+    const LaunchShape shape{dim3(static_cast<unsigned>(std::min<int64_t>(ctas, ctx->sm_count * 8))), kThreads};
+    if (!vector) return launch_kernel(ctx, "dropout launch", dropout_kernel<T>, shape, a);
+    if (a.residual != nullptr) return launch_kernel(ctx, "dropout launch", dropout_vector_kernel<T, true>, shape, a);
+    return launch_kernel(ctx, "dropout launch", dropout_vector_kernel<T, false>, shape, a);
 }
 
 }  // namespace
@@ -99,7 +207,7 @@ int bulletou_b200_dropout_device(BulletOuCudaCppContext* ctx, const BulletOuB200
     a.x = x->data;
     a.residual = residual != nullptr ? residual->data : nullptr;
     a.out = out->data;
-    a.cols = static_cast<uint32_t>(x->cols);
+    a.cols = x->cols;
     a.x_stride = x->row_stride;
     a.residual_stride = residual != nullptr ? residual->row_stride : 0;
     a.out_stride = out->row_stride;
@@ -107,13 +215,17 @@ int bulletou_b200_dropout_device(BulletOuCudaCppContext* ctx, const BulletOuB200
     a.offset = make_uint2(static_cast<uint32_t>(offset), static_cast<uint32_t>(offset >> 32));
     a.threshold = static_cast<uint32_t>(std::floor(static_cast<double>(probability) * 65536.0 + 0.5));
     a.factor = a.threshold < 65536u ? static_cast<float>(65536.0 / (65536.0 - a.threshold)) : 0.0f;
-    const size_t blocks = (a.n + kLanes * kThreads - 1) / (kLanes * kThreads);
-    const int grid = static_cast<int>(std::min<size_t>(blocks, static_cast<size_t>(ctx->sm_count) * 8));
-    if (x->type == BULLETOU_B200_TYPE_F32)
-        dropout_kernel<float><<<grid, kThreads, 0, ctx->stream>>>(a);
-    else
-        dropout_kernel<__nv_bfloat16><<<grid, kThreads, 0, ctx->stream>>>(a);
-    return check_launch("dropout launch") != 0 ? -1 : ok();
+    // a vector where every eight is aligned: rows of whole eights, or no gaps between rows at all
+    const bool flat = is_flat(*x) && is_flat(*out) && (residual == nullptr || is_flat(*residual));
+    const size_t unit = kLanes * type_bytes(x->type);
+    auto aligned = [&](const BulletOuB200Matrix& m) {
+        return flat ? reinterpret_cast<uintptr_t>(m.data) % unit == 0 : rows_aligned(m, unit);
+    };
+    const bool vector = (flat || x->cols % kLanes == 0) && aligned(*x) && aligned(*out) && (residual == nullptr || aligned(*residual));
+    if (flat) a.cols = a.n;
+    const int rc = x->type == BULLETOU_B200_TYPE_F32 ? launch_dropout<float>(ctx, a, vector)
+                                                     : launch_dropout<__nv_bfloat16>(ctx, a, vector);
+    return rc != 0 ? rc : ok();
 }
 
 }  // extern "C"
