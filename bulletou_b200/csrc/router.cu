@@ -8,12 +8,15 @@
 // Gradient with u = dL/dg and h_e = balance * E * f_e / rows * dL/dloss:
 //   plain gates       dz = p * (h + u - sum p (h + u))         (u at the chosen)
 //   normalised gates  dz = p * (h - sum p h) + g * (u - sum g u)
-// Sums over a row are trees over a warp's lanes; the sums over rows are added
-// up per lane, warp and CTA and joined in a fixed order, so no result depends
-// on timing.  Counts are integers.
+// A row is read once in each direction and held in registers.  Sums over a row
+// are trees over the lanes that share it; the sums over rows are added up per
+// lane, warp and CTA and joined in a fixed order, so no result depends on
+// timing.  Counts are integers.
 #include <algorithm>
+#include <type_traits>
 
 #include "device_matrix.cuh"
+#include "token_launch.cuh"
 
 namespace bou {
 namespace {
@@ -22,7 +25,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxExperts = BULLETOU_B200_ROUTER_MAX_EXPERTS;
 constexpr int kMaxTopK = BULLETOU_B200_ROUTER_MAX_TOP_K;
-constexpr int kPerLane = kMaxExperts / 32;
+constexpr int kJoinThreads = 1024;
 
 struct RouterArgs {
     const void* logits;
@@ -48,224 +51,285 @@ struct RouterArgs {
     size_t logit_grad_stride;
 };
 
-__device__ __forceinline__ float warp_max(float v) {
+// Sums and maxima over the kGroup lanes that share a row.
+template <int kGroup>
+__device__ __forceinline__ float group_max(float v) {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+    for (int d = kGroup / 2; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
     return v;
 }
-__device__ __forceinline__ float warp_sum(float v) {
+template <int kGroup>
+__device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    for (int d = kGroup / 2; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
     return v;
 }
 
-// A row's logits and probabilities, expert e in lane e % 32, place e / 32.
+// A row's logits and probabilities: expert e in lane e % kGroup, place
+// e / kGroup.  All lanes of a warp come here together; a row past the end is
+// one that is not alive.
+template <int kGroup, int kPlaces>
 struct Row {
-    float z[kPerLane];
-    float p[kPerLane];
-    bool alive;  // the largest logit is finite
+    float z[kPlaces];
+    float p[kPlaces];
+    float top, inverse;  // p = exp(z - top) * inverse
+    bool alive;          // the largest logit is finite
+
+    template <typename T>
+    __device__ __forceinline__ void load(const RouterArgs& a, int64_t t, int lane) {
+        const T* src = static_cast<const T*>(a.logits) + (t < a.rows ? t : 0) * a.logit_stride;
+        bool nan = false;
+        top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kPlaces; ++i) {
+            const int e = lane + kGroup * i;
+            z[i] = t < a.rows && e < a.experts ? to_f32(src[e]) : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < kPlaces; ++i) {
+            nan |= z[i] != z[i];
+            top = fmaxf(top, z[i]);
+        }
+        // NaN goes through the maximum as +inf: both break the row alike
+        top = group_max<kGroup>(nan ? INFINITY : top);
+        alive = top > -INFINITY && top < INFINITY;
+        const float shift = alive ? top : 0.0f;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPlaces; ++i) {
+            p[i] = expf(z[i] - shift);
+            sum += p[i];
+        }
+        sum = group_sum<kGroup>(sum);
+        // a masked row's exponentials are zeros; a broken row is NaN
+        inverse = alive ? 1.0f / sum : top == INFINITY ? NAN : 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPlaces; ++i) p[i] = lane + kGroup * i < a.experts ? p[i] * inverse : 0.0f;
+    }
 };
 
-template <typename T>
-__device__ __forceinline__ void load_row(const RouterArgs& a, int t, int lane, Row& r) {
-    const T* src = static_cast<const T*>(a.logits) + t * a.logit_stride;
-    float top = -INFINITY;
-    bool nan = false;
-#pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-        const int e = lane + 32 * i;
-        r.z[i] = e < a.experts ? to_f32(src[e]) : -INFINITY;
-        nan |= r.z[i] != r.z[i];
-        top = fmaxf(top, r.z[i]);
+// Means and loss from the sums of the probabilities and the counts; every
+// thread of the CTA comes here.
+__device__ void finish(const RouterArgs& a, const float* p_sums, const int* counts) {
+    __shared__ int choices;
+    __shared__ float warp_terms[32];
+    if (threadIdx.x == 0) choices = 0;
+    __syncthreads();
+    int c = 0;
+    for (int e = threadIdx.x; e < a.experts; e += blockDim.x) c += counts[e];
+    if (c != 0) atomicAdd(&choices, c);
+    __syncthreads();
+    const float rows = static_cast<float>(max(counts[a.experts], 1)), all = static_cast<float>(max(choices, 1));
+    float s = 0.0f;
+    for (int e = threadIdx.x; e < a.experts; e += blockDim.x) {
+        const float mean = p_sums[e] / rows;
+        a.mean[e] = mean;
+        a.counts[e] = counts[e];
+        s += static_cast<float>(counts[e]) / all * mean;
     }
-    nan = __any_sync(0xffffffffu, nan);
-    top = warp_max(top);
-    r.alive = !nan && top > -INFINITY && top < INFINITY;
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-        r.p[i] = r.alive ? expf(r.z[i] - top) : 0.0f;
-        sum += r.p[i];
-    }
-    sum = warp_sum(sum);
-    const float broken = (nan || top == INFINITY) ? NAN : 0.0f;
-#pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-        const bool used = lane + 32 * i < a.experts;
-        r.p[i] = r.alive ? r.p[i] / sum : (used ? broken : 0.0f);
+    if (threadIdx.x == 0) a.counts[a.experts] = counts[a.experts];
+    s = group_sum<32>(s);
+    if ((threadIdx.x & 31) == 0) warp_terms[threadIdx.x >> 5] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float total = 0.0f;
+        for (unsigned w = 0; w < blockDim.x / 32; ++w) total += warp_terms[w];
+        a.loss[0] = a.balance * static_cast<float>(a.experts) * total;
     }
 }
 
-template <typename T>
+// kGroup lanes for each row (at least top_k), kPlaces experts in each lane.  One
+// CTA alone also finishes; otherwise the CTAs leave their sums to router_join_kernel.
+template <typename T, int kGroup, int kPlaces>
 __global__ void __launch_bounds__(kThreads) router_forward_kernel(const RouterArgs a) {
     __shared__ int count[kMaxExperts + 1];
-    __shared__ float psum[kWarps][kMaxExperts];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ float psum[kWarps][kGroup * kPlaces];
+    const int lane = threadIdx.x & (kGroup - 1), warp = threadIdx.x >> 5;
+    let_next_start();
     for (int i = threadIdx.x; i <= a.experts; i += kThreads) count[i] = 0;
     __syncthreads();
-    float acc[kPerLane] = {};
-    for (int t = blockIdx.x * kWarps + warp; t < a.rows; t += gridDim.x * kWarps) {
-        Row r;
-        load_row<T>(a, t, lane, r);
+    float acc[kPlaces] = {};
+    int alive = 0;
+    constexpr int kRows = kThreads / kGroup;
+    for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * kRows; t0 < a.rows; t0 += static_cast<int64_t>(gridDim.x) * kRows) {
+        const int64_t t = t0 + threadIdx.x / kGroup;
+        Row<kGroup, kPlaces> r;
+        r.template load<T>(a, t, lane);
 #pragma unroll
-        for (int i = 0; i < kPerLane; ++i) acc[i] += r.p[i];
-        int pick[kMaxTopK];
-        float gate[kMaxTopK];
-        float total = 0.0f;
-#pragma unroll
-        for (int j = 0; j < kMaxTopK; ++j) {
-            if (j >= a.top_k) break;
-            float best = -INFINITY, best_p = 0.0f;
+        for (int i = 0; i < kPlaces; ++i) acc[i] += r.p[i];
+        alive += r.alive && lane == 0;
+        float total = 0.0f, own = 0.0f;  // lane j keeps the j-th choice
+        int pick = -1;
+#pragma unroll 1
+        for (int j = 0; j < a.top_k; ++j) {
+            float best = -INFINITY;
             int at = kMaxExperts;
 #pragma unroll
-            for (int i = 0; i < kPerLane; ++i)
+            for (int i = 0; i < kPlaces; ++i)
                 if (r.z[i] > best) {
                     best = r.z[i];
-                    best_p = r.p[i];
-                    at = lane + 32 * i;
+                    at = lane + kGroup * i;
                 }
 #pragma unroll
-            for (int d = 16; d > 0; d >>= 1) {
+            for (int d = kGroup / 2; d > 0; d >>= 1) {
                 const float z = __shfl_xor_sync(0xffffffffu, best, d);
-                const float p = __shfl_xor_sync(0xffffffffu, best_p, d);
                 const int e = __shfl_xor_sync(0xffffffffu, at, d);
                 if (z > best || (z == best && e < at)) {
                     best = z;
-                    best_p = p;
                     at = e;
                 }
             }
             const bool some = r.alive && best > -INFINITY;
-            pick[j] = some ? at : -1;
-            gate[j] = some ? best_p : 0.0f;
-            total += gate[j];
-#pragma unroll
-            for (int i = 0; i < kPerLane; ++i)
-                if (lane + 32 * i == at) r.z[i] = -INFINITY;
-        }
-        if (lane == 0) {
-            if (r.alive) atomicAdd(count + a.experts, 1);
-            for (int j = 0; j < kMaxTopK; ++j) {
-                if (j >= a.top_k) break;
-                if (pick[j] >= 0) atomicAdd(count + pick[j], 1);
-                a.chosen[t * a.chosen_stride + j] = pick[j];
-                a.gates[t * a.gate_stride + j] = a.normalize && pick[j] >= 0 ? gate[j] / total : gate[j];
+            const float gate = some ? expf(best - r.top) * r.inverse : 0.0f;
+            total += gate;
+            if (j == lane) {
+                pick = some ? at : -1;
+                own = gate;
             }
+#pragma unroll
+            for (int i = 0; i < kPlaces; ++i)
+                if (lane + kGroup * i == at) r.z[i] = -INFINITY;
+        }
+        if (lane < a.top_k && t < a.rows) {
+            a.chosen[t * a.chosen_stride + lane] = pick;
+            a.gates[t * a.gate_stride + lane] = a.normalize && pick >= 0 ? own / total : own;
+            if (pick >= 0) atomicAdd(count + pick, 1);
         }
     }
+    if (alive != 0) atomicAdd(count + a.experts, alive);
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) psum[warp][lane + 32 * i] = acc[i];
+    for (int i = 0; i < kPlaces; ++i) {
+#pragma unroll
+        for (int d = kGroup; d < 32; d <<= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], d);
+        if ((threadIdx.x & 31) < kGroup) psum[warp][lane + kGroup * i] = acc[i];
+    }
     __syncthreads();
     for (int e = threadIdx.x; e < a.experts; e += kThreads) {
         float s = 0.0f;
         for (int w = 0; w < kWarps; ++w) s += psum[w][e];
-        a.part_p[static_cast<size_t>(blockIdx.x) * a.experts + e] = s;
+        if (gridDim.x == 1) psum[0][e] = s;
+        else a.part_p[static_cast<size_t>(blockIdx.x) * a.experts + e] = s;
+    }
+    __syncthreads();
+    if (gridDim.x == 1) {
+        finish(a, psum[0], count);
+        return;
     }
     for (int e = threadIdx.x; e <= a.experts; e += kThreads)
         a.part_c[static_cast<size_t>(blockIdx.x) * (a.experts + 1) + e] = count[e];
 }
 
-// One CTA: the CTAs' parts joined in order, means and loss.
-__global__ void __launch_bounds__(kMaxExperts) router_join_kernel(const RouterArgs a, int parts) {
-    __shared__ float term[kMaxExperts];
-    __shared__ int rows, choices;
-    if (threadIdx.x == 0) rows = choices = 0;
+// One CTA: the CTAs' sums joined, each warp every 32nd of them, then the warps
+// in order.
+__global__ void __launch_bounds__(kJoinThreads) router_join_kernel(const RouterArgs a, int parts) {
+    constexpr int kJoinWarps = kJoinThreads / 32, kAtOnce = 128;
+    __shared__ float part[kJoinWarps][kAtOnce];
+    __shared__ float p_sums[kMaxExperts];
+    __shared__ int count[kMaxExperts + 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int e = threadIdx.x; e <= a.experts; e += kJoinThreads) count[e] = 0;
     __syncthreads();
-    float p = 0.0f;
-    int c = 0;
-    const int e = threadIdx.x;
-    if (e < a.experts)
-        for (int i = 0; i < parts; ++i) {
-            p += a.part_p[static_cast<size_t>(i) * a.experts + e];
-            c += a.part_c[static_cast<size_t>(i) * (a.experts + 1) + e];
+    wait_for_previous();
+    for (int e0 = 0; e0 <= a.experts; e0 += kAtOnce) {
+        float p[kAtOnce / 32] = {};
+        int c[kAtOnce / 32] = {};
+#pragma unroll 4
+        for (int i = warp; i < parts; i += kJoinWarps) {
+#pragma unroll
+            for (int j = 0; j < kAtOnce / 32; ++j) {
+                const int e = e0 + lane + 32 * j;
+                if (e < a.experts) p[j] += a.part_p[static_cast<size_t>(i) * a.experts + e];
+                if (e <= a.experts) c[j] += a.part_c[static_cast<size_t>(i) * (a.experts + 1) + e];
+            }
         }
-    atomicAdd(&choices, c);
-    int r = 0;
-    for (int i = threadIdx.x; i < parts; i += kMaxExperts) r += a.part_c[static_cast<size_t>(i) * (a.experts + 1) + a.experts];
-    atomicAdd(&rows, r);
-    __syncthreads();
-    const float mean = p / static_cast<float>(max(rows, 1));
-    term[e] = 0.0f;
-    if (e < a.experts) {
-        a.mean[e] = mean;
-        a.counts[e] = c;
-        term[e] = static_cast<float>(c) / static_cast<float>(max(choices, 1)) * mean;
-    }
-    if (e == 0) a.counts[a.experts] = rows;
-    __syncthreads();
-    for (int d = kMaxExperts / 2; d > 0; d >>= 1) {
-        if (e < d) term[e] += term[e + d];
+#pragma unroll
+        for (int j = 0; j < kAtOnce / 32; ++j) {
+            part[warp][lane + 32 * j] = p[j];
+            if (c[j] != 0) atomicAdd(count + e0 + lane + 32 * j, c[j]);
+        }
+        __syncthreads();
+        if (threadIdx.x < kAtOnce && e0 + static_cast<int>(threadIdx.x) < a.experts) {
+            float s = 0.0f;
+            for (int w = 0; w < kJoinWarps; ++w) s += part[w][threadIdx.x];
+            p_sums[e0 + threadIdx.x] = s;
+        }
         __syncthreads();
     }
-    if (e == 0) a.loss[0] = a.balance * static_cast<float>(a.experts) * term[0];
+    finish(a, p_sums, count);
 }
 
-template <typename T>
+template <typename T, int kGroup, int kPlaces>
 __global__ void __launch_bounds__(kThreads) router_backward_kernel(const RouterArgs a) {
     __shared__ int choices;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & (kGroup - 1);
     if (threadIdx.x == 0) choices = 0;
     __syncthreads();
     int c = 0;
     for (int e = threadIdx.x; e < a.experts; e += kThreads) c += a.counts[e];
-    atomicAdd(&choices, c);
+    if (c != 0) atomicAdd(&choices, c);
     __syncthreads();
     // the balance loss's pull on every probability of an expert
-    float h[kPerLane];
+    float h[kPlaces];
     const float unit = (a.loss_grad != nullptr ? a.loss_grad[0] : 0.0f) * a.balance * static_cast<float>(a.experts) /
-                       static_cast<float>(max(a.counts[a.experts], 1));
+                       static_cast<float>(max(a.counts[a.experts], 1)) / static_cast<float>(max(choices, 1));
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-        const int e = lane + 32 * i;
-        h[i] = e < a.experts ? static_cast<float>(a.counts[e]) / static_cast<float>(max(choices, 1)) * unit : 0.0f;
+    for (int i = 0; i < kPlaces; ++i) {
+        const int e = lane + kGroup * i;
+        h[i] = e < a.experts ? static_cast<float>(a.counts[e]) * unit : 0.0f;
     }
-    for (int t = blockIdx.x * kWarps + warp; t < a.rows; t += gridDim.x * kWarps) {
-        Row r;
-        load_row<T>(a, t, lane, r);
-        float u[kPerLane], g[kPerLane];  // gate gradients and gates at the chosen experts
+    constexpr int kRows = kThreads / kGroup;
+    for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * kRows; t0 < a.rows; t0 += static_cast<int64_t>(gridDim.x) * kRows) {
+        const int64_t t = t0 + threadIdx.x / kGroup;
+        // lane j holds the j-th choice
+        int pick = -1;
+        float up = 0.0f;
+        if (a.gate_grad != nullptr && lane < a.top_k && t < a.rows) {
+            pick = a.chosen[t * a.chosen_stride + lane];
+            up = a.gate_grad[t * a.gate_grad_stride + lane];
+        }
+        Row<kGroup, kPlaces> r;
+        r.template load<T>(a, t, lane);
+        float direct[kPlaces];  // plain gates: their gradient joins the pull; normalised: p_e (u_e - sum g u) / sum p
         float total = 0.0f, dot = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kPerLane; ++i) u[i] = g[i] = 0.0f;
-        if (a.gate_grad != nullptr)
+        for (int i = 0; i < kPlaces; ++i) direct[i] = 0.0f;
+        if (a.gate_grad != nullptr) {
+            bool mine[kPlaces] = {};
+#pragma unroll 1
             for (int j = 0; j < a.top_k; ++j) {
-                const int e = a.chosen[t * a.chosen_stride + j];
-                if (e < 0 || e >= a.experts) continue;
-                const float up = a.gate_grad[t * a.gate_grad_stride + j];
+                const int e = __shfl_sync(0xffffffffu, pick, j, kGroup);
+                const float u = __shfl_sync(0xffffffffu, up, j, kGroup);
 #pragma unroll
-                for (int i = 0; i < kPerLane; ++i)
-                    if (lane + 32 * i == e) {
-                        u[i] = up;
-                        g[i] = r.p[i];
+                for (int i = 0; i < kPlaces; ++i)
+                    if (lane + kGroup * i == e && e < a.experts) {
+                        direct[i] = u;
+                        mine[i] = true;
                     }
             }
-        if (a.normalize && a.gate_grad != nullptr) {
+            if (a.normalize) {
+                float weighted = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kPerLane; ++i) total += g[i];
-            total = warp_sum(total);
-            float own = 0.0f;
+                for (int i = 0; i < kPlaces; ++i) {
+                    total += mine[i] ? r.p[i] : 0.0f;
+                    weighted += mine[i] ? r.p[i] * direct[i] : 0.0f;
+                }
+                total = group_sum<kGroup>(total);
+                weighted = group_sum<kGroup>(weighted);
+                const float scale = total > 0.0f ? 1.0f / total : 0.0f;
 #pragma unroll
-            for (int i = 0; i < kPerLane; ++i) {
-                g[i] = total > 0.0f ? g[i] / total : 0.0f;
-                own += g[i] * u[i];
+                for (int i = 0; i < kPlaces; ++i) direct[i] = mine[i] ? (direct[i] - weighted * scale) * scale : 0.0f;
             }
-            own = warp_sum(own);
-#pragma unroll
-            for (int i = 0; i < kPerLane; ++i) {
-                g[i] *= u[i] - own;  // the part through the gates
-                u[i] = 0.0f;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kPerLane; ++i) g[i] = 0.0f;
         }
+        // normalised gates sum to one, so their part has no mean to take off
 #pragma unroll
-        for (int i = 0; i < kPerLane; ++i) dot += r.p[i] * (h[i] + u[i]);
-        dot = warp_sum(dot);
+        for (int i = 0; i < kPlaces; ++i) dot += r.p[i] * (a.normalize ? h[i] : h[i] + direct[i]);
+        dot = group_sum<kGroup>(dot);
+        if (t >= a.rows) continue;  // the whole group
         T* dst = static_cast<T*>(a.logit_grad) + t * a.logit_grad_stride;
 #pragma unroll
-        for (int i = 0; i < kPerLane; ++i) {
-            const int e = lane + 32 * i;
-            if (e < a.experts) dst[e] = from_f32<T>(r.p[i] * (h[i] + u[i] - dot) + g[i]);
+        for (int i = 0; i < kPlaces; ++i) {
+            const int e = lane + kGroup * i;
+            if (e < a.experts) dst[e] = from_f32<T>(r.p[i] * (h[i] + direct[i] - dot));
         }
     }
 }
@@ -279,8 +343,55 @@ int validate_counts(const RouterArgs& a) {
     return 0;
 }
 
-int router_grid(const BulletOuCudaCppContext* ctx, int rows) {
-    return std::max(1, std::min((rows + kWarps - 1) / kWarps, ctx->sm_count * 4));
+// The lanes of a row: few enough that a lane has several experts and the trees
+// over lanes stay short, and one for every choice.
+template <typename F>
+int with_shape(const RouterArgs& a, F&& f) {
+    if (a.experts <= 16 && a.top_k <= 4) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
+    if (a.experts <= 32 && a.top_k <= 4) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 8>{});
+    if (a.experts <= 64) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 8>{});
+    if (a.experts <= 96) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 12>{});
+    if (a.experts <= 128) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 16>{});
+    if (a.experts <= 256) return f(std::integral_constant<int, 16>{}, std::integral_constant<int, 16>{});
+    return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 16>{});
+}
+
+// CTAs for the rows; up to four rounds of rows are left to one CTA, which then
+// needs no second launch.
+int router_grid(const BulletOuCudaCppContext* ctx, int rows, int group) {
+    const int per = kThreads / group;
+    const int64_t ctas = (static_cast<int64_t>(rows) + per - 1) / per;
+    return ctas <= 4 ? 1 : static_cast<int>(std::min<int64_t>(ctas, static_cast<int64_t>(ctx->sm_count) * 4));
+}
+
+template <typename T>
+int forward(BulletOuCudaCppContext* ctx, RouterArgs a) {
+    return with_shape(a, [&](auto group, auto places) {
+        const int grid = router_grid(ctx, a.rows, group);
+        if (grid > 1) {
+            void* p = nullptr;
+            if (scratch_slot(ctx, kScratchRouter, static_cast<size_t>(grid) * (2 * a.experts + 1) * 4, &p,
+                             "cudaMalloc router parts") != 0)
+                return -1;
+            a.part_p = static_cast<float*>(p);
+            a.part_c = static_cast<int*>(p) + static_cast<size_t>(grid) * a.experts;
+        }
+        LaunchShape shape{dim3(grid), kThreads};
+        if (launch_kernel(ctx, "router forward launch", router_forward_kernel<T, group(), places()>, shape, a) != 0) return -1;
+        if (grid == 1) return 0;
+        LaunchShape join{dim3(1), kJoinThreads};
+        join.chained = true;
+        return launch_kernel(ctx, "router join launch", router_join_kernel, join, a, grid);
+    });
+}
+
+template <typename T>
+int backward(BulletOuCudaCppContext* ctx, const RouterArgs& a) {
+    return with_shape(a, [&](auto group, auto places) {
+        const int64_t ctas = (static_cast<int64_t>(a.rows) * group + kThreads - 1) / kThreads;
+        const LaunchShape shape{dim3(static_cast<unsigned>(std::min<int64_t>(ctas, static_cast<int64_t>(ctx->sm_count) * 8))), kThreads};
+        return launch_kernel(ctx, "router backward launch", router_backward_kernel<T, group(), places()>, shape, a);
+    });
 }
 
 }  // namespace
@@ -325,19 +436,8 @@ int bulletou_b200_router_forward_device(BulletOuCudaCppContext* ctx, const Bulle
     a.counts = static_cast<int*>(counts->data);
     a.mean = static_cast<float*>(mean_probabilities->data);
     a.loss = static_cast<float*>(loss->data);
-    const int grid = router_grid(ctx, a.rows);
-    void* p = nullptr;
-    if (scratch_slot(ctx, kScratchRouter, static_cast<size_t>(grid) * (2 * a.experts + 1) * 4, &p,
-                     "cudaMalloc router parts") != 0)
-        return -1;
-    a.part_p = static_cast<float*>(p);
-    a.part_c = static_cast<int*>(p) + static_cast<size_t>(grid) * a.experts;
-    if (logits->type == BULLETOU_B200_TYPE_F32)
-        router_forward_kernel<float><<<grid, kThreads, 0, ctx->stream>>>(a);
-    else
-        router_forward_kernel<__nv_bfloat16><<<grid, kThreads, 0, ctx->stream>>>(a);
-    router_join_kernel<<<1, kMaxExperts, 0, ctx->stream>>>(a, grid);
-    return check_launch("router forward launch") != 0 ? -1 : ok();
+    const int rc = logits->type == BULLETOU_B200_TYPE_F32 ? forward<float>(ctx, a) : forward<__nv_bfloat16>(ctx, a);
+    return rc != 0 ? rc : ok();
 }
 
 int bulletou_b200_router_backward_device(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix* logits,
@@ -377,12 +477,8 @@ int bulletou_b200_router_backward_device(BulletOuCudaCppContext* ctx, const Bull
     a.loss_grad = loss_gradient != nullptr ? static_cast<const float*>(loss_gradient->data) : nullptr;
     a.logit_grad = logit_gradients->data;
     a.logit_grad_stride = logit_gradients->row_stride;
-    const int grid = router_grid(ctx, a.rows);
-    if (logits->type == BULLETOU_B200_TYPE_F32)
-        router_backward_kernel<float><<<grid, kThreads, 0, ctx->stream>>>(a);
-    else
-        router_backward_kernel<__nv_bfloat16><<<grid, kThreads, 0, ctx->stream>>>(a);
-    return check_launch("router backward launch") != 0 ? -1 : ok();
+    const int rc = logits->type == BULLETOU_B200_TYPE_F32 ? backward<float>(ctx, a) : backward<__nv_bfloat16>(ctx, a);
+    return rc != 0 ? rc : ok();
 }
 
 }  // extern "C"
