@@ -83,12 +83,6 @@ class RowExchange(ctypes.Structure):
                 ("slot_rows", Z), ("epoch", I), ("small_recv", U64 * 8), ("small_len", Z), ("small_flag_base", Z)]
 
 
-class Matrix(ctypes.Structure):
-    """BulletOuB200Matrix."""
-
-    _fields_ = [("data", P), ("type", I), ("rows", Z), ("cols", Z), ("row_stride", Z)]
-
-
 class LossSpec(ctypes.Structure):
     """BulletOuB200LossSpec."""
 

@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kLanes = 8;  // elements of one Philox block
+constexpr int kCtas = 4;   // CTAs on an SM: 64 registers for each thread
 
 struct Philox {
     uint32_t w[4];
@@ -44,6 +45,7 @@ struct DropoutArgs {
     void* out;
     size_t n;                         // elements
     size_t cols;
+    bool flat;                        // no gaps between the rows of any operand
     size_t x_stride, residual_stride, out_stride;
     uint2 key, offset;
     uint32_t threshold;               // dropped below; 65536: everything
@@ -87,24 +89,24 @@ struct Eight<__nv_bfloat16> {
     __device__ __forceinline__ void set(int j, float v) { e[j] = __float2bfloat16_rn(v); }
 };
 
-// Rows whose eights are aligned (or one flat vector as a single row): a thread
-// takes the eight elements of one block, kBlocks of them in flight.
-template <typename T, bool kResidual>
-__global__ void __launch_bounds__(kThreads) dropout_vector_kernel(const DropoutArgs a) {
-    constexpr int kBlocks = 2;
+// Rows whose eights are aligned, or (kFlat) one vector: a thread takes the eight
+// elements of a block, kBlocks of them with their loads in flight while the
+// Philox rounds run.
+template <typename T, bool kResidual, bool kFlat>
+__global__ void __launch_bounds__(kThreads, kCtas) dropout_vector_kernel(const DropoutArgs a) {
+    constexpr int kBlocks = sizeof(T) == 2 ? 2 : 1;
     const size_t blocks = a.n / kLanes, step = static_cast<size_t>(gridDim.x) * kThreads;
-    const bool flat = a.cols == a.n;
     for (size_t b0 = static_cast<size_t>(blockIdx.x) * kThreads + threadIdx.x; b0 < blocks; b0 += step * kBlocks) {
         Eight<T> x[kBlocks], r[kBlocks];
-        size_t row[kBlocks], col[kBlocks];
+        T* out[kBlocks];
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i) {
             const size_t e = (b0 + i * step) * kLanes;
-            row[i] = flat ? 0 : e / a.cols;
-            col[i] = e - row[i] * a.cols;
+            const size_t row = kFlat ? 0 : e / a.cols, col = kFlat ? e : e - row * a.cols;
+            out[i] = static_cast<T*>(a.out) + row * a.out_stride + col;
             if (b0 + i * step < blocks) {
-                x[i].load(static_cast<const T*>(a.x) + row[i] * a.x_stride + col[i]);
-                if (kResidual) r[i].load(static_cast<const T*>(a.residual) + row[i] * a.residual_stride + col[i]);
+                x[i].load(static_cast<const T*>(a.x) + row * a.x_stride + col);
+                if (kResidual) r[i].load(static_cast<const T*>(a.residual) + row * a.residual_stride + col);
             }
         }
 #pragma unroll
@@ -112,17 +114,16 @@ __global__ void __launch_bounds__(kThreads) dropout_vector_kernel(const DropoutA
             const size_t b = b0 + i * step;
             if (b >= blocks) break;
             const Philox random = philox_block(b, a.offset, a.key);
-            Eight<T> y;
 #pragma unroll
             for (int j = 0; j < kLanes; ++j) {
                 const float v = kept(random, j, a.threshold) ? x[i].get(j) : 0.0f;
-                y.set(j, kResidual ? __fmaf_rn(v, a.factor, r[i].get(j)) : v * a.factor);
+                x[i].set(j, kResidual ? __fmaf_rn(v, a.factor, r[i].get(j)) : v * a.factor);
             }
-            y.store(static_cast<T*>(a.out) + row[i] * a.out_stride + col[i]);
+            x[i].store(out[i]);
         }
     }
     // the last elements of a flat vector
-    if (blockIdx.x == 0 && threadIdx.x < a.n - blocks * kLanes) {
+    if (kFlat && blockIdx.x == 0 && threadIdx.x < a.n - blocks * kLanes) {
         const size_t e = blocks * kLanes + threadIdx.x;
         const Philox random = philox_block(blocks, a.offset, a.key);
         const float v = kept(random, threadIdx.x, a.threshold) ? to_f32(static_cast<const T*>(a.x)[e]) : 0.0f;
@@ -135,51 +136,64 @@ __global__ void __launch_bounds__(kThreads) dropout_vector_kernel(const DropoutA
 // row-major order.  Each lane computes one block's eight decisions; the
 // elements are then read and written 32 neighbours at a time, each lane asking
 // the lane that holds its element's block.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) dropout_kernel(const DropoutArgs a) {
+template <typename T, bool kResidual>
+__global__ void __launch_bounds__(kThreads, kCtas) dropout_kernel(const DropoutArgs a) {
     const int lane = threadIdx.x & 31;
     const size_t blocks = (a.n + kLanes - 1) / kLanes;
-    const size_t row_step = 32 / a.cols, col_step = 32 % a.cols;
+    // 32 elements further on: so many rows and columns, and what a full row's end adds
+    const uint32_t cols = static_cast<uint32_t>(a.cols), rows32 = 32 / cols, cols32 = 32 % cols;
+    const size_t x_step = rows32 * a.x_stride + cols32, x_wrap = a.x_stride - cols;
+    const size_t r_step = rows32 * a.residual_stride + cols32, r_wrap = a.residual_stride - cols;
+    const size_t out_step = rows32 * a.out_stride + cols32, out_wrap = a.out_stride - cols;
     for (size_t b0 = static_cast<size_t>(blockIdx.x) * kThreads + (threadIdx.x & ~31); b0 < blocks;
          b0 += static_cast<size_t>(gridDim.x) * kThreads) {
+        const size_t e = b0 * kLanes + lane, row = e / cols;
+        uint32_t col = static_cast<uint32_t>(e - row * cols);
+        const int left = static_cast<int>(a.n - b0 * kLanes < 256 ? a.n - b0 * kLanes : 256);
+        const T* x_at = static_cast<const T*>(a.x) + row * a.x_stride + col;
+        const T* r_at = kResidual ? static_cast<const T*>(a.residual) + row * a.residual_stride + col : nullptr;
+        float x[kLanes], r[kLanes];
+        uint32_t wraps = 0;  // bit j: element j is followed by a row's end
+#pragma unroll
+        for (int j = 0; j < kLanes; ++j) {
+            const bool in = j * 32 + lane < left;
+            x[j] = in ? to_f32(*x_at) : 0.0f;
+            if (kResidual) r[j] = in ? to_f32(*r_at) : 0.0f;
+            col += cols32;
+            const bool wrap = col >= cols;
+            if (wrap) col -= cols;
+            wraps |= wrap ? 1u << j : 0u;
+            x_at += x_step + (wrap ? x_wrap : 0);
+            if (kResidual) r_at += r_step + (wrap ? r_wrap : 0);
+        }
         const Philox random = philox_block(b0 + lane, a.offset, a.key);
         uint32_t mask = 0;
 #pragma unroll
         for (int j = 0; j < kLanes; ++j) mask |= kept(random, j, a.threshold) ? 1u << j : 0u;
-        size_t row = (b0 * kLanes + lane) / a.cols, col = b0 * kLanes + lane - row * a.cols;
-        float x[kLanes], r[kLanes];
-        size_t at[kLanes];
-#pragma unroll
-        for (int j = 0; j < kLanes; ++j) {
-            const bool in = b0 * kLanes + j * 32 + lane < a.n;
-            at[j] = row * a.out_stride + col;
-            x[j] = in ? to_f32(static_cast<const T*>(a.x)[row * a.x_stride + col]) : 0.0f;
-            r[j] = in && a.residual != nullptr ? to_f32(static_cast<const T*>(a.residual)[row * a.residual_stride + col]) : 0.0f;
-            row += row_step;
-            col += col_step;
-            if (col >= a.cols) {
-                col -= a.cols;
-                ++row;
-            }
-        }
+        T* out = static_cast<T*>(a.out) + row * a.out_stride + (e - row * cols);
 #pragma unroll
         for (int j = 0; j < kLanes; ++j) {
             const uint32_t theirs = __shfl_sync(0xffffffffu, mask, j * 4 + (lane >> 3));
             const float v = (theirs >> (lane & 7)) & 1u ? x[j] : 0.0f;
-            if (b0 * kLanes + j * 32 + lane < a.n)
-                static_cast<T*>(a.out)[at[j]] = from_f32<T>(a.residual != nullptr ? __fmaf_rn(v, a.factor, r[j]) : v * a.factor);
+            if (j * 32 + lane < left) *out = from_f32<T>(kResidual ? __fmaf_rn(v, a.factor, r[j]) : v * a.factor);
+            out += out_step + ((wraps >> j) & 1u ? out_wrap : 0);
         }
     }
 }
 
-template <typename T>
-int launch_dropout(BulletOuCudaCppContext* ctx, DropoutArgs a, bool vector) {
+template <typename T, bool kResidual>
+int launch_dropout(BulletOuCudaCppContext* ctx, const DropoutArgs& a, bool vector) {
     const int64_t per_cta = static_cast<int64_t>(kThreads) * kLanes;
     const int64_t ctas = (static_cast<int64_t>(a.n) + per_cta - 1) / per_cta;
-    const LaunchShape shape{dim3(static_cast<unsigned>(std::min<int64_t>(ctas, ctx->sm_count * 8))), kThreads};
-    if (!vector) return launch_kernel(ctx, "dropout launch", dropout_kernel<T>, shape, a);
-    if (a.residual != nullptr) return launch_kernel(ctx, "dropout launch", dropout_vector_kernel<T, true>, shape, a);
-    return launch_kernel(ctx, "dropout launch", dropout_vector_kernel<T, false>, shape, a);
+    const LaunchShape shape{dim3(static_cast<unsigned>(std::min<int64_t>(ctas, ctx->sm_count * kCtas))), kThreads};
+    if (!vector) return launch_kernel(ctx, "dropout launch", dropout_kernel<T, kResidual>, shape, a);
+    if (a.flat) return launch_kernel(ctx, "dropout launch", dropout_vector_kernel<T, kResidual, true>, shape, a);
+    return launch_kernel(ctx, "dropout launch", dropout_vector_kernel<T, kResidual, false>, shape, a);
+}
+
+template <typename T>
+int launch_dropout(BulletOuCudaCppContext* ctx, const DropoutArgs& a, bool vector) {
+    return a.residual != nullptr ? launch_dropout<T, true>(ctx, a, vector) : launch_dropout<T, false>(ctx, a, vector);
 }
 
 }  // namespace
@@ -216,13 +230,12 @@ int bulletou_b200_dropout_device(BulletOuCudaCppContext* ctx, const BulletOuB200
     a.threshold = static_cast<uint32_t>(std::floor(static_cast<double>(probability) * 65536.0 + 0.5));
     a.factor = a.threshold < 65536u ? static_cast<float>(65536.0 / (65536.0 - a.threshold)) : 0.0f;
     // a vector where every eight is aligned: rows of whole eights, or no gaps between rows at all
-    const bool flat = is_flat(*x) && is_flat(*out) && (residual == nullptr || is_flat(*residual));
+    a.flat = is_flat(*x) && is_flat(*out) && (residual == nullptr || is_flat(*residual));
     const size_t unit = kLanes * type_bytes(x->type);
     auto aligned = [&](const BulletOuB200Matrix& m) {
-        return flat ? reinterpret_cast<uintptr_t>(m.data) % unit == 0 : rows_aligned(m, unit);
+        return a.flat ? reinterpret_cast<uintptr_t>(m.data) % unit == 0 : rows_aligned(m, unit);
     };
-    const bool vector = (flat || x->cols % kLanes == 0) && aligned(*x) && aligned(*out) && (residual == nullptr || aligned(*residual));
-    if (flat) a.cols = a.n;
+    const bool vector = (a.flat || x->cols % kLanes == 0) && aligned(*x) && aligned(*out) && (residual == nullptr || aligned(*residual));
     const int rc = x->type == BULLETOU_B200_TYPE_F32 ? launch_dropout<float>(ctx, a, vector)
                                                      : launch_dropout<__nv_bfloat16>(ctx, a, vector);
     return rc != 0 ? rc : ok();

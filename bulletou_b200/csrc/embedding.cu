@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kLookupCtas = 5;  // CTAs on an SM
 
 // Tokens in row-major order; those outside [0, vocab) become vocab.
 struct Tokens {
@@ -37,50 +38,44 @@ struct Tokens {
     }
 };
 
-// kUnit elements that are loaded or stored together: 16 bytes of the narrower
-// type where the rows allow it, else one element.
+// kUnit elements that are loaded or stored together, as they are in memory: 16
+// bytes of the narrower type where the rows allow it, else one element.
 template <typename T, int kUnit>
-__device__ __forceinline__ void load_unit(const T* p, float* v) {
-    if constexpr (kUnit == 1) {
-        v[0] = to_f32(*p);
-    } else {
-        constexpr int kWords = kUnit * sizeof(T) / 4;
-        uint32_t raw[kWords];
-        if constexpr (kWords == 2) {
+struct Raw {
+    static constexpr int kWords = kUnit == 1 ? 1 : kUnit * static_cast<int>(sizeof(T)) / 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (kUnit == 1) {
+            *reinterpret_cast<T*>(w) = *p;
+        } else if constexpr (kWords == 2) {
             const uint2 u = *reinterpret_cast<const uint2*>(p);
-            raw[0] = u.x, raw[1] = u.y;
+            w[0] = u.x, w[1] = u.y;
         } else {
 #pragma unroll
             for (int i = 0; i < kWords; i += 4) {
-                const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p) + 4 * i);
-                raw[i] = u.x, raw[i + 1] = u.y, raw[i + 2] = u.z, raw[i + 3] = u.w;
+                const uint4 u = *(reinterpret_cast<const uint4*>(p) + i / 4);
+                w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
             }
         }
-        const T* e = reinterpret_cast<const T*>(raw);
-#pragma unroll
-        for (int i = 0; i < kUnit; ++i) v[i] = to_f32(e[i]);
     }
-}
-template <typename T, int kUnit>
-__device__ __forceinline__ void store_unit(T* p, const float* v) {
-    if constexpr (kUnit == 1) {
-        *p = from_f32<T>(v[0]);
-    } else {
-        constexpr int kWords = kUnit * sizeof(T) / 4;
-        uint32_t raw[kWords];
-        T* e = reinterpret_cast<T*>(raw);
-#pragma unroll
-        for (int i = 0; i < kUnit; ++i) e[i] = from_f32<T>(v[i]);
-        if constexpr (kWords == 2) {
-            __stcs(reinterpret_cast<uint2*>(p), make_uint2(raw[0], raw[1]));
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (kUnit == 1) {
+            *p = *reinterpret_cast<const T*>(w);
+        } else if constexpr (kWords == 2) {
+            __stcs(reinterpret_cast<uint2*>(p), make_uint2(w[0], w[1]));
         } else {
 #pragma unroll
             for (int i = 0; i < kWords; i += 4)
-                __stcs(reinterpret_cast<uint4*>(reinterpret_cast<char*>(p) + 4 * i),
-                       make_uint4(raw[i], raw[i + 1], raw[i + 2], raw[i + 3]));
+                __stcs(reinterpret_cast<uint4*>(p) + i / 4, make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]));
         }
     }
-}
+    __device__ __forceinline__ float get(int j) const { return to_f32(reinterpret_cast<const T*>(w)[j]); }
+    __device__ __forceinline__ void set(int j, float v) { reinterpret_cast<T*>(w)[j] = from_f32<T>(v); }
+};
 // The vector unit of a pair of types: 8 bf16 or 4 f32 fill 16 bytes.
 template <typename A, typename B>
 constexpr int kVectorUnit = sizeof(A) == 2 && sizeof(B) == 2 ? 8 : 4;
@@ -95,41 +90,37 @@ struct LookupArgs {
     float scale;
 };
 
-// A group of 2^k lanes, enough for a row's units, takes kRows rows at a time, so
-// that kRows loads of each lane are in flight behind the kRows tokens.  The
-// stores stream past L2, which keeps the table.
+// A group of 2^k lanes, enough for a row's units, takes kRows neighbouring rows
+// at a time, so that kRows loads of each lane are in flight behind the kRows
+// tokens.  The stores stream past L2, which keeps the table.
 template <typename In, typename Out, int kUnit>
-__global__ void __launch_bounds__(kThreads) lookup_kernel(const LookupArgs a, int group) {
+__global__ void __launch_bounds__(kThreads, kLookupCtas) lookup_kernel(const LookupArgs a, int group) {
     constexpr int kRows = 4;
     const int lane = threadIdx.x & (group - 1);
     const int units = a.width / kUnit;
     const int64_t groups = static_cast<int64_t>(gridDim.x) * (kThreads / group);
     const int64_t first = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / group;
-    for (int64_t r0 = first; r0 < a.tokens.n; r0 += groups * kRows) {
+    for (int64_t r0 = first * kRows; r0 < a.tokens.n; r0 += groups * kRows) {
+        const int rows = static_cast<int>(min(static_cast<int64_t>(kRows), a.tokens.n - r0));
         int token[kRows];
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-            const int64_t r = r0 + i * groups;
-            token[i] = r < a.tokens.n ? a.tokens(static_cast<int>(r)) : a.tokens.vocab;
-        }
+        for (int i = 0; i < kRows; ++i) token[i] = i < rows ? a.tokens(static_cast<int>(r0) + i) : a.tokens.vocab;
         for (int u = lane; u < units; u += group) {
-            float v[kRows][kUnit];
+            Raw<In, kUnit> v[kRows];
+            const In* column = static_cast<const In*>(a.table) + u * kUnit;
+#pragma unroll
+            for (int i = 0; i < kRows; ++i)
+                if (token[i] < a.tokens.vocab) v[i].load(column + token[i] * a.table_stride);
+                else v[i].clear();
+            Out* out = static_cast<Out*>(a.out) + r0 * a.out_stride + u * kUnit;
 #pragma unroll
             for (int i = 0; i < kRows; ++i) {
-                if (token[i] < a.tokens.vocab) {
-                    load_unit<In, kUnit>(static_cast<const In*>(a.table) + token[i] * a.table_stride + u * kUnit, v[i]);
+                if (i >= rows) break;
+                Raw<Out, kUnit> y;
 #pragma unroll
-                    for (int j = 0; j < kUnit; ++j) v[i][j] *= a.scale;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < kUnit; ++j) v[i][j] = 0.0f;
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < kRows; ++i) {
-                const int64_t r = r0 + i * groups;
-                if (r < a.tokens.n)
-                    store_unit<Out, kUnit>(static_cast<Out*>(a.out) + r * a.out_stride + u * kUnit, v[i]);
+                for (int j = 0; j < kUnit; ++j) y.set(j, v[i].get(j) * a.scale);
+                y.store(out);
+                out += a.out_stride;
             }
         }
     }
@@ -153,19 +144,24 @@ struct SortPass {
     int* counts;             // [bins][tiles], turned into starts inside a bin
     int* totals;             // [bins]
     int n, tiles, shift, bins;
-    int tile;                // keys of one CTA, a multiple of 32 * kWarps
     __device__ __forceinline__ int key(int i) const { return keys_in != nullptr ? keys_in[i] : tokens(i); }
     __device__ __forceinline__ int digit(int k) const { return (k >> shift) & (bins - 1); }
 };
 
+template <int kSteps>
 __global__ void __launch_bounds__(kThreads) sort_count_kernel(const SortPass s) {
     __shared__ int count[kMaxBins];
     let_next_start();
-    wait_for_previous();
     for (int b = threadIdx.x; b < s.bins; b += kThreads) count[b] = 0;
     __syncthreads();
-    const int first = blockIdx.x * s.tile;
-    for (int i = first + threadIdx.x; i < min(s.n, first + s.tile); i += kThreads) atomicAdd(count + s.digit(s.key(i)), 1);
+    wait_for_previous();
+    const int first = blockIdx.x * (kSteps * kThreads) + threadIdx.x;
+    int key[kSteps];
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) key[j] = first + j * kThreads < s.n ? s.key(first + j * kThreads) : -1;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j)
+        if (key[j] >= 0) atomicAdd(count + s.digit(key[j]), 1);
     __syncthreads();
     for (int b = threadIdx.x; b < s.bins; b += kThreads) s.counts[static_cast<size_t>(b) * s.tiles + blockIdx.x] = count[b];
 }
@@ -211,6 +207,7 @@ __global__ void __launch_bounds__(kThreads) sort_scan_kernel(const SortPass s) {
 // CTA per tile, each warp a run of consecutive keys: a key's place is the start
 // of its bin, its tile's start in the bin, the keys of earlier warps and steps,
 // and its rank among the equal digits of its warp's step.
+template <int kSteps>
 __global__ void __launch_bounds__(kThreads) sort_scatter_kernel(const SortPass s) {
     extern __shared__ int places[];  // [kWarps][bins]
     __shared__ int warp_sums[kWarps];
@@ -220,10 +217,17 @@ __global__ void __launch_bounds__(kThreads) sort_scatter_kernel(const SortPass s
     for (int i = threadIdx.x; i < kWarps * s.bins; i += kThreads) places[i] = 0;
     __syncthreads();
     wait_for_previous();
-    const int per_warp = s.tile / kWarps;
-    const int first = blockIdx.x * s.tile + warp * per_warp;
-    const int end = min(s.n, first + per_warp);
-    for (int i = first + lane; i < end; i += 32) atomicAdd(place + s.digit(s.key(i)), 1);
+    const int first = blockIdx.x * (kSteps * kThreads) + warp * (kSteps * 32) + lane;
+    int key[kSteps], position[kSteps];
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+        const int i = first + j * 32;
+        key[j] = i < s.n ? s.key(i) : -1;
+        position[j] = i < s.n && s.positions_in != nullptr ? s.positions_in[i] : i;
+    }
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j)
+        if (key[j] >= 0) atomicAdd(place + s.digit(key[j]), 1);
     __syncthreads();
     int run = 0;
     for (int b0 = 0; b0 < s.bins; b0 += kThreads) {
@@ -241,18 +245,17 @@ __global__ void __launch_bounds__(kThreads) sort_scatter_kernel(const SortPass s
         }
     }
     __syncthreads();
-    for (int i0 = first; i0 < end; i0 += 32) {
-        const int i = i0 + lane;
-        const unsigned active = __ballot_sync(0xffffffffu, i < end);
-        if (i < end) {
-            const int k = s.key(i);
-            const int d = s.digit(k);
-            const unsigned peers = __match_any_sync(active, d);
-            const int start = place[d];
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+        // lanes past the last key share a digit of their own
+        const int d = key[j] >= 0 ? s.digit(key[j]) : -1;
+        const unsigned peers = __match_any_sync(0xffffffffu, d);
+        const int start = d >= 0 ? place[d] : 0;
+        __syncwarp();  // every lane has read its start
+        if (d >= 0) {
             const int at = start + __popc(peers & ((1u << lane) - 1));
-            s.keys_out[at] = k;
-            s.positions_out[at] = s.positions_in != nullptr ? s.positions_in[i] : i;
-            __syncwarp(active);  // every lane has read `start`
+            s.keys_out[at] = key[j];
+            s.positions_out[at] = position[j];
             if (lane == 31 - __clz(peers)) place[d] = start + __popc(peers);
         }
         __syncwarp();
@@ -306,18 +309,19 @@ __device__ void write_empty_rows(const GradientArgs& a, int block) {
         empty[threadIdx.x] = none;
     }
     __syncthreads();
-    const float zeros[kUnit] = {};
+    Raw<Out, kUnit> zeros;
+    zeros.clear();
     for (int r = threadIdx.x >> 5; r < kEmptyRows; r += kWarps) {
         if (!empty[r]) continue;
         Out* out = static_cast<Out*>(a.out) + (v0 + r) * a.out_stride;
-        for (int u = threadIdx.x & 31; u < a.width / kUnit; u += 32) store_unit<Out, kUnit>(out + u * kUnit, zeros);
+        for (int u = threadIdx.x & 31; u < a.width / kUnit; u += 32) zeros.store(out + u * kUnit);
     }
 }
 
 // kLanes lanes hold kUnits units of a row each; blockIdx.y cuts wider rows.
 template <typename In, typename Out, int kUnit, int kLanes, int kUnits>
-__global__ void __launch_bounds__(kThreads) gradient_kernel(const GradientArgs a) {
-    constexpr int kBatch = kUnit * kUnits > 8 ? 4 : 8;  // rows in flight
+__global__ void __launch_bounds__(kThreads, 3) gradient_kernel(const GradientArgs a) {
+    constexpr int kBatch = 4;  // rows in flight
     let_next_start();
     wait_for_previous();
     if (static_cast<int>(blockIdx.x) < a.row_blocks) {
@@ -342,13 +346,15 @@ __global__ void __launch_bounds__(kThreads) gradient_kernel(const GradientArgs a
                 const int u = u0 + k * kLanes;
                 if (u >= units) continue;
                 if (part != nullptr) {
+                    Raw<float, kUnit> v;
 #pragma unroll
-                    for (int j = 0; j < kUnit; ++j) part[static_cast<size_t>(c) * a.width + u * kUnit + j] = sum[k][j];
+                    for (int j = 0; j < kUnit; ++j) v.set(j, sum[k][j]);
+                    v.store(part + static_cast<size_t>(c) * a.width + u * kUnit);
                 } else {
-                    float v[kUnit];
+                    Raw<Out, kUnit> v;
 #pragma unroll
-                    for (int j = 0; j < kUnit; ++j) v[j] = sum[k][j] * a.scale;
-                    store_unit<Out, kUnit>(static_cast<Out*>(a.out) + current * a.out_stride + u * kUnit, v);
+                    for (int j = 0; j < kUnit; ++j) v.set(j, sum[k][j] * a.scale);
+                    v.store(static_cast<Out*>(a.out) + current * a.out_stride + u * kUnit);
                 }
             }
         }
@@ -368,7 +374,7 @@ __global__ void __launch_bounds__(kThreads) gradient_kernel(const GradientArgs a
     };
     fetch(begin);
     for (int i0 = begin; i0 < end; i0 += kBatch) {
-        float v[kBatch][kUnits][kUnit];
+        Raw<In, kUnit> v[kBatch][kUnits];
         int k_now[kBatch];
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
@@ -377,12 +383,8 @@ __global__ void __launch_bounds__(kThreads) gradient_kernel(const GradientArgs a
 #pragma unroll
             for (int k = 0; k < kUnits; ++k) {
                 const int u = u0 + k * kLanes;
-                if (key[b] < a.vocab && u < units) {
-                    load_unit<In, kUnit>(row + u * kUnit, v[b][k]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < kUnit; ++j) v[b][k][j] = 0.0f;
-                }
+                if (key[b] < a.vocab && u < units) v[b][k].load(row + u * kUnit);
+                else v[b][k].clear();
             }
         }
         fetch(i0 + kBatch);
@@ -397,7 +399,7 @@ __global__ void __launch_bounds__(kThreads) gradient_kernel(const GradientArgs a
 #pragma unroll
             for (int k = 0; k < kUnits; ++k)
 #pragma unroll
-                for (int j = 0; j < kUnit; ++j) sum[k][j] += v[b][k][j];
+                for (int j = 0; j < kUnit; ++j) sum[k][j] += v[b][k].get(j);
         }
     }
     flush(current == after);
@@ -406,12 +408,13 @@ __global__ void __launch_bounds__(kThreads) gradient_kernel(const GradientArgs a
 // CTA for kWarps chunks: the rows whose run begins in a chunk and goes on after
 // it.  Runs over up to kShortRun more chunks take a warp each; longer ones are
 // shared by the CTA's warps, each a run of consecutive chunks, and joined in
-// that order.
+// that order.  A lane takes eight columns at a time, whose loads do not wait
+// for one another.
 template <typename Out>
 __global__ void __launch_bounds__(kThreads) joined_rows_kernel(const GradientArgs a) {
-    constexpr int kShortRun = 16;
+    constexpr int kShortRun = 8, kColumns = 8, kBlock = 32 * kColumns;
     __shared__ int first_key[kWarps], more[kWarps];  // of each chunk's tail run: its row, the chunks after it
-    __shared__ float part[kWarps][32];
+    __shared__ float part[kWarps][kBlock];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     wait_for_previous();
     const int c0 = blockIdx.x * kWarps;
@@ -424,46 +427,56 @@ __global__ void __launch_bounds__(kThreads) joined_rows_kernel(const GradientArg
             const bool begun_here = !(begin > 0 && a.keys[begin] == k && a.keys[begin - 1] == k);
             if (k < a.vocab && a.keys[last + 1] == k && begun_here) {
                 row = k;
-                // the chunk that holds the run's last entry
-                count = (lower_bound(a.keys, a.n, k + 1) - 1) / a.chunk - c;
+                // up to the chunk that holds the run's last entry
+                int next = c + 1;
+                while (next < a.chunks - 1 && next - c <= kShortRun && a.keys[next * a.chunk + a.chunk] == k) ++next;
+                count = next - c <= kShortRun ? next - c : (lower_bound(a.keys, a.n, k + 1) - 1) / a.chunk - c;
             }
         }
         first_key[threadIdx.x] = row;
         more[threadIdx.x] = count;
     }
     __syncthreads();
-    auto sum_heads = [&](int first, int count, int column) {
-        float s = 0.0f;
-        int i = 0;
-        for (; i + 8 <= count; i += 8) {
-            float v[8];
+    auto add_heads = [&](int first, int count, int base, float* s) {
+        const float* row = a.heads + static_cast<size_t>(first) * a.width + base + lane;
+#pragma unroll 2
+        for (int i = 0; i < count; ++i, row += a.width)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = a.heads[static_cast<size_t>(first + i + j) * a.width + column];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s += v[j];
-        }
-        for (; i < count; ++i) s += a.heads[static_cast<size_t>(first + i) * a.width + column];
-        return s;
+            for (int j = 0; j < kColumns; ++j)
+                if (base + lane + 32 * j < a.width) s[j] += row[32 * j];
     };
-    if (first_key[warp] >= 0 && more[warp] <= kShortRun) {
-        const int c = c0 + warp;
-        for (int column = lane; column < a.width; column += 32) {
-            const float s = a.tails[static_cast<size_t>(c) * a.width + column] + sum_heads(c + 1, more[warp], column);
-            static_cast<Out*>(a.out)[first_key[warp] * a.out_stride + column] = from_f32<Out>(s * a.scale);
+    auto finish = [&](int c, int key, int base, float* s) {
+#pragma unroll
+        for (int j = 0; j < kColumns; ++j) {
+            const int column = base + lane + 32 * j;
+            if (column < a.width)
+                static_cast<Out*>(a.out)[key * a.out_stride + column] =
+                    from_f32<Out>((a.tails[static_cast<size_t>(c) * a.width + column] + s[j]) * a.scale);
         }
-    }
+    };
+    if (first_key[warp] >= 0 && more[warp] <= kShortRun)
+        for (int base = 0; base < a.width; base += kBlock) {
+            float s[kColumns] = {};
+            add_heads(c0 + warp + 1, more[warp], base, s);
+            finish(c0 + warp, first_key[warp], base, s);
+        }
     for (int w = 0; w < kWarps; ++w) {
         if (first_key[w] < 0 || more[w] <= kShortRun) continue;
-        const int c = c0 + w, share = (more[w] + kWarps - 1) / kWarps;
+        const int share = (more[w] + kWarps - 1) / kWarps;
         const int first = min(more[w], warp * share), count = min(more[w], first + share) - first;
-        for (int base = 0; base < a.width; base += 32) {
-            const int column = base + lane;
-            part[warp][lane] = column < a.width ? sum_heads(c + 1 + first, count, column) : 0.0f;
+        for (int base = 0; base < a.width; base += kBlock) {
+            float s[kColumns] = {};
+            add_heads(c0 + w + 1 + first, count, base, s);
+#pragma unroll
+            for (int j = 0; j < kColumns; ++j) part[warp][lane + 32 * j] = s[j];
             __syncthreads();
-            if (warp == 0 && column < a.width) {
-                float s = a.tails[static_cast<size_t>(c) * a.width + column];
-                for (int x = 0; x < kWarps; ++x) s += part[x][lane];
-                static_cast<Out*>(a.out)[first_key[w] * a.out_stride + column] = from_f32<Out>(s * a.scale);
+            if (warp == 0) {
+#pragma unroll
+                for (int j = 0; j < kColumns; ++j) {
+                    s[j] = 0.0f;
+                    for (int x = 0; x < kWarps; ++x) s[j] += part[x][lane + 32 * j];
+                }
+                finish(c0 + w, first_key[w], base, s);
             }
             __syncthreads();
         }
@@ -505,14 +518,16 @@ GradientPlan plan_gradient(const BulletOuCudaCppContext* ctx, int n, int vocab, 
     p.tile = n >= kMaxTile * ctx->sm_count ? kMaxTile : kMaxTile / 2;  // a CTA for every SM while there are tokens enough
     p.tiles = (n + p.tile - 1) / p.tile;
     p.row = (static_cast<size_t>(n) + 63) / 64 * 64;
-    p.counts = (static_cast<size_t>(1) << p.digit_bits) * p.tiles;
-    p.width = width;
+    p.counts = ((static_cast<size_t>(1) << p.digit_bits) * p.tiles + 63) / 64 * 64;
+    p.width = (static_cast<size_t>(width) + 3) / 4 * 4;  // partial rows in whole units
     p.unit = vector ? vector_unit : 1;
     const int units = width / p.unit;
     p.lanes = units <= 4 ? 4 : units <= 8 ? 8 : units <= 16 ? 16 : 32;
-    // 8 values for each lane, so that 8 rows in flight fit the registers
-    p.units = std::min(8 / p.unit, (units + p.lanes - 1) / p.lanes);
-    p.units = p.units >= 8 ? 8 : p.units >= 4 ? 4 : p.units >= 2 ? 2 : 1;
+    // up to 8 values for each lane (5 single ones), so that 4 rows in flight fit
+    // the registers; a wider row is cut into equal parts
+    const int most = p.unit == 1 ? 5 : 8 / p.unit;
+    const int parts = (units + p.lanes * most - 1) / (p.lanes * most);
+    p.units = (units + p.lanes * parts - 1) / (p.lanes * parts);
     // Chunks long enough that the two partial rows of each cost little, short
     // enough that every SM has its 64 warps.
     const int64_t groups = static_cast<int64_t>(ctx->sm_count) * 64 * 32 / p.lanes;
@@ -527,7 +542,6 @@ int sort_tokens(BulletOuCudaCppContext* ctx, const Tokens& tokens, const Gradien
     SortPass s{};
     s.tokens = tokens;
     s.n = tokens.n;
-    s.tile = plan.tile;
     s.tiles = plan.tiles;
     s.bins = 1 << plan.digit_bits;
     s.totals = base + 4 * plan.row;
@@ -536,15 +550,18 @@ int sort_tokens(BulletOuCudaCppContext* ctx, const Tokens& tokens, const Gradien
         s.shift = pass * plan.digit_bits;
         s.keys_out = base + (pass & 1) * 2 * plan.row;
         s.positions_out = s.keys_out + plan.row;
+        const bool large = plan.tile == kMaxTile;
         LaunchShape shape{dim3(plan.tiles), kThreads};
         shape.chained = pass > 0;
-        if (launch_kernel(ctx, "embedding sort launch", sort_count_kernel, shape, s) != 0) return -1;
+        if (launch_kernel(ctx, "embedding sort launch", large ? sort_count_kernel<kMaxTile / kThreads> : sort_count_kernel<kMaxTile / kThreads / 2>, shape, s) != 0)
+            return -1;
         shape.chained = true;
         shape.grid = dim3(s.bins);
         if (launch_kernel(ctx, "embedding sort launch", sort_scan_kernel, shape, s) != 0) return -1;
         shape.grid = dim3(plan.tiles);
         shape.smem = static_cast<size_t>(kWarps) * s.bins * sizeof(int);
-        if (launch_kernel(ctx, "embedding sort launch", sort_scatter_kernel, shape, s) != 0) return -1;
+        if (launch_kernel(ctx, "embedding sort launch", large ? sort_scatter_kernel<kMaxTile / kThreads> : sort_scatter_kernel<kMaxTile / kThreads / 2>, shape, s) != 0)
+            return -1;
         s.keys_in = s.keys_out;
         s.positions_in = s.positions_out;
     }
@@ -573,8 +590,9 @@ int launch_gradient_unit(BulletOuCudaCppContext* ctx, const GradientArgs& a, con
     if (p.lanes == 8) return launch_gradient<In, Out, kUnit, 8, 1>(ctx, a);
     if (p.lanes == 16) return launch_gradient<In, Out, kUnit, 16, 1>(ctx, a);
     if constexpr (kUnit == 1) {
-        if (p.units == 8) return launch_gradient<In, Out, 1, 32, 8>(ctx, a);
+        if (p.units == 5) return launch_gradient<In, Out, 1, 32, 5>(ctx, a);
         if (p.units == 4) return launch_gradient<In, Out, 1, 32, 4>(ctx, a);
+        if (p.units == 3) return launch_gradient<In, Out, 1, 32, 3>(ctx, a);
     }
     if constexpr (kUnit <= 4) {
         if (p.units == 2) return launch_gradient<In, Out, kUnit, 32, 2>(ctx, a);
@@ -614,7 +632,7 @@ int lookup(BulletOuCudaCppContext* ctx, const LookupArgs& a, const BulletOuB200M
     int group = 1;
     while (group < 32 && group < units) group *= 2;
     const int64_t blocks = (static_cast<int64_t>(a.tokens.n) * group + kThreads - 1) / kThreads;
-    const LaunchShape shape{dim3(static_cast<unsigned>(std::min<int64_t>(blocks, ctx->sm_count * 8))), kThreads};
+    const LaunchShape shape{dim3(static_cast<unsigned>(std::min<int64_t>(blocks, ctx->sm_count * kLookupCtas))), kThreads};
     if (vector) return launch_kernel(ctx, "embedding lookup launch", lookup_kernel<In, Out, kVectorUnit<In, Out>>, shape, a, group);
     return launch_kernel(ctx, "embedding lookup launch", lookup_kernel<In, Out, 1>, shape, a, group);
 }

@@ -37,49 +37,54 @@ struct QuantizeArgs {
 
 constexpr int kGroup = 16;  // columns that a thread takes together: a 16-byte store of q
 
+// kGroup values of a row as they are in memory.
 template <typename T>
-__device__ __forceinline__ void load_group(const T* x, int c, int cols, bool vector, float* v) {
-    if (vector && c + kGroup <= cols) {
-        constexpr int kVec = 16 / sizeof(T);
+struct Group {
+    uint4 raw[kGroup * sizeof(T) / 16];
+    __device__ __forceinline__ void load(const T* x, int c, int cols, bool vector) {
+        if (vector && c + kGroup <= cols) {
 #pragma unroll
-        for (int i = 0; i < kGroup; i += kVec) {
-            const uint4 raw = __ldcs(reinterpret_cast<const uint4*>(x + c + i));
-            const T* e = reinterpret_cast<const T*>(&raw);
+            for (int i = 0; i < static_cast<int>(kGroup * sizeof(T) / 16); ++i)
+                raw[i] = __ldcs(reinterpret_cast<const uint4*>(x + c) + i);
+        } else {
+            T* e = reinterpret_cast<T*>(raw);
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) v[i + j] = to_f32(e[j]);
+            for (int i = 0; i < kGroup; ++i) e[i] = c + i < cols ? x[c + i] : from_f32<T>(0.0f);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < kGroup; ++i) v[i] = c + i < cols ? to_f32(x[c + i]) : 0.0f;
     }
-}
-
-__device__ __forceinline__ void store_group(const QuantizeArgs& a, int8_t* q, int c, const float* v, float factor, bool some) {
-    int8_t b[kGroup];
+    __device__ __forceinline__ float get(int i) const { return to_f32(reinterpret_cast<const T*>(raw)[i]); }
+    // max |x|; NaN becomes +inf
+    __device__ __forceinline__ float top() const {
+        float t = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kGroup; ++i) b[i] = static_cast<int8_t>(some ? quantised(v[i], factor) : 0);
-    if (a.q_vector) {
-        uint4 packed;
-        uint32_t* w = reinterpret_cast<uint32_t*>(&packed);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            w[i] = static_cast<uint8_t>(b[4 * i]) | static_cast<uint32_t>(static_cast<uint8_t>(b[4 * i + 1])) << 8 |
-                   static_cast<uint32_t>(static_cast<uint8_t>(b[4 * i + 2])) << 16 |
-                   static_cast<uint32_t>(static_cast<uint8_t>(b[4 * i + 3])) << 24;
-        *reinterpret_cast<uint4*>(q + c) = packed;
-    } else {
-#pragma unroll
-        for (int i = 0; i < kGroup; ++i)
-            if (c + i < a.padded_cols) q[c + i] = b[i];
+        for (int i = 0; i < kGroup; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(t) : "f"(fabsf(get(i))));
+        return t == t ? t : INFINITY;
     }
-}
+    __device__ __forceinline__ void store(const QuantizeArgs& a, int8_t* q, int c, float factor, bool some) const {
+        uint32_t words[kGroup / 4];
+#pragma unroll
+        for (int w = 0; w < kGroup / 4; ++w) {
+            words[w] = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                words[w] |= (static_cast<uint32_t>(quantised(get(4 * w + j), factor)) & 0xffu) << (8 * j);
+            if (!some) words[w] = 0;
+        }
+        if (a.q_vector) {
+            *reinterpret_cast<uint4*>(q + c) = make_uint4(words[0], words[1], words[2], words[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kGroup; ++i)
+                if (c + i < a.padded_cols) q[c + i] = static_cast<int8_t>(words[i >> 2] >> (8 * (i & 3)));
+        }
+    }
+};
 
-// kRowThreads threads for each row, which holds its values in registers
-// between the maximum and the rounding: x is read once.  Rows longer than
-// 2 * kGroup * kRowThreads (only with kRowThreads == kThreads) read the rest
-// again, from L2.
+// kRowThreads threads for each row, which hold its values in registers between
+// the maximum and the rounding: x is read once.  Rows longer than 2 * kGroup *
+// kRowThreads (only with kRowThreads == kThreads) read the rest again, from L2.
 template <typename T, int kRowThreads>
-__global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) quantize_kernel(const QuantizeArgs a) {
     constexpr int kHeld = 2, kRowWarps = kRowThreads / 32;
     __shared__ float warp_top[kWarps];
     let_next_start();
@@ -87,27 +92,19 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeArgs a
     const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / kRowThreads) + threadIdx.x / kRowThreads;
     const bool live = row < a.rows;
     const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.x_stride;
-    float held[kHeld][kGroup];
-    float top = 0.0f;  // NaN and infinities become +inf here
-    auto take = [&](const float* v) {
-#pragma unroll
-        for (int i = 0; i < kGroup; ++i) {
-            const float m = fabsf(v[i]);
-            top = fmaxf(top, m == m ? m : INFINITY);
-        }
-    };
+    Group<T> held[kHeld];
+    float top = 0.0f;
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) {
         const int c = (in_row + j * kRowThreads) * kGroup;
-        if (live && c < a.cols) {
-            load_group(x, c, a.cols, a.x_vector, held[j]);
-            take(held[j]);
-        }
+        held[j].load(x, c, live ? a.cols : 0, a.x_vector);
     }
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) top = fmaxf(top, held[j].top());
     for (int c = (in_row + kHeld * kRowThreads) * kGroup; live && c < a.cols; c += kRowThreads * kGroup) {
-        float v[kGroup];
-        load_group(x, c, a.cols, a.x_vector, v);
-        take(v);
+        Group<T> g;
+        g.load(x, c, a.cols, a.x_vector);
+        top = fmaxf(top, g.top());
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
@@ -125,12 +122,12 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const QuantizeArgs a
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) {
         const int c = (in_row + j * kRowThreads) * kGroup;
-        if (c < a.padded_cols) store_group(a, q, c, held[j], factor, some && c < a.cols);
+        if (c < a.padded_cols) held[j].store(a, q, c, factor, some);
     }
     for (int c = (in_row + kHeld * kRowThreads) * kGroup; c < a.padded_cols; c += kRowThreads * kGroup) {
-        float v[kGroup];
-        load_group(x, c, a.cols, a.x_vector, v);
-        store_group(a, q, c, v, factor, some);
+        Group<T> g;
+        g.load(x, c, a.cols, a.x_vector);
+        g.store(a, q, c, factor, some);
     }
     if (in_row == 0) a.scales[row] = top == INFINITY ? NAN : some ? row_scale(top) : 0.0f;
 }

@@ -21,7 +21,7 @@
 namespace bou {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxExperts = BULLETOU_B200_ROUTER_MAX_EXPERTS;
 constexpr int kMaxTopK = BULLETOU_B200_ROUTER_MAX_TOP_K;
@@ -51,11 +51,24 @@ struct RouterArgs {
     size_t logit_grad_stride;
 };
 
-// Sums and maxima over the kGroup lanes that share a row.
+// 2^x to about two units in the last place, and a maximum that keeps NaN.
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+constexpr float kLog2E = 1.4426950408889634f;
+
+// Over the kGroup lanes that share a row.
 template <int kGroup>
 __device__ __forceinline__ float group_max(float v) {
 #pragma unroll
-    for (int d = kGroup / 2; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+    for (int d = kGroup / 2; d > 0; d >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, d));
     return v;
 }
 template <int kGroup>
@@ -64,47 +77,49 @@ __device__ __forceinline__ float group_sum(float v) {
     for (int d = kGroup / 2; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
     return v;
 }
+template <int kGroup>
+__device__ __forceinline__ int group_min(int v) {
+#pragma unroll
+    for (int d = kGroup / 2; d > 0; d >>= 1) v = min(v, __shfl_xor_sync(0xffffffffu, v, d));
+    return v;
+}
 
-// A row's logits and probabilities: expert e in lane e % kGroup, place
-// e / kGroup.  All lanes of a warp come here together; a row past the end is
-// one that is not alive.
+// A row's logits and their exponentials: expert e in lane e % kGroup, place
+// e / kGroup; places past the last expert hold -inf and 0.  All lanes of a warp
+// come here together; a row past the end is one that is not alive.
+//
+// exp(z - top) is taken as 2^((z - top) log2 e): two roundings of 2^-24 relative
+// in an exponent below 20 wherever p > 10^-6.
 template <int kGroup, int kPlaces>
 struct Row {
     float z[kPlaces];
-    float p[kPlaces];
-    float top, inverse;  // p = exp(z - top) * inverse
-    bool alive;          // the largest logit is finite
+    float e[kPlaces];
+    float top, shift, inverse;  // p = e * inverse, e = exp(z - shift); shift is top where that is finite
+    bool alive;                 // the largest logit is finite
+
+    __device__ __forceinline__ float exponential(float logit) const { return exp2_approx((logit - shift) * kLog2E); }
 
     template <typename T>
     __device__ __forceinline__ void load(const RouterArgs& a, int64_t t, int lane) {
-        const T* src = static_cast<const T*>(a.logits) + (t < a.rows ? t : 0) * a.logit_stride;
-        bool nan = false;
-        top = -INFINITY;
+        const T* src = static_cast<const T*>(a.logits) + t * a.logit_stride + lane;
+        const int mine = t < a.rows ? a.experts - lane : 0;
 #pragma unroll
-        for (int i = 0; i < kPlaces; ++i) {
-            const int e = lane + kGroup * i;
-            z[i] = t < a.rows && e < a.experts ? to_f32(src[e]) : -INFINITY;
-        }
+        for (int i = 0; i < kPlaces; ++i) z[i] = kGroup * i < mine ? to_f32(src[kGroup * i]) : -INFINITY;
+        top = z[0];
 #pragma unroll
-        for (int i = 0; i < kPlaces; ++i) {
-            nan |= z[i] != z[i];
-            top = fmaxf(top, z[i]);
-        }
-        // NaN goes through the maximum as +inf: both break the row alike
-        top = group_max<kGroup>(nan ? INFINITY : top);
+        for (int i = 1; i < kPlaces; ++i) top = max_nan(top, z[i]);
+        top = group_max<kGroup>(top);
         alive = top > -INFINITY && top < INFINITY;
-        const float shift = alive ? top : 0.0f;
+        shift = alive ? top : 0.0f;
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < kPlaces; ++i) {
-            p[i] = expf(z[i] - shift);
-            sum += p[i];
+            e[i] = exponential(z[i]);
+            sum += e[i];
         }
         sum = group_sum<kGroup>(sum);
         // a masked row's exponentials are zeros; a broken row is NaN
-        inverse = alive ? 1.0f / sum : top == INFINITY ? NAN : 0.0f;
-#pragma unroll
-        for (int i = 0; i < kPlaces; ++i) p[i] = lane + kGroup * i < a.experts ? p[i] * inverse : 0.0f;
+        inverse = alive ? 1.0f / sum : top == -INFINITY ? 0.0f : NAN;
     }
 };
 
@@ -156,39 +171,32 @@ __global__ void __launch_bounds__(kThreads) router_forward_kernel(const RouterAr
         Row<kGroup, kPlaces> r;
         r.template load<T>(a, t, lane);
 #pragma unroll
-        for (int i = 0; i < kPlaces; ++i) acc[i] += r.p[i];
+        for (int i = 0; i < kPlaces; ++i) acc[i] = __fmaf_rn(r.e[i], r.inverse, acc[i]);
         alive += r.alive && lane == 0;
         float total = 0.0f, own = 0.0f;  // lane j keeps the j-th choice
         int pick = -1;
-#pragma unroll 1
-        for (int j = 0; j < a.top_k; ++j) {
-            float best = -INFINITY;
-            int at = kMaxExperts;
+        float best = r.top;
+        for (int j = 0;;) {
+            int at = kMaxExperts;  // the lowest index that has the largest logit left
 #pragma unroll
-            for (int i = 0; i < kPlaces; ++i)
-                if (r.z[i] > best) {
-                    best = r.z[i];
-                    at = lane + kGroup * i;
-                }
-#pragma unroll
-            for (int d = kGroup / 2; d > 0; d >>= 1) {
-                const float z = __shfl_xor_sync(0xffffffffu, best, d);
-                const int e = __shfl_xor_sync(0xffffffffu, at, d);
-                if (z > best || (z == best && e < at)) {
-                    best = z;
-                    at = e;
-                }
-            }
+            for (int i = kPlaces - 1; i >= 0; --i)
+                if (r.z[i] == best) at = lane + kGroup * i;
+            at = group_min<kGroup>(at);
             const bool some = r.alive && best > -INFINITY;
-            const float gate = some ? expf(best - r.top) * r.inverse : 0.0f;
+            const float gate = some ? r.exponential(best) * r.inverse : 0.0f;
             total += gate;
             if (j == lane) {
                 pick = some ? at : -1;
                 own = gate;
             }
+            if (++j >= a.top_k) break;
 #pragma unroll
             for (int i = 0; i < kPlaces; ++i)
                 if (lane + kGroup * i == at) r.z[i] = -INFINITY;
+            best = r.z[0];
+#pragma unroll
+            for (int i = 1; i < kPlaces; ++i) best = fmaxf(best, r.z[i]);
+            best = group_max<kGroup>(best);
         }
         if (lane < a.top_k && t < a.rows) {
             a.chosen[t * a.chosen_stride + lane] = pick;
@@ -233,14 +241,26 @@ __global__ void __launch_bounds__(kJoinThreads) router_join_kernel(const RouterA
     for (int e0 = 0; e0 <= a.experts; e0 += kAtOnce) {
         float p[kAtOnce / 32] = {};
         int c[kAtOnce / 32] = {};
-#pragma unroll 4
-        for (int i = warp; i < parts; i += kJoinWarps) {
+        for (int i0 = warp; i0 < parts; i0 += 4 * kJoinWarps) {
+            float pv[4][kAtOnce / 32];
+            int cv[4][kAtOnce / 32];
 #pragma unroll
-            for (int j = 0; j < kAtOnce / 32; ++j) {
-                const int e = e0 + lane + 32 * j;
-                if (e < a.experts) p[j] += a.part_p[static_cast<size_t>(i) * a.experts + e];
-                if (e <= a.experts) c[j] += a.part_c[static_cast<size_t>(i) * (a.experts + 1) + e];
+            for (int b = 0; b < 4; ++b) {
+                const int i = i0 + b * kJoinWarps;
+#pragma unroll
+                for (int j = 0; j < kAtOnce / 32; ++j) {
+                    const int e = e0 + lane + 32 * j;
+                    pv[b][j] = i < parts && e < a.experts ? a.part_p[static_cast<size_t>(i) * a.experts + e] : 0.0f;
+                    cv[b][j] = i < parts && e <= a.experts ? a.part_c[static_cast<size_t>(i) * (a.experts + 1) + e] : 0;
+                }
             }
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int j = 0; j < kAtOnce / 32; ++j) {
+                    p[j] += pv[b][j];
+                    c[j] += cv[b][j];
+                }
         }
 #pragma unroll
         for (int j = 0; j < kAtOnce / 32; ++j) {
@@ -277,60 +297,54 @@ __global__ void __launch_bounds__(kThreads) router_backward_kernel(const RouterA
         const int e = lane + kGroup * i;
         h[i] = e < a.experts ? static_cast<float>(a.counts[e]) * unit : 0.0f;
     }
+    const T* const logits = static_cast<const T*>(a.logits);
     constexpr int kRows = kThreads / kGroup;
     for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * kRows; t0 < a.rows; t0 += static_cast<int64_t>(gridDim.x) * kRows) {
         const int64_t t = t0 + threadIdx.x / kGroup;
-        // lane j holds the j-th choice
+        // lane j holds the j-th choice: its logit, its pull and its gate's gradient
         int pick = -1;
-        float up = 0.0f;
+        float up = 0.0f, z = -INFINITY, pull = 0.0f;
         if (a.gate_grad != nullptr && lane < a.top_k && t < a.rows) {
             pick = a.chosen[t * a.chosen_stride + lane];
-            up = a.gate_grad[t * a.gate_grad_stride + lane];
+            if (pick >= 0 && pick < a.experts) {
+                up = a.gate_grad[t * a.gate_grad_stride + lane];
+                z = to_f32(logits[t * a.logit_stride + pick]);
+                pull = static_cast<float>(a.counts[pick]) * unit;
+            } else {
+                pick = -1;
+            }
         }
         Row<kGroup, kPlaces> r;
         r.template load<T>(a, t, lane);
-        float direct[kPlaces];  // plain gates: their gradient joins the pull; normalised: p_e (u_e - sum g u) / sum p
-        float total = 0.0f, dot = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kPlaces; ++i) direct[i] = 0.0f;
-        if (a.gate_grad != nullptr) {
-            bool mine[kPlaces] = {};
-#pragma unroll 1
-            for (int j = 0; j < a.top_k; ++j) {
-                const int e = __shfl_sync(0xffffffffu, pick, j, kGroup);
-                const float u = __shfl_sync(0xffffffffu, up, j, kGroup);
-#pragma unroll
-                for (int i = 0; i < kPlaces; ++i)
-                    if (lane + kGroup * i == e && e < a.experts) {
-                        direct[i] = u;
-                        mine[i] = true;
-                    }
-            }
-            if (a.normalize) {
-                float weighted = 0.0f;
-#pragma unroll
-                for (int i = 0; i < kPlaces; ++i) {
-                    total += mine[i] ? r.p[i] : 0.0f;
-                    weighted += mine[i] ? r.p[i] * direct[i] : 0.0f;
-                }
-                total = group_sum<kGroup>(total);
-                weighted = group_sum<kGroup>(weighted);
-                const float scale = total > 0.0f ? 1.0f / total : 0.0f;
-#pragma unroll
-                for (int i = 0; i < kPlaces; ++i) direct[i] = mine[i] ? (direct[i] - weighted * scale) * scale : 0.0f;
-            }
-        }
-        // normalised gates sum to one, so their part has no mean to take off
-#pragma unroll
-        for (int i = 0; i < kPlaces; ++i) dot += r.p[i] * (a.normalize ? h[i] : h[i] + direct[i]);
-        dot = group_sum<kGroup>(dot);
-        if (t >= a.rows) continue;  // the whole group
-        T* dst = static_cast<T*>(a.logit_grad) + t * a.logit_grad_stride;
+        const float p = pick >= 0 ? r.exponential(z) * r.inverse : 0.0f;
+        float dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < kPlaces; ++i) {
-            const int e = lane + kGroup * i;
-            if (e < a.experts) dst[e] = from_f32<T>(r.p[i] * (h[i] + direct[i] - dot));
+            r.e[i] *= r.inverse;
+            dot = __fmaf_rn(r.e[i], h[i], dot);
         }
+        float direct = up;
+        if (a.gate_grad != nullptr) {
+            const float weighted = group_sum<kGroup>(p * up);
+            if (a.normalize) {
+                // p (u - sum g u) / sum p: gates that sum to one take no part in the mean
+                const float total = group_sum<kGroup>(p);
+                const float scale = total > 0.0f ? 1.0f / total : 0.0f;
+                direct = (up - weighted * scale) * scale;
+                dot = group_sum<kGroup>(dot);
+            } else {
+                dot = group_sum<kGroup>(dot) + weighted;
+            }
+        } else {
+            dot = group_sum<kGroup>(dot);
+        }
+        T* const dst = static_cast<T*>(a.logit_grad) + t * a.logit_grad_stride;
+        const int mine = t < a.rows ? a.experts - lane : 0;
+#pragma unroll
+        for (int i = 0; i < kPlaces; ++i)
+            if (kGroup * i < mine) dst[lane + kGroup * i] = from_f32<T>(r.e[i] * (h[i] - dot));
+        __syncwarp();  // the chosen ones are written again, after the lane that had them
+        if (pick >= 0) dst[pick] = from_f32<T>(p * (pull + direct - dot));
     }
 }
 
@@ -361,7 +375,7 @@ int with_shape(const RouterArgs& a, F&& f) {
 int router_grid(const BulletOuCudaCppContext* ctx, int rows, int group) {
     const int per = kThreads / group;
     const int64_t ctas = (static_cast<int64_t>(rows) + per - 1) / per;
-    return ctas <= 4 ? 1 : static_cast<int>(std::min<int64_t>(ctas, static_cast<int64_t>(ctx->sm_count) * 4));
+    return ctas <= 4 ? 1 : static_cast<int>(std::min<int64_t>(ctas, static_cast<int64_t>(ctx->sm_count) * 2));
 }
 
 template <typename T>

@@ -15,9 +15,9 @@ stream=torch.cuda.current_stream().cuda_stream)`` shares torch's).
 """
 from __future__ import annotations
 
-from ctypes import byref
+import struct
 
-from ._lib import CudaCppError, Matrix
+from ._lib import CudaCppError
 from .cuda_cpp import Context, F32Buffer, I32Buffer
 
 F32, BF16, I8, I32 = "f32", "bf16", "i8", "i32"
@@ -26,7 +26,12 @@ _TYPE_BYTES = {F32: 4, BF16: 2, I8: 1, I32: 4}
 _TORCH_TYPES: dict = {}  # torch dtype -> type id, filled when the first tensor comes
 
 
-class DeviceMatrix(Matrix):
+# BulletOuB200Matrix as bytes (the type is followed by padding): a call reads
+# it before it returns, and building it costs a quarter of a ctypes structure.
+_pack = struct.Struct("=QiiQQQ").pack
+
+
+class DeviceMatrix:
     """rows x cols elements of a library buffer from element `offset` on, rows
     `row_stride` elements apart (default: without a gap).  bf16 and i8 elements
     live packed in an I32Buffer, as the quantised tensors do."""
@@ -45,47 +50,49 @@ class DeviceMatrix(Matrix):
         if used > held:
             raise CudaCppError(f"matrix of {rows} x {cols} {type} (row stride {stride}, offset {offset}) needs {used} "
                                f"elements, the buffer holds {held}")
-        super().__init__((buffer.device_ptr() or 0) + offset * _TYPE_BYTES[type], _TYPE_IDS[type], rows, cols, stride)
-        self.buffer = buffer  # keeps the memory
+        self.buffer, self.type, self.rows, self.cols, self.row_stride = buffer, type, rows, cols, stride
+        self.data = (buffer.device_ptr() or 0) + offset * _TYPE_BYTES[type]
         self.device = buffer.ctx.device
+        self.packed = _pack(self.data, _TYPE_IDS[type], 0, rows, cols, stride)
 
 
-def _torch_matrix(t, ctx: Context) -> Matrix:
-    if not _TORCH_TYPES:
+def _tensor(t, device: int) -> bytes:
+    """A torch tensor of one (a row) or two dimensions."""
+    kind = _TORCH_TYPES.get(t.dtype)
+    if kind is None:
+        if _TORCH_TYPES:
+            raise CudaCppError(f"tensor type {t.dtype} is not supported")
         import torch
 
         _TORCH_TYPES.update({torch.float32: 0, torch.bfloat16: 1, torch.int8: 2, torch.int32: 3})
-    kind = _TORCH_TYPES.get(t.dtype)
-    if kind is None:
-        raise CudaCppError(f"tensor type {t.dtype} is not supported")
-    if not t.is_cuda or t.get_device() != ctx.device:
-        raise CudaCppError(f"tensor is on {t.device}, the context on cuda:{ctx.device}")
+        return _tensor(t, device)
+    if t.get_device() != device:
+        raise CudaCppError(f"tensor is on {t.device}, the context on cuda:{device}")
     shape, stride = t.shape, t.stride()
-    n = len(shape)
-    if n == 2:
+    if len(shape) == 2:
         rows, cols = shape
-        if cols > 1 and stride[1] != 1 and rows:
+        if stride[1] != 1 and cols > 1 and rows:
             raise CudaCppError(f"tensor of strides {stride}: its last dimension must be contiguous")
-        return Matrix(t.data_ptr(), kind, rows, cols, stride[0])
-    if n != 1 or (shape[0] > 1 and stride[0] != 1):
+        return _pack(t.data_ptr(), kind, 0, rows, cols, stride[0])
+    if len(shape) != 1 or (stride[0] != 1 and shape[0] > 1):
         raise CudaCppError(f"tensor of shape {tuple(shape)} and strides {stride}: one or two dimensions, the last one "
                            "contiguous, are supported")
-    return Matrix(t.data_ptr(), kind, 1, shape[0], shape[0])
+    return _pack(t.data_ptr(), kind, 0, 1, shape[0], shape[0])
 
 
 def _matrix(x, ctx: Context):
-    """Pointer to the C view of an operand (None stays None)."""
+    """The C view of an operand (None stays None)."""
     if x is None:
         return None
-    if hasattr(x, "data_ptr"):
-        return byref(_torch_matrix(x, ctx))
+    if isinstance(x, DeviceMatrix):
+        if x.device != ctx.device:
+            raise CudaCppError(f"matrix is on device {x.device}, the context on {ctx.device}")
+        return x.packed
     if isinstance(x, (F32Buffer, I32Buffer)):
-        x = DeviceMatrix(x, 1, len(x))
-    if not isinstance(x, DeviceMatrix):
+        return _matrix(DeviceMatrix(x, 1, len(x)), ctx)
+    if not hasattr(x, "data_ptr"):
         raise CudaCppError(f"a matrix is expected, got {type(x).__name__}")
-    if x.device != ctx.device:
-        raise CudaCppError(f"matrix is on device {x.device}, the context on {ctx.device}")
-    return byref(x)
+    return _tensor(x, ctx.device)
 
 
 def embedding_forward(ctx: Context, table, tokens, out, *, scale: float = 1.0) -> None:
