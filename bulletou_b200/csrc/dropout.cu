@@ -132,10 +132,49 @@ __global__ void __launch_bounds__(kThreads, kCtas) dropout_vector_kernel(const D
     }
 }
 
-// Any strides and alignment: a warp takes 32 blocks, that is 256 elements in
-// row-major order.  Each lane computes one block's eight decisions; the
-// elements are then read and written 32 neighbours at a time, each lane asking
-// the lane that holds its element's block.
+// Rows of any stride and alignment, wide ones: a warp takes a piece of a row, up
+// to kPiece elements, whose blocks its 32 lanes can compute wherever the piece
+// begins inside a block.  The elements are read and written 32 neighbours at a
+// time, each lane asking the lane that holds its element's block.
+constexpr int kPiece = 31 * kLanes;
+constexpr int kWideRow = 64;  // columns from which a piece fills most of a warp's turns
+
+template <typename T, bool kResidual>
+__global__ void __launch_bounds__(kThreads, kCtas) dropout_row_kernel(const DropoutArgs a, int pieces, int piece) {
+    const int lane = threadIdx.x & 31;
+    const size_t rows = a.n / a.cols, step = static_cast<size_t>(gridDim.x) * (kThreads / 32);
+    for (size_t row = static_cast<size_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); row < rows; row += step)
+        for (int s = blockIdx.y; s < pieces; s += gridDim.y) {
+            const size_t col = static_cast<size_t>(s) * piece;
+            const int count = static_cast<int>(min(static_cast<size_t>(piece), a.cols - col));
+            const T* const x_at = static_cast<const T*>(a.x) + row * a.x_stride + col + lane;
+            const T* const r_at = kResidual ? static_cast<const T*>(a.residual) + row * a.residual_stride + col + lane : nullptr;
+            T* const out = static_cast<T*>(a.out) + row * a.out_stride + col + lane;
+            T x[kLanes], r[kLanes];
+#pragma unroll
+            for (int j = 0; j < kLanes; ++j)
+                if (j * 32 + lane < count) {
+                    x[j] = x_at[j * 32];
+                    if (kResidual) r[j] = r_at[j * 32];
+                }
+            const size_t element = row * a.cols + col;
+            const Philox random = philox_block(element / kLanes + lane, a.offset, a.key);
+            uint32_t mask = 0;
+#pragma unroll
+            for (int j = 0; j < kLanes; ++j) mask |= kept(random, j, a.threshold) ? 1u << j : 0u;
+            const int place = static_cast<int>(element % kLanes) + lane;
+#pragma unroll
+            for (int j = 0; j < kLanes; ++j) {
+                if (j * 32 >= count) break;  // for the whole warp
+                const uint32_t theirs = __shfl_sync(0xffffffffu, mask, (j * 32 + place) >> 3);
+                const float v = (theirs >> (place & 7)) & 1u ? to_f32(x[j]) : 0.0f;
+                if (j * 32 + lane < count) out[j * 32] = from_f32<T>(kResidual ? __fmaf_rn(v, a.factor, to_f32(r[j])) : v * a.factor);
+            }
+        }
+}
+
+// Narrow rows of any stride and alignment: a warp takes 32 blocks, that is 256
+// elements in row-major order over as many rows as they are.
 template <typename T, bool kResidual>
 __global__ void __launch_bounds__(kThreads, kCtas) dropout_kernel(const DropoutArgs a) {
     const int lane = threadIdx.x & 31;
@@ -186,6 +225,15 @@ int launch_dropout(BulletOuCudaCppContext* ctx, const DropoutArgs& a, bool vecto
     const int64_t per_cta = static_cast<int64_t>(kThreads) * kLanes;
     const int64_t ctas = (static_cast<int64_t>(a.n) + per_cta - 1) / per_cta;
     const LaunchShape shape{dim3(static_cast<unsigned>(std::min<int64_t>(ctas, ctx->sm_count * kCtas))), kThreads};
+    if (!vector && a.cols >= kWideRow) {
+        const int64_t rows = static_cast<int64_t>(a.n / a.cols), row_ctas = (rows + kThreads / 32 - 1) / (kThreads / 32);
+        const int pieces = static_cast<int>((a.cols + kPiece - 1) / kPiece);
+        const int piece = static_cast<int>((a.cols + pieces - 1) / pieces);
+        const int64_t resident = static_cast<int64_t>(ctx->sm_count) * kCtas;
+        const unsigned x = static_cast<unsigned>(std::min(row_ctas, resident));
+        const unsigned y = static_cast<unsigned>(std::min<int64_t>(pieces, std::max<int64_t>(1, resident / x)));
+        return launch_kernel(ctx, "dropout launch", dropout_row_kernel<T, kResidual>, LaunchShape{dim3(x, y), kThreads}, a, pieces, piece);
+    }
     if (!vector) return launch_kernel(ctx, "dropout launch", dropout_kernel<T, kResidual>, shape, a);
     if (a.flat) return launch_kernel(ctx, "dropout launch", dropout_vector_kernel<T, kResidual, true>, shape, a);
     return launch_kernel(ctx, "dropout launch", dropout_vector_kernel<T, kResidual, false>, shape, a);

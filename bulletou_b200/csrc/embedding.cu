@@ -9,6 +9,7 @@
 // order: no floating atomics, the same bits from call to call, every row of
 // out_gradients read once and every row of the table written once.
 #include <algorithm>
+#include <utility>
 
 #include "device_matrix.cuh"
 #include "token_launch.cuh"
@@ -27,14 +28,16 @@ struct Tokens {
     int cols;
     size_t row_stride;  // == cols where rows follow one another
     int vocab;
+    __device__ __forceinline__ int checked(int t) const {
+        return static_cast<unsigned>(t) < static_cast<unsigned>(vocab) ? t : vocab;
+    }
     __device__ __forceinline__ int operator()(int i) const {
         size_t at = i;
         if (row_stride != static_cast<size_t>(cols)) {
             const int r = i / cols;
             at = r * row_stride + (i - r * cols);
         }
-        const int t = data[at];
-        return t < 0 || t >= vocab ? vocab : t;
+        return checked(data[at]);
     }
 };
 
@@ -42,7 +45,7 @@ struct Tokens {
 // bytes of the narrower type where the rows allow it, else one element.
 template <typename T, int kUnit>
 struct Raw {
-    static constexpr int kWords = kUnit == 1 ? 1 : kUnit * static_cast<int>(sizeof(T)) / 4;
+    static constexpr int kWords = kUnit == 1 ? 1 : kUnit * static_cast<int>(sizeof(T)) / 4;  // 1, 2, 4 or 8
     uint32_t w[kWords];
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -51,6 +54,8 @@ struct Raw {
     __device__ __forceinline__ void load(const T* p) {
         if constexpr (kUnit == 1) {
             *reinterpret_cast<T*>(w) = *p;
+        } else if constexpr (kWords == 1) {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
         } else if constexpr (kWords == 2) {
             const uint2 u = *reinterpret_cast<const uint2*>(p);
             w[0] = u.x, w[1] = u.y;
@@ -65,6 +70,8 @@ struct Raw {
     __device__ __forceinline__ void store(T* p) const {
         if constexpr (kUnit == 1) {
             *p = *reinterpret_cast<const T*>(w);
+        } else if constexpr (kWords == 1) {
+            __stcs(reinterpret_cast<uint32_t*>(p), w[0]);
         } else if constexpr (kWords == 2) {
             __stcs(reinterpret_cast<uint2*>(p), make_uint2(w[0], w[1]));
         } else {
@@ -90,37 +97,44 @@ struct LookupArgs {
     float scale;
 };
 
-// A group of 2^k lanes, enough for a row's units, takes kRows neighbouring rows
-// at a time, so that kRows loads of each lane are in flight behind the kRows
-// tokens.  The stores stream past L2, which keeps the table.
+// A group of 2^k lanes, enough for a row's units, takes `span` neighbouring rows
+// (at most a row for each lane): each lane fetches one row's token, and the
+// rows' units are then loaded kRows at a time, all in flight together.  The
+// stores stream past L2, which keeps the table.
 template <typename In, typename Out, int kUnit>
-__global__ void __launch_bounds__(kThreads, kLookupCtas) lookup_kernel(const LookupArgs a, int group) {
+__global__ void __launch_bounds__(kThreads, kLookupCtas) lookup_kernel(const LookupArgs a, int group, int span) {
     constexpr int kRows = 4;
     const int lane = threadIdx.x & (group - 1);
-    const int units = a.width / kUnit;
+    // blockIdx.y cuts the columns
+    const int share = (a.width / kUnit + gridDim.y - 1) / gridDim.y;
+    const int unit0 = blockIdx.y * share, units = min(a.width / kUnit, unit0 + share);
     const int64_t groups = static_cast<int64_t>(gridDim.x) * (kThreads / group);
     const int64_t first = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / group;
-    for (int64_t r0 = first * kRows; r0 < a.tokens.n; r0 += groups * kRows) {
-        const int rows = static_cast<int>(min(static_cast<int64_t>(kRows), a.tokens.n - r0));
-        int token[kRows];
+    // the lanes of a warp stay together for the shuffles: a group past the end has no rows
+    for (int64_t r0 = first * span; __any_sync(0xffffffffu, r0 < a.tokens.n); r0 += groups * span) {
+        const int rows = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(span), a.tokens.n - r0)));
+        const int own = lane < rows ? a.tokens(static_cast<int>(r0) + lane) : a.tokens.vocab;
+        const In* const table = static_cast<const In*>(a.table);
+        Out* const out = static_cast<Out*>(a.out) + r0 * a.out_stride;
+        for (int i0 = 0; i0 < span; i0 += kRows) {
+            int token[kRows];
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) token[i] = i < rows ? a.tokens(static_cast<int>(r0) + i) : a.tokens.vocab;
-        for (int u = lane; u < units; u += group) {
-            Raw<In, kUnit> v[kRows];
-            const In* column = static_cast<const In*>(a.table) + u * kUnit;
+            for (int i = 0; i < kRows; ++i) token[i] = __shfl_sync(0xffffffffu, own, i0 + i, group);
+            for (int u = unit0 + lane; u < units; u += group) {
+                Raw<In, kUnit> v[kRows];
 #pragma unroll
-            for (int i = 0; i < kRows; ++i)
-                if (token[i] < a.tokens.vocab) v[i].load(column + token[i] * a.table_stride);
-                else v[i].clear();
-            Out* out = static_cast<Out*>(a.out) + r0 * a.out_stride + u * kUnit;
+                for (int i = 0; i < kRows; ++i) {
+                    if (i0 + i < rows && token[i] < a.tokens.vocab) v[i].load(table + token[i] * a.table_stride + u * kUnit);
+                    else v[i].clear();
+                }
 #pragma unroll
-            for (int i = 0; i < kRows; ++i) {
-                if (i >= rows) break;
-                Raw<Out, kUnit> y;
+                for (int i = 0; i < kRows; ++i) {
+                    if (i0 + i >= rows) break;
+                    Raw<Out, kUnit> y;
 #pragma unroll
-                for (int j = 0; j < kUnit; ++j) y.set(j, v[i].get(j) * a.scale);
-                y.store(out);
-                out += a.out_stride;
+                    for (int j = 0; j < kUnit; ++j) y.set(j, v[i].get(j) * a.scale);
+                    y.store(out + (i0 + i) * a.out_stride + u * kUnit);
+                }
             }
         }
     }
@@ -137,14 +151,13 @@ constexpr int kMaxTile = 2048;
 
 struct SortPass {
     Tokens tokens;           // keys of the first pass
-    const int* keys_in;      // null: the tokens themselves, at positions 0..n-1
-    const int* positions_in;
-    int* keys_out;
-    int* positions_out;
+    const int2* in;          // (token, position); null: the tokens themselves, at positions 0..n-1
+    int2* out;
+    int2* other;             // where the pass after this one goes
     int* counts;             // [bins][tiles], turned into starts inside a bin
     int* totals;             // [bins]
-    int n, tiles, shift, bins;
-    __device__ __forceinline__ int key(int i) const { return keys_in != nullptr ? keys_in[i] : tokens(i); }
+    int n, tiles, shift, digit_bits, bins;
+    __device__ __forceinline__ int2 entry(int i) const { return in != nullptr ? in[i] : make_int2(tokens(i), i); }
     __device__ __forceinline__ int digit(int k) const { return (k >> shift) & (bins - 1); }
 };
 
@@ -158,7 +171,7 @@ __global__ void __launch_bounds__(kThreads) sort_count_kernel(const SortPass s) 
     const int first = blockIdx.x * (kSteps * kThreads) + threadIdx.x;
     int key[kSteps];
 #pragma unroll
-    for (int j = 0; j < kSteps; ++j) key[j] = first + j * kThreads < s.n ? s.key(first + j * kThreads) : -1;
+    for (int j = 0; j < kSteps; ++j) key[j] = first + j * kThreads < s.n ? s.entry(first + j * kThreads).x : -1;
 #pragma unroll
     for (int j = 0; j < kSteps; ++j)
         if (key[j] >= 0) atomicAdd(count + s.digit(key[j]), 1);
@@ -204,61 +217,90 @@ __global__ void __launch_bounds__(kThreads) sort_scan_kernel(const SortPass s) {
     if (threadIdx.x == 0) s.totals[blockIdx.x] = run;
 }
 
-// CTA per tile, each warp a run of consecutive keys: a key's place is the start
-// of its bin, its tile's start in the bin, the keys of earlier warps and steps,
-// and its rank among the equal digits of its warp's step.
-template <int kSteps>
-__global__ void __launch_bounds__(kThreads) sort_scatter_kernel(const SortPass s) {
+// CTA per tile, each warp a run of consecutive entries: an entry's place is the
+// start of its bin, its tile's start in the bin, the entries of earlier warps,
+// and its rank among the equal digits of its warp.  kAlone: one tile holds all
+// entries, so its own counts are all there is and the CTA runs every pass.
+template <int kSteps, bool kAlone>
+__global__ void __launch_bounds__(kThreads) sort_scatter_kernel(SortPass s, int passes) {
+    constexpr int kBinsOfThread = kMaxBins / kThreads;
     extern __shared__ int places[];  // [kWarps][bins]
     __shared__ int warp_sums[kWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int* const place = places + warp * s.bins;
     let_next_start();
-    for (int i = threadIdx.x; i < kWarps * s.bins; i += kThreads) places[i] = 0;
-    __syncthreads();
-    wait_for_previous();
-    const int first = blockIdx.x * (kSteps * kThreads) + warp * (kSteps * 32) + lane;
-    int key[kSteps], position[kSteps];
+    const int per = (s.bins + kThreads - 1) / kThreads, bin0 = threadIdx.x * per;
+    for (int pass = 0; pass < passes; ++pass) {
+        for (int i = threadIdx.x; i < kWarps * s.bins; i += kThreads) places[i] = 0;
+        __syncthreads();
+        if (pass == 0) wait_for_previous();
+        const int first = blockIdx.x * (kSteps * kThreads) + warp * (kSteps * 32) + lane;
+        int2 entry[kSteps];
+        int rank[kSteps];
 #pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-        const int i = first + j * 32;
-        key[j] = i < s.n ? s.key(i) : -1;
-        position[j] = i < s.n && s.positions_in != nullptr ? s.positions_in[i] : i;
-    }
+        for (int j = 0; j < kSteps; ++j) entry[j] = first + j * 32 < s.n ? s.entry(first + j * 32) : make_int2(-1, 0);
+        int total[kBinsOfThread], start[kBinsOfThread];
+        if (!kAlone) {
 #pragma unroll
-    for (int j = 0; j < kSteps; ++j)
-        if (key[j] >= 0) atomicAdd(place + s.digit(key[j]), 1);
-    __syncthreads();
-    int run = 0;
-    for (int b0 = 0; b0 < s.bins; b0 += kThreads) {
-        const int b = b0 + threadIdx.x;
-        int total;
-        int at = run + block_exclusive(b < s.bins ? s.totals[b] : 0, warp_sums, &total);
-        run += total;
-        if (b < s.bins) {
-            at += s.counts[static_cast<size_t>(b) * s.tiles + blockIdx.x];
-            for (int w = 0; w < kWarps; ++w) {
-                const int c = places[w * s.bins + b];
-                places[w * s.bins + b] = at;
-                at += c;
+            for (int i = 0; i < kBinsOfThread; ++i) {
+                const bool in = i < per && bin0 + i < s.bins;
+                total[i] = in ? s.totals[bin0 + i] : 0;
+                start[i] = in ? s.counts[static_cast<size_t>(bin0 + i) * s.tiles + blockIdx.x] : 0;
             }
         }
-    }
-    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-        // lanes past the last key share a digit of their own
-        const int d = key[j] >= 0 ? s.digit(key[j]) : -1;
-        const unsigned peers = __match_any_sync(0xffffffffu, d);
-        const int start = d >= 0 ? place[d] : 0;
-        __syncwarp();  // every lane has read its start
-        if (d >= 0) {
-            const int at = start + __popc(peers & ((1u << lane) - 1));
-            s.keys_out[at] = key[j];
-            s.positions_out[at] = position[j];
-            if (lane == 31 - __clz(peers)) place[d] = start + __popc(peers);
+        for (int j = 0; j < kSteps; ++j) {
+            // the lanes with this lane's digit; those past the last entry go by themselves
+            const bool live = entry[j].x >= 0;
+            const int d = live ? s.digit(entry[j].x) : 0;
+            unsigned peers = __ballot_sync(0xffffffffu, live);
+            peers = live ? peers : ~peers;
+            for (int bit = 1; bit < s.bins; bit <<= 1) {
+                const unsigned set = __ballot_sync(0xffffffffu, d & bit);
+                peers &= d & bit ? set : ~set;
+            }
+            const int before = live ? place[d] : 0;
+            __syncwarp();  // every lane has read it
+            rank[j] = before + __popc(peers & ((1u << lane) - 1));
+            if (live && lane == 31 - __clz(peers)) place[d] = before + __popc(peers);
+            __syncwarp();
         }
-        __syncwarp();
+        __syncthreads();
+        int sum = 0;
+#pragma unroll
+        for (int i = 0; i < kBinsOfThread; ++i) {
+            if (kAlone) {
+                start[i] = total[i] = 0;
+                if (i < per && bin0 + i < s.bins)
+                    for (int w = 0; w < kWarps; ++w) total[i] += places[w * s.bins + bin0 + i];
+            }
+            sum += total[i];
+        }
+        int all;
+        int at = block_exclusive(sum, warp_sums, &all);
+#pragma unroll
+        for (int i = 0; i < kBinsOfThread; ++i) {
+            if (i < per && bin0 + i < s.bins) {
+                int next = at + start[i];
+                for (int w = 0; w < kWarps; ++w) {
+                    const int c = places[w * s.bins + bin0 + i];
+                    places[w * s.bins + bin0 + i] = next;
+                    next += c;
+                }
+            }
+            at += total[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j)
+            if (entry[j].x >= 0) s.out[place[s.digit(entry[j].x)] + rank[j]] = entry[j];
+        if (kAlone) {
+            __syncthreads();
+            s.in = s.out;
+            s.out = s.other;
+            s.other = const_cast<int2*>(s.in);
+            s.shift += s.digit_bits;
+        }
     }
 }
 
@@ -269,27 +311,28 @@ __global__ void __launch_bounds__(kThreads) sort_scatter_kernel(const SortPass s
 // row's gradient and is written; a run that goes on beyond the chunk leaves a
 // partial row, and joined_rows_kernel adds those up in the order of the chunks.
 struct GradientArgs {
-    const int* keys;       // sorted
-    const int* positions;
+    const int2* entries;   // (token, position), sorted by token
     int n, chunk, chunks;
     const void* grad;
     void* out;
     int vocab, width;
     size_t grad_stride, out_stride;
     float scale;
-    float* heads;          // [chunks][width]: the chunk's first run, begun before it
-    float* tails;          // [chunks][width]: the run that begins in the chunk and goes on after it
+    // partial rows, part_stride floats apart (whole 16 bytes), one for each chunk:
+    float* heads;          // the chunk's first run, begun before it
+    float* tails;          // the run that begins in the chunk and goes on after it
+    size_t part_stride;
     int row_blocks;        // CTAs that write the rows no token names
 };
 
 constexpr int kEmptyRows = 128;  // table rows of one such CTA
 
-// First place in the sorted keys whose key is not below `v`.
-__device__ __forceinline__ int lower_bound(const int* keys, int n, int v) {
+// First place in the sorted entries whose token is not below `v`.
+__device__ __forceinline__ int lower_bound(const int2* entries, int n, int v) {
     int lo = 0, hi = n;
     while (lo < hi) {
         const int mid = lo + ((hi - lo) >> 1);
-        if (keys[mid] < v) lo = mid + 1;
+        if (entries[mid].x < v) lo = mid + 1;
         else hi = mid;
     }
     return lo;
@@ -303,8 +346,8 @@ __device__ void write_empty_rows(const GradientArgs& a, int block) {
         const int64_t v = v0 + threadIdx.x;
         bool none = false;
         if (v < a.vocab) {
-            const int at = lower_bound(a.keys, a.n, static_cast<int>(v));
-            none = at == a.n || a.keys[at] != v;
+            const int at = lower_bound(a.entries, a.n, static_cast<int>(v));
+            none = at == a.n || a.entries[at].x != v;
         }
         empty[threadIdx.x] = none;
     }
@@ -334,9 +377,9 @@ __global__ void __launch_bounds__(kThreads, 3) gradient_kernel(const GradientArg
     const int units = a.width / kUnit;
     const int u0 = blockIdx.y * kLanes * kUnits + lane;
     const int begin = c * a.chunk, end = min(a.n, begin + a.chunk);
-    const int before = begin > 0 ? a.keys[begin - 1] : -1, after = end < a.n ? a.keys[end] : -1;
+    const int before = begin > 0 ? a.entries[begin - 1].x : -1, after = end < a.n ? a.entries[end].x : -1;
     float sum[kUnits][kUnit] = {};
-    int current = a.keys[begin];
+    int current = a.entries[begin].x;
     bool from_before = current == before;
     auto flush = [&](bool goes_on) {
         if (current < a.vocab) {
@@ -349,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 3) gradient_kernel(const GradientArg
                     Raw<float, kUnit> v;
 #pragma unroll
                     for (int j = 0; j < kUnit; ++j) v.set(j, sum[k][j]);
-                    v.store(part + static_cast<size_t>(c) * a.width + u * kUnit);
+                    v.store(part + c * a.part_stride + u * kUnit);
                 } else {
                     Raw<Out, kUnit> v;
 #pragma unroll
@@ -363,14 +406,10 @@ __global__ void __launch_bounds__(kThreads, 3) gradient_kernel(const GradientArg
 #pragma unroll
             for (int j = 0; j < kUnit; ++j) sum[k][j] = 0.0f;
     };
-    int key[kBatch], position[kBatch];
+    int2 entry[kBatch];
     auto fetch = [&](int i0) {
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-            const bool in = i0 + b < end;
-            key[b] = in ? a.keys[i0 + b] : a.vocab;
-            position[b] = in ? a.positions[i0 + b] : 0;
-        }
+        for (int b = 0; b < kBatch; ++b) entry[b] = i0 + b < end ? a.entries[i0 + b] : make_int2(a.vocab, 0);
     };
     fetch(begin);
     for (int i0 = begin; i0 < end; i0 += kBatch) {
@@ -378,12 +417,12 @@ __global__ void __launch_bounds__(kThreads, 3) gradient_kernel(const GradientArg
         int k_now[kBatch];
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
-            k_now[b] = key[b];
-            const In* row = static_cast<const In*>(a.grad) + position[b] * a.grad_stride;
+            k_now[b] = entry[b].x;
+            const In* row = static_cast<const In*>(a.grad) + entry[b].y * a.grad_stride;
 #pragma unroll
             for (int k = 0; k < kUnits; ++k) {
                 const int u = u0 + k * kLanes;
-                if (key[b] < a.vocab && u < units) v[b][k].load(row + u * kUnit);
+                if (entry[b].x < a.vocab && u < units) v[b][k].load(row + u * kUnit);
                 else v[b][k].clear();
             }
         }
@@ -408,55 +447,78 @@ __global__ void __launch_bounds__(kThreads, 3) gradient_kernel(const GradientArg
 // CTA for kWarps chunks: the rows whose run begins in a chunk and goes on after
 // it.  Runs over up to kShortRun more chunks take a warp each; longer ones are
 // shared by the CTA's warps, each a run of consecutive chunks, and joined in
-// that order.  A lane takes eight columns at a time, whose loads do not wait
-// for one another.
-template <typename Out>
-__global__ void __launch_bounds__(kThreads) joined_rows_kernel(const GradientArgs a) {
-    constexpr int kShortRun = 8, kColumns = 8, kBlock = 32 * kColumns;
+// that order.  A lane takes eight columns at a time, two 16-byte loads of every
+// partial row.
+template <typename Out, bool kVector>
+__global__ void __launch_bounds__(kThreads, 4) joined_rows_kernel(const GradientArgs a) {
+    constexpr int kShortRun = 8, kQuads = 2, kBlock = 128 * kQuads;
     __shared__ int first_key[kWarps], more[kWarps];  // of each chunk's tail run: its row, the chunks after it
-    __shared__ float part[kWarps][kBlock];
+    __shared__ float4 part[kWarps][32 * kQuads];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     wait_for_previous();
     const int c0 = blockIdx.x * kWarps;
-    if (threadIdx.x < kWarps) {
-        const int c = c0 + threadIdx.x;
+    {
+        const int c = c0 + warp;
         int row = -1, count = 0;
         if (c + 1 < a.chunks) {
             const int begin = c * a.chunk, last = begin + a.chunk - 1;
-            const int k = a.keys[last];
-            const bool begun_here = !(begin > 0 && a.keys[begin] == k && a.keys[begin - 1] == k);
-            if (k < a.vocab && a.keys[last + 1] == k && begun_here) {
+            const int k = a.entries[last].x, next = a.entries[last + 1].x, own = a.entries[begin].x;
+            const int before = begin > 0 ? a.entries[begin - 1].x : -1;
+            if (k < a.vocab && next == k && !(own == k && before == k)) {
                 row = k;
-                // up to the chunk that holds the run's last entry
-                int next = c + 1;
-                while (next < a.chunks - 1 && next - c <= kShortRun && a.keys[next * a.chunk + a.chunk] == k) ++next;
-                count = next - c <= kShortRun ? next - c : (lower_bound(a.keys, a.n, k + 1) - 1) / a.chunk - c;
+                // Chunks [c + 1, c + 1 + count) begin with the row; the lanes ask 32 chunks at a
+                // time, ever closer to the last of them.
+                int lo = c + 1, hi = a.chunks;  // chunk lo begins with it, chunk hi does not (or is past the end)
+                int stride = 1;
+                while (hi - lo > 1) {
+                    const int at = lo + (lane + 1) * stride;
+                    const bool same = at < hi && a.entries[static_cast<int64_t>(at) * a.chunk].x == k;
+                    const int m = __popc(__ballot_sync(0xffffffffu, same));
+                    if (m < 32) hi = static_cast<int>(min(static_cast<int64_t>(hi), lo + static_cast<int64_t>(m + 1) * stride));
+                    lo += m * stride;
+                    stride = (hi - lo + 31) / 32;
+                }
+                count = lo - c;
             }
         }
-        first_key[threadIdx.x] = row;
-        more[threadIdx.x] = count;
+        if (lane == 0) {
+            first_key[warp] = row;
+            more[warp] = count;
+        }
     }
     __syncthreads();
-    auto add_heads = [&](int first, int count, int base, float* s) {
-        const float* row = a.heads + static_cast<size_t>(first) * a.width + base + lane;
-#pragma unroll 2
-        for (int i = 0; i < count; ++i, row += a.width)
+    auto add = [](float4& s, const float4& v) { s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w; };
+    auto add_heads = [&](int first, int count, int base, float4* s) {
+        const float* row = a.heads + first * a.part_stride + base + lane * 4;
+#pragma unroll 4
+        for (int i = 0; i < count; ++i, row += a.part_stride)
 #pragma unroll
-            for (int j = 0; j < kColumns; ++j)
-                if (base + lane + 32 * j < a.width) s[j] += row[32 * j];
+            for (int j = 0; j < kQuads; ++j)
+                if (base + lane * 4 + 128 * j < a.width) add(s[j], *reinterpret_cast<const float4*>(row + 128 * j));
     };
-    auto finish = [&](int c, int key, int base, float* s) {
+    auto finish = [&](int c, int key, int base, float4* s) {
 #pragma unroll
-        for (int j = 0; j < kColumns; ++j) {
-            const int column = base + lane + 32 * j;
-            if (column < a.width)
-                static_cast<Out*>(a.out)[key * a.out_stride + column] =
-                    from_f32<Out>((a.tails[static_cast<size_t>(c) * a.width + column] + s[j]) * a.scale);
+        for (int j = 0; j < kQuads; ++j) {
+            const int column = base + lane * 4 + 128 * j;
+            if (column >= a.width) continue;
+            add(s[j], *reinterpret_cast<const float4*>(a.tails + c * a.part_stride + column));
+            const float v[4] = {s[j].x, s[j].y, s[j].z, s[j].w};
+            Out* out = static_cast<Out*>(a.out) + key * a.out_stride + column;
+            if constexpr (kVector) {
+                Raw<Out, 4> y;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y.set(i, v[i] * a.scale);
+                y.store(out);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (column + i < a.width) out[i] = from_f32<Out>(v[i] * a.scale);
+            }
         }
     };
     if (first_key[warp] >= 0 && more[warp] <= kShortRun)
         for (int base = 0; base < a.width; base += kBlock) {
-            float s[kColumns] = {};
+            float4 s[kQuads] = {};
             add_heads(c0 + warp + 1, more[warp], base, s);
             finish(c0 + warp, first_key[warp], base, s);
         }
@@ -465,16 +527,16 @@ __global__ void __launch_bounds__(kThreads) joined_rows_kernel(const GradientArg
         const int share = (more[w] + kWarps - 1) / kWarps;
         const int first = min(more[w], warp * share), count = min(more[w], first + share) - first;
         for (int base = 0; base < a.width; base += kBlock) {
-            float s[kColumns] = {};
+            float4 s[kQuads] = {};
             add_heads(c0 + w + 1 + first, count, base, s);
 #pragma unroll
-            for (int j = 0; j < kColumns; ++j) part[warp][lane + 32 * j] = s[j];
+            for (int j = 0; j < kQuads; ++j) part[warp][lane + 32 * j] = s[j];
             __syncthreads();
             if (warp == 0) {
 #pragma unroll
-                for (int j = 0; j < kColumns; ++j) {
-                    s[j] = 0.0f;
-                    for (int x = 0; x < kWarps; ++x) s[j] += part[x][lane + 32 * j];
+                for (int j = 0; j < kQuads; ++j) {
+                    s[j] = part[0][lane + 32 * j];
+                    for (int x = 1; x < kWarps; ++x) add(s[j], part[x][lane + 32 * j]);
                 }
                 finish(c0 + w, first_key[w], base, s);
             }
@@ -515,7 +577,8 @@ GradientPlan plan_gradient(const BulletOuCudaCppContext* ctx, int n, int vocab, 
     while (static_cast<int64_t>(vocab) >> bits != 0) ++bits;
     p.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
     p.digit_bits = (bits + p.passes - 1) / p.passes;
-    p.tile = n >= kMaxTile * ctx->sm_count ? kMaxTile : kMaxTile / 2;  // a CTA for every SM while there are tokens enough
+    // a CTA for every SM while there are tokens enough; one alone where it can hold them all
+    p.tile = n <= kMaxTile || n >= kMaxTile * ctx->sm_count ? kMaxTile : kMaxTile / 2;
     p.tiles = (n + p.tile - 1) / p.tile;
     p.row = (static_cast<size_t>(n) + 63) / 64 * 64;
     p.counts = ((static_cast<size_t>(1) << p.digit_bits) * p.tiles + 63) / 64 * 64;
@@ -529,10 +592,10 @@ GradientPlan plan_gradient(const BulletOuCudaCppContext* ctx, int n, int vocab, 
     const int parts = (units + p.lanes * most - 1) / (p.lanes * most);
     p.units = (units + p.lanes * parts - 1) / (p.lanes * parts);
     // Chunks long enough that the two partial rows of each cost little, short
-    // enough that every SM has its 64 warps.
-    const int64_t groups = static_cast<int64_t>(ctx->sm_count) * 64 * 32 / p.lanes;
+    // enough that every SM has the 24 warps that fit it.
+    const int64_t groups = static_cast<int64_t>(ctx->sm_count) * 24 * 32 / p.lanes;
     p.chunk = 128;
-    while (p.chunk > 16 && n / p.chunk < groups) p.chunk /= 2;
+    while (p.chunk > 16 && static_cast<int64_t>(n / p.chunk) * parts < groups) p.chunk /= 2;
     p.chunks = (n + p.chunk - 1) / p.chunk;
     return p;
 }
@@ -546,27 +609,38 @@ int sort_tokens(BulletOuCudaCppContext* ctx, const Tokens& tokens, const Gradien
     s.bins = 1 << plan.digit_bits;
     s.totals = base + 4 * plan.row;
     s.counts = s.totals + kMaxBins;
+    s.digit_bits = plan.digit_bits;
+    s.out = reinterpret_cast<int2*>(base);
+    s.other = s.out + plan.row;
+    LaunchShape shape{dim3(plan.tiles), kThreads};
+    const size_t places = static_cast<size_t>(kWarps) * s.bins * sizeof(int);
+    constexpr int kSteps = kMaxTile / kThreads;
+    if (plan.tile == kMaxTile && plan.tiles == 1) {
+        shape.smem = places;
+        if (launch_kernel(ctx, "embedding sort launch", sort_scatter_kernel<kSteps, true>, shape, s, plan.passes) != 0) return -1;
+        out->entries = plan.passes % 2 == 1 ? s.out : s.other;
+        return 0;
+    }
+    const bool large = plan.tile == kMaxTile;
     for (int pass = 0; pass < plan.passes; ++pass) {
         s.shift = pass * plan.digit_bits;
-        s.keys_out = base + (pass & 1) * 2 * plan.row;
-        s.positions_out = s.keys_out + plan.row;
-        const bool large = plan.tile == kMaxTile;
-        LaunchShape shape{dim3(plan.tiles), kThreads};
         shape.chained = pass > 0;
-        if (launch_kernel(ctx, "embedding sort launch", large ? sort_count_kernel<kMaxTile / kThreads> : sort_count_kernel<kMaxTile / kThreads / 2>, shape, s) != 0)
+        shape.smem = 0;
+        shape.grid = dim3(plan.tiles);
+        if (launch_kernel(ctx, "embedding sort launch", large ? sort_count_kernel<kSteps> : sort_count_kernel<kSteps / 2>, shape, s) != 0)
             return -1;
         shape.chained = true;
         shape.grid = dim3(s.bins);
         if (launch_kernel(ctx, "embedding sort launch", sort_scan_kernel, shape, s) != 0) return -1;
         shape.grid = dim3(plan.tiles);
-        shape.smem = static_cast<size_t>(kWarps) * s.bins * sizeof(int);
-        if (launch_kernel(ctx, "embedding sort launch", large ? sort_scatter_kernel<kMaxTile / kThreads> : sort_scatter_kernel<kMaxTile / kThreads / 2>, shape, s) != 0)
+        shape.smem = places;
+        if (launch_kernel(ctx, "embedding sort launch",
+                          large ? sort_scatter_kernel<kSteps, false> : sort_scatter_kernel<kSteps / 2, false>, shape, s, 1) != 0)
             return -1;
-        s.keys_in = s.keys_out;
-        s.positions_in = s.positions_out;
+        s.in = s.out;
+        std::swap(s.out, s.other);
     }
-    out->keys = s.keys_in;
-    out->positions = s.positions_in;
+    out->entries = s.in;
     return 0;
 }
 
@@ -581,7 +655,7 @@ int launch_gradient(BulletOuCudaCppContext* ctx, const GradientArgs& a) {
     if (a.chunks <= 1) return 0;
     LaunchShape join{dim3((a.chunks + kWarps - 1) / kWarps), kThreads};
     join.chained = true;
-    return launch_kernel(ctx, "embedding gradient join launch", joined_rows_kernel<Out>, join, a);
+    return launch_kernel(ctx, "embedding gradient join launch", joined_rows_kernel<Out, kUnit % 4 == 0>, join, a);
 }
 
 template <typename In, typename Out, int kUnit>
@@ -609,6 +683,7 @@ int gradient(BulletOuCudaCppContext* ctx, const Tokens& t, GradientArgs a, bool 
         int* const base = static_cast<int*>(scratch);
         a.heads = reinterpret_cast<float*>(base + 4 * p.row + kMaxBins + p.counts);
         a.tails = a.heads + static_cast<size_t>(p.chunks) * p.width;
+        a.part_stride = p.width;
         if (sort_tokens(ctx, t, p, base, &a) != 0) return -1;
     }
     a.chunk = p.chunk;
@@ -617,24 +692,34 @@ int gradient(BulletOuCudaCppContext* ctx, const Tokens& t, GradientArgs a, bool 
     return vector ? launch_gradient_unit<In, Out, kVectorUnit<In, Out>>(ctx, a, p) : launch_gradient_unit<In, Out, 1>(ctx, a, p);
 }
 
-// Whether rows of `width` can be taken in vector units.
-template <typename A, typename B>
-bool vector_rows(const BulletOuB200Matrix& a, const BulletOuB200Matrix& b) {
-    constexpr int kUnit = kVectorUnit<A, B>;
+// Whether the rows of both can be taken in units of kUnit elements.
+template <typename A, typename B, int kUnit>
+bool rows_of_units(const BulletOuB200Matrix& a, const BulletOuB200Matrix& b) {
     return a.cols % kUnit == 0 && rows_aligned(a, std::min<size_t>(16, kUnit * sizeof(A))) &&
            rows_aligned(b, std::min<size_t>(16, kUnit * sizeof(B)));
 }
 
-template <typename In, typename Out>
-int lookup(BulletOuCudaCppContext* ctx, const LookupArgs& a, const BulletOuB200Matrix& table, const BulletOuB200Matrix& out) {
-    const bool vector = vector_rows<In, Out>(table, out);
-    const int units = a.width / (vector ? kVectorUnit<In, Out> : 1);
+template <typename In, typename Out, int kUnit>
+int launch_lookup(BulletOuCudaCppContext* ctx, const LookupArgs& a) {
+    const int units = a.width / kUnit;
     int group = 1;
     while (group < 32 && group < units) group *= 2;
-    const int64_t blocks = (static_cast<int64_t>(a.tokens.n) * group + kThreads - 1) / kThreads;
-    const LaunchShape shape{dim3(static_cast<unsigned>(std::min<int64_t>(blocks, ctx->sm_count * kLookupCtas))), kThreads};
-    if (vector) return launch_kernel(ctx, "embedding lookup launch", lookup_kernel<In, Out, kVectorUnit<In, Out>>, shape, a, group);
-    return launch_kernel(ctx, "embedding lookup launch", lookup_kernel<In, Out, 1>, shape, a, group);
+    // as many rows for a group as leave every resident group its share; where
+    // the rows are few, their columns are shared too
+    const int64_t resident = static_cast<int64_t>(ctx->sm_count) * kLookupCtas;
+    int span = 1;
+    while (span < group && resident * (kThreads / group) * span < a.tokens.n) span *= 2;
+    const int64_t blocks = ((static_cast<int64_t>(a.tokens.n) + span - 1) / span * group + kThreads - 1) / kThreads;
+    const unsigned x = static_cast<unsigned>(std::min(blocks, resident));
+    const unsigned y = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(units / 64, resident / x)));
+    return launch_kernel(ctx, "embedding lookup launch", lookup_kernel<In, Out, kUnit>, LaunchShape{dim3(x, y), kThreads}, a, group, span);
+}
+
+template <typename In, typename Out>
+int lookup(BulletOuCudaCppContext* ctx, const LookupArgs& a, const BulletOuB200Matrix& table, const BulletOuB200Matrix& out) {
+    if (rows_of_units<In, Out, kVectorUnit<In, Out>>(table, out)) return launch_lookup<In, Out, kVectorUnit<In, Out>>(ctx, a);
+    if (rows_of_units<In, Out, 2>(table, out)) return launch_lookup<In, Out, 2>(ctx, a);
+    return launch_lookup<In, Out, 1>(ctx, a);
 }
 
 }  // namespace
@@ -694,8 +779,8 @@ int bulletou_b200_embedding_backward_device(BulletOuCudaCppContext* ctx, const B
     const bool out16 = table_gradients->type == BULLETOU_B200_TYPE_BF16;
     using B = __nv_bfloat16;
     const BulletOuB200Matrix &g = *out_gradients, &o = *table_gradients;
-    const int rc = in16 ? (out16 ? gradient<B, B>(ctx, t, a, vector_rows<B, B>(g, o)) : gradient<B, float>(ctx, t, a, vector_rows<B, float>(g, o)))
-                        : (out16 ? gradient<float, B>(ctx, t, a, vector_rows<float, B>(g, o)) : gradient<float, float>(ctx, t, a, vector_rows<float, float>(g, o)));
+    const int rc = in16 ? (out16 ? gradient<B, B>(ctx, t, a, rows_of_units<B, B, kVectorUnit<B, B>>(g, o)) : gradient<B, float>(ctx, t, a, rows_of_units<B, float, kVectorUnit<B, float>>(g, o)))
+                        : (out16 ? gradient<float, B>(ctx, t, a, rows_of_units<float, B, kVectorUnit<float, B>>(g, o)) : gradient<float, float>(ctx, t, a, rows_of_units<float, float, kVectorUnit<float, float>>(g, o)));
     return rc != 0 ? rc : ok();
 }
 

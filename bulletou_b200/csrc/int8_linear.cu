@@ -22,6 +22,51 @@ __device__ __forceinline__ float row_factor(float top) { return 127.0f * __frcp_
 __device__ __forceinline__ float row_scale(float top) { return top * (1.0f / 127.0f); }
 __device__ __forceinline__ int quantised(float x, float factor) { return __float2int_rn(x * factor); }
 
+// ------------------------------------------------------------------ repacking
+// Rows of bytes into rows that start on 16 bytes, for the TMA.
+struct RepackArgs {
+    const int8_t* src;
+    size_t src_stride;
+    int8_t* dst;
+    size_t dst_stride;
+    int rows, cols;
+};
+
+constexpr int kRepackWords = 8;  // 4-byte words that a thread has in flight
+
+__device__ void repack_rows(const RepackArgs& a, unsigned block, unsigned blocks) {
+    const unsigned words = (a.cols + 3) / 4, parts = (words + kThreads - 1) / kThreads;
+    // a CTA takes kRepackWords neighbouring pieces of kThreads words
+    const int64_t pieces = static_cast<int64_t>(a.rows) * parts;
+    for (int64_t p0 = static_cast<int64_t>(block) * kRepackWords; p0 < pieces; p0 += static_cast<int64_t>(blocks) * kRepackWords) {
+        uint32_t word[kRepackWords];
+        int64_t row = p0 / parts;
+        unsigned part = static_cast<unsigned>(p0 - row * parts);
+        const int64_t row0 = row;
+        const unsigned part0 = part;
+#pragma unroll
+        for (int i = 0; i < kRepackWords; ++i) {
+            const int c = static_cast<int>(part * kThreads + threadIdx.x) * 4;
+            const int8_t* s = a.src + row * a.src_stride + c;
+            word[i] = 0;
+            if (row < a.rows)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (c + j < a.cols) word[i] |= static_cast<uint32_t>(static_cast<uint8_t>(s[j])) << (8 * j);
+            if (++part == parts) part = 0, ++row;
+        }
+        row = row0, part = part0;
+#pragma unroll
+        for (int i = 0; i < kRepackWords; ++i) {
+            const int c = static_cast<int>(part * kThreads + threadIdx.x) * 4;
+            if (row < a.rows && c < a.cols) *reinterpret_cast<uint32_t*>(a.dst + row * a.dst_stride + c) = word[i];
+            if (++part == parts) part = 0, ++row;
+        }
+    }
+}
+
+__global__ void __launch_bounds__(kThreads) repack_kernel(const RepackArgs a) { repack_rows(a, blockIdx.x, gridDim.x); }
+
 // ------------------------------------------------------------------ quantisation
 struct QuantizeArgs {
     const void* x;
@@ -33,6 +78,8 @@ struct QuantizeArgs {
     int padded_cols;  // columns [cols, padded_cols) of q are zeroed
     bool x_vector;    // 16-byte aligned rows of x
     bool q_vector;    // 16-byte aligned rows of q, padded_cols a multiple of 16
+    unsigned ctas;    // the CTAs after these repack the weights
+    RepackArgs weights;
 };
 
 constexpr int kGroup = 16;  // columns that a thread takes together: a 16-byte store of q
@@ -88,6 +135,10 @@ __global__ void __launch_bounds__(kThreads, 4) quantize_kernel(const QuantizeArg
     constexpr int kHeld = 2, kRowWarps = kRowThreads / 32;
     __shared__ float warp_top[kWarps];
     let_next_start();
+    if (blockIdx.x >= a.ctas) {
+        repack_rows(a.weights, blockIdx.x - a.ctas, gridDim.x - a.ctas);
+        return;
+    }
     const int in_row = threadIdx.x % kRowThreads;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / kRowThreads) + threadIdx.x / kRowThreads;
     const bool live = row < a.rows;
@@ -130,24 +181,6 @@ __global__ void __launch_bounds__(kThreads, 4) quantize_kernel(const QuantizeArg
         g.store(a, q, c, factor, some);
     }
     if (in_row == 0) a.scales[row] = top == INFINITY ? NAN : some ? row_scale(top) : 0.0f;
-}
-
-// Rows of bytes into rows that start on 16 bytes, for the TMA.
-__global__ void __launch_bounds__(kThreads) repack_kernel(const int8_t* src, size_t src_stride, int8_t* dst,
-                                                          size_t dst_stride, int rows, int cols) {
-    const int words = (cols + 3) / 4;
-    const size_t n = static_cast<size_t>(rows) * words;
-    for (size_t i = static_cast<size_t>(blockIdx.x) * kThreads + threadIdx.x; i < n;
-         i += static_cast<size_t>(gridDim.x) * kThreads) {
-        const size_t r = i / words;
-        const int c = static_cast<int>(i - r * words) * 4;
-        const int8_t* s = src + r * src_stride + c;
-        uint32_t w = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (c + j < cols) w |= static_cast<uint32_t>(static_cast<uint8_t>(s[j])) << (8 * j);
-        *reinterpret_cast<uint32_t*>(dst + r * dst_stride + c) = w;
-    }
 }
 
 // ------------------------------------------------------------------ few rows
@@ -274,21 +307,32 @@ __global__ void __launch_bounds__(kThreads) few_rows_kernel(const FewRowsArgs a)
 // ------------------------------------------------------------------ host
 size_t padded(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
-template <typename T>
-void launch_quantize(BulletOuCudaCppContext* ctx, const QuantizeArgs& a) {
-    const int cols = std::max(a.cols, a.padded_cols);
-    auto grid = [&](int row_threads) {
-        const int per = kThreads / row_threads;
-        return static_cast<unsigned>((static_cast<int64_t>(a.rows) + per - 1) / per);
-    };
-    if (cols <= 32 * 32) quantize_kernel<T, 32><<<grid(32), kThreads, 0, ctx->stream>>>(a);
-    else if (cols <= 64 * 32) quantize_kernel<T, 64><<<grid(64), kThreads, 0, ctx->stream>>>(a);
-    else if (cols <= 128 * 32) quantize_kernel<T, 128><<<grid(128), kThreads, 0, ctx->stream>>>(a);
-    else quantize_kernel<T, 256><<<grid(256), kThreads, 0, ctx->stream>>>(a);
+unsigned repack_ctas(const BulletOuCudaCppContext* ctx, const RepackArgs& a) {
+    const int64_t words = (static_cast<int64_t>(a.cols) + 3) / 4;
+    const int64_t pieces = a.rows * ((words + kThreads - 1) / kThreads);
+    return static_cast<unsigned>(std::min<int64_t>((pieces + kRepackWords - 1) / kRepackWords, ctx->sm_count * 4));
 }
 
+template <typename T, int kRowThreads>
+int launch_quantize(BulletOuCudaCppContext* ctx, QuantizeArgs a) {
+    constexpr int kRows = kThreads / kRowThreads;
+    a.ctas = static_cast<unsigned>((static_cast<int64_t>(a.rows) + kRows - 1) / kRows);
+    const unsigned more = a.weights.rows > 0 ? repack_ctas(ctx, a.weights) : 0;
+    return launch_kernel(ctx, "int8 quantise launch", quantize_kernel<T, kRowThreads>, LaunchShape{dim3(a.ctas + more), kThreads}, a);
+}
+
+template <typename T>
+int launch_quantize(BulletOuCudaCppContext* ctx, const QuantizeArgs& a) {
+    const int cols = std::max(a.cols, a.padded_cols);
+    if (cols <= 32 * 32) return launch_quantize<T, 32>(ctx, a);
+    if (cols <= 64 * 32) return launch_quantize<T, 64>(ctx, a);
+    if (cols <= 128 * 32) return launch_quantize<T, 128>(ctx, a);
+    return launch_quantize<T, 256>(ctx, a);
+}
+
+// `weights`: rows to repack in the same launch (none: rows == 0).
 int quantize(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix& x, int8_t* q, size_t q_stride, int padded_cols,
-             float* scales) {
+             float* scales, const RepackArgs& weights) {
     QuantizeArgs a{};
     a.x = x.data;
     a.x_stride = x.row_stride;
@@ -300,9 +344,8 @@ int quantize(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix& x, int8_t* q
     a.padded_cols = padded_cols;
     a.x_vector = rows_aligned(x, 16);
     a.q_vector = padded_cols % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 && (x.rows <= 1 || q_stride % 16 == 0);
-    if (x.type == BULLETOU_B200_TYPE_F32) launch_quantize<float>(ctx, a);
-    else launch_quantize<__nv_bfloat16>(ctx, a);
-    return check_launch("int8 quantise launch");
+    a.weights = weights;
+    return x.type == BULLETOU_B200_TYPE_F32 ? launch_quantize<float>(ctx, a) : launch_quantize<__nv_bfloat16>(ctx, a);
 }
 
 // Whether TMA can read these rows as they are.
@@ -310,11 +353,8 @@ bool tma_rows(const void* data, size_t rows, size_t stride) {
     return reinterpret_cast<uintptr_t>(data) % 16 == 0 && (rows <= 1 || stride % 16 == 0);
 }
 
-int repack(BulletOuCudaCppContext* ctx, const int8_t* src, size_t stride, int8_t* dst, size_t dst_stride, int rows, int cols) {
-    const size_t words = static_cast<size_t>(rows) * ((cols + 3) / 4);
-    const int grid = static_cast<int>(std::min<size_t>((words + kThreads - 1) / kThreads, static_cast<size_t>(ctx->sm_count) * 8));
-    repack_kernel<<<grid, kThreads, 0, ctx->stream>>>(src, stride, dst, dst_stride, rows, cols);
-    return check_launch("int8 repack launch");
+int repack(BulletOuCudaCppContext* ctx, const RepackArgs& a) {
+    return launch_kernel(ctx, "int8 repack launch", repack_kernel, LaunchShape{dim3(repack_ctas(ctx, a)), kThreads}, a);
 }
 
 template <typename T, typename Out>
@@ -359,16 +399,18 @@ int product(BulletOuCudaCppContext* ctx, ProductArgs p, const BulletOuB200Matrix
     float* const scales = static_cast<float*>(scratch);
     int8_t* const q = static_cast<int8_t*>(scratch) + scale_bytes;
     int8_t* const w = q + q_bytes;
+    RepackArgs weights{};
     if (own_w) {
-        if (p.k > 0 && repack(ctx, p.w, p.w_stride, w, pitch, p.n, p.k) != 0) return -1;
+        if (p.k > 0) weights = {p.w, p.w_stride, w, pitch, p.n, p.k};
         p.w = w;
         p.w_stride = pitch;
     }
     if (x != nullptr) {
-        if (quantize(ctx, *x, q, pitch, static_cast<int>(pitch), scales) != 0) return -1;
+        if (quantize(ctx, *x, q, pitch, static_cast<int>(pitch), scales, weights) != 0) return -1;
         p.scales = scales;
-    } else if (own_q && p.k > 0 && repack(ctx, p.q, p.q_stride, q, pitch, p.m, p.k) != 0) {
-        return -1;
+    } else {
+        if (weights.rows > 0 && repack(ctx, weights) != 0) return -1;
+        if (own_q && p.k > 0 && repack(ctx, {p.q, p.q_stride, q, pitch, p.m, p.k}) != 0) return -1;
     }
     if (own_q) {
         p.q = q;
@@ -377,7 +419,7 @@ int product(BulletOuCudaCppContext* ctx, ProductArgs p, const BulletOuB200Matrix
     // a single row's stride is the caller's and may be anything
     if (p.m == 1) p.q_stride = pitch;
     if (p.n == 1) p.w_stride = pitch;
-    return launch_int8_mma(ctx, p, out_type, x != nullptr);
+    return launch_int8_mma(ctx, p, out_type, x != nullptr, weights.rows == 0);
 }
 
 // The weight side's checks, shared by the two products.
@@ -431,7 +473,7 @@ int bulletou_b200_int8_quantize_rows_device(BulletOuCudaCppContext* ctx, const B
         return -1;
     if (x->rows == 0) return ok();
     return quantize(ctx, *x, static_cast<int8_t*>(q->data), q->row_stride, static_cast<int>(x->cols),
-                    static_cast<float*>(scales->data)) != 0
+                    static_cast<float*>(scales->data), RepackArgs{}) != 0
                ? -1
                : ok();
 }

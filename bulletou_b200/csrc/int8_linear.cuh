@@ -27,7 +27,8 @@ __device__ __forceinline__ float int8_result(int sum, float row_scale, float col
 
 // The product on the tensor cores; q and w as a TMA can read them (16-byte
 // aligned base and row stride).  `after_quantise`: the launch directly before
-// this one on the stream is quantize_kernel, which lets it start early.
-int launch_int8_mma(BulletOuCudaCppContext* ctx, const ProductArgs& a, int out_type, bool after_quantise);
+// this one on the stream is quantize_kernel, which lets it start early;
+// `weights_ready`: that launch does not write the weights.
+int launch_int8_mma(BulletOuCudaCppContext* ctx, const ProductArgs& a, int out_type, bool after_quantise, bool weights_ready);
 
 }  // namespace bou

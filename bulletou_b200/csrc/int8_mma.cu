@@ -150,7 +150,7 @@ struct TileShape {
 template <int TN, typename Out>
 __global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ CUtensorMap map_q,
                                                         const __grid_constant__ CUtensorMap map_w, const ProductArgs a,
-                                                        int splits, bool vector_ok) {
+                                                        int splits, bool vector_ok, bool weights_ready) {
     using S = TileShape<TN>;
     extern __shared__ uint8_t raw[];
     const uint32_t raw_addr = smem_u32(raw);
@@ -199,6 +199,7 @@ __global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ 
     if (warp == 0 && lane == 0) {
         // the weights of the first stages come while the rows are still being quantised
         const int ahead = min(count, S::kStages);
+        if (!weights_ready) wait_for_previous();
         for (int i = 0; i < ahead; ++i) {
             mbar_expect_tx(full + 8 * i, S::kStageBytes);
             tma_load_2d(base + i * S::kStageBytes + kABytes, &map_w, (k0 + i) * kTileK, col0, full + 8 * i);
@@ -458,7 +459,7 @@ int operand_map(CUtensorMap* map, const int8_t* data, int rows, int k, size_t st
 }
 
 template <int TN, typename Out>
-int launch_tiles(BulletOuCudaCppContext* ctx, const ProductArgs& a, bool vector_ok, bool early) {
+int launch_tiles(BulletOuCudaCppContext* ctx, const ProductArgs& a, bool vector_ok, bool early, bool weights_ready) {
     const int64_t tiles = static_cast<int64_t>((a.m + kTileM - 1) / kTileM) * ((a.n + TN - 1) / TN);
     const int blocks = (a.k + kTileK - 1) / kTileK;
     int splits = 1;
@@ -468,7 +469,7 @@ int launch_tiles(BulletOuCudaCppContext* ctx, const ProductArgs& a, bool vector_
     if (operand_map(&q, a.q, a.m, a.k, a.q_stride, kTileM) != 0 || operand_map(&w, a.w, a.n, a.k, a.w_stride, TN) != 0)
         return -1;
     const LaunchShape shape{dim3(static_cast<unsigned>(tiles * splits)), TileShape<TN>::kThreads, TileShape<TN>::kSmem, splits, early};
-    return launch_kernel(ctx, "int8 product launch", int8_tile_kernel<TN, Out>, shape, q, w, a, splits, vector_ok);
+    return launch_kernel(ctx, "int8 product launch", int8_tile_kernel<TN, Out>, shape, q, w, a, splits, vector_ok, weights_ready);
 }
 
 template <typename Out>
@@ -481,21 +482,21 @@ int launch_pairs(BulletOuCudaCppContext* ctx, const ProductArgs& a, int tiles, b
 }
 
 template <typename Out>
-int launch_typed(BulletOuCudaCppContext* ctx, const ProductArgs& a, bool early) {
+int launch_typed(BulletOuCudaCppContext* ctx, const ProductArgs& a, bool early, bool weights_ready) {
     const bool vector_ok = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && (a.m <= 1 || a.out_stride * sizeof(Out) % 16 == 0);
     const int64_t pairs = static_cast<int64_t>((a.m + 255) / 256) * ((a.n + 255) / 256);
     if (pairs >= ctx->sm_count / 2 && pairs <= INT32_MAX)
         return launch_pairs<Out>(ctx, a, static_cast<int>(pairs), vector_ok, early);
     const int64_t wide = static_cast<int64_t>((a.m + 127) / 128) * ((a.n + 127) / 128);
-    return wide >= ctx->sm_count ? launch_tiles<128, Out>(ctx, a, vector_ok, early)
-                                 : launch_tiles<64, Out>(ctx, a, vector_ok, early);
+    return wide >= ctx->sm_count ? launch_tiles<128, Out>(ctx, a, vector_ok, early, weights_ready)
+                                 : launch_tiles<64, Out>(ctx, a, vector_ok, early, weights_ready);
 }
 
 }  // namespace
 
-int launch_int8_mma(BulletOuCudaCppContext* ctx, const ProductArgs& a, int out_type, bool after_quantise) {
-    return out_type == BULLETOU_B200_TYPE_F32 ? launch_typed<float>(ctx, a, after_quantise)
-                                              : launch_typed<__nv_bfloat16>(ctx, a, after_quantise);
+int launch_int8_mma(BulletOuCudaCppContext* ctx, const ProductArgs& a, int out_type, bool after_quantise, bool weights_ready) {
+    return out_type == BULLETOU_B200_TYPE_F32 ? launch_typed<float>(ctx, a, after_quantise, weights_ready)
+                                              : launch_typed<__nv_bfloat16>(ctx, a, after_quantise, weights_ready);
 }
 
 }  // namespace bou

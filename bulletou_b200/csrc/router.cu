@@ -21,7 +21,10 @@
 namespace bou {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
+// CTAs on an SM by the places of a lane: 64 registers for each thread, 80 for 16 places
+template <int kPlaces>
+constexpr int kCtas = kPlaces > 12 ? 3 : 4;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxExperts = BULLETOU_B200_ROUTER_MAX_EXPERTS;
 constexpr int kMaxTopK = BULLETOU_B200_ROUTER_MAX_TOP_K;
@@ -51,7 +54,7 @@ struct RouterArgs {
     size_t logit_grad_stride;
 };
 
-// 2^x to about two units in the last place, and a maximum that keeps NaN.
+// 2^x and 1 / x to about two units in the last place, and a maximum that keeps NaN.
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -60,6 +63,11 @@ __device__ __forceinline__ float exp2_approx(float x) {
 __device__ __forceinline__ float max_nan(float a, float b) {
     float y;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ float reciprocal_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 constexpr float kLog2E = 1.4426950408889634f;
@@ -119,7 +127,7 @@ struct Row {
         }
         sum = group_sum<kGroup>(sum);
         // a masked row's exponentials are zeros; a broken row is NaN
-        inverse = alive ? 1.0f / sum : top == -INFINITY ? 0.0f : NAN;
+        inverse = alive ? reciprocal_approx(sum) : top == -INFINITY ? 0.0f : NAN;
     }
 };
 
@@ -156,7 +164,7 @@ __device__ void finish(const RouterArgs& a, const float* p_sums, const int* coun
 // kGroup lanes for each row (at least top_k), kPlaces experts in each lane.  One
 // CTA alone also finishes; otherwise the CTAs leave their sums to router_join_kernel.
 template <typename T, int kGroup, int kPlaces>
-__global__ void __launch_bounds__(kThreads) router_forward_kernel(const RouterArgs a) {
+__global__ void __launch_bounds__(kThreads, kCtas<kPlaces>) router_forward_kernel(const RouterArgs a) {
     __shared__ int count[kMaxExperts + 1];
     __shared__ float psum[kWarps][kGroup * kPlaces];
     const int lane = threadIdx.x & (kGroup - 1), warp = threadIdx.x >> 5;
@@ -200,7 +208,7 @@ __global__ void __launch_bounds__(kThreads) router_forward_kernel(const RouterAr
         }
         if (lane < a.top_k && t < a.rows) {
             a.chosen[t * a.chosen_stride + lane] = pick;
-            a.gates[t * a.gate_stride + lane] = a.normalize && pick >= 0 ? own / total : own;
+            a.gates[t * a.gate_stride + lane] = a.normalize && pick >= 0 ? own * reciprocal_approx(total) : own;
             if (pick >= 0) atomicAdd(count + pick, 1);
         }
     }
@@ -279,7 +287,7 @@ __global__ void __launch_bounds__(kJoinThreads) router_join_kernel(const RouterA
 }
 
 template <typename T, int kGroup, int kPlaces>
-__global__ void __launch_bounds__(kThreads) router_backward_kernel(const RouterArgs a) {
+__global__ void __launch_bounds__(kThreads, kCtas<kPlaces>) router_backward_kernel(const RouterArgs a) {
     __shared__ int choices;
     const int lane = threadIdx.x & (kGroup - 1);
     if (threadIdx.x == 0) choices = 0;
@@ -329,7 +337,7 @@ __global__ void __launch_bounds__(kThreads) router_backward_kernel(const RouterA
             if (a.normalize) {
                 // p (u - sum g u) / sum p: gates that sum to one take no part in the mean
                 const float total = group_sum<kGroup>(p);
-                const float scale = total > 0.0f ? 1.0f / total : 0.0f;
+                const float scale = total > 0.0f ? reciprocal_approx(total) : 0.0f;
                 direct = (up - weighted * scale) * scale;
                 dot = group_sum<kGroup>(dot);
             } else {
@@ -372,16 +380,16 @@ int with_shape(const RouterArgs& a, F&& f) {
 
 // CTAs for the rows; up to four rounds of rows are left to one CTA, which then
 // needs no second launch.
-int router_grid(const BulletOuCudaCppContext* ctx, int rows, int group) {
+int router_grid(const BulletOuCudaCppContext* ctx, int rows, int group, int resident) {
     const int per = kThreads / group;
     const int64_t ctas = (static_cast<int64_t>(rows) + per - 1) / per;
-    return ctas <= 4 ? 1 : static_cast<int>(std::min<int64_t>(ctas, static_cast<int64_t>(ctx->sm_count) * 2));
+    return ctas <= 4 ? 1 : static_cast<int>(std::min<int64_t>(ctas, static_cast<int64_t>(ctx->sm_count) * resident));
 }
 
 template <typename T>
 int forward(BulletOuCudaCppContext* ctx, RouterArgs a) {
     return with_shape(a, [&](auto group, auto places) {
-        const int grid = router_grid(ctx, a.rows, group);
+        const int grid = router_grid(ctx, a.rows, group, kCtas<places()>);
         if (grid > 1) {
             void* p = nullptr;
             if (scratch_slot(ctx, kScratchRouter, static_cast<size_t>(grid) * (2 * a.experts + 1) * 4, &p,
@@ -403,7 +411,7 @@ template <typename T>
 int backward(BulletOuCudaCppContext* ctx, const RouterArgs& a) {
     return with_shape(a, [&](auto group, auto places) {
         const int64_t ctas = (static_cast<int64_t>(a.rows) * group + kThreads - 1) / kThreads;
-        const LaunchShape shape{dim3(static_cast<unsigned>(std::min<int64_t>(ctas, static_cast<int64_t>(ctx->sm_count) * 8))), kThreads};
+        const LaunchShape shape{dim3(static_cast<unsigned>(std::min<int64_t>(ctas, static_cast<int64_t>(ctx->sm_count) * kCtas<places()>))), kThreads};
         return launch_kernel(ctx, "router backward launch", router_backward_kernel<T, group(), places()>, shape, a);
     });
 }
