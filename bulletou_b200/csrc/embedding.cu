@@ -221,15 +221,14 @@ __global__ void __launch_bounds__(kThreads) sort_scan_kernel(const SortPass s) {
 // start of its bin, its tile's start in the bin, the entries of earlier warps,
 // and its rank among the equal digits of its warp.  kAlone: one tile holds all
 // entries, so its own counts are all there is and the CTA runs every pass.
-template <int kSteps, bool kAlone>
-__global__ void __launch_bounds__(kThreads) sort_scatter_kernel(SortPass s, int passes) {
-    constexpr int kBinsOfThread = kMaxBins / kThreads;
+template <int kSteps, bool kAlone, int kBinsOfThread>
+__global__ void __launch_bounds__(kThreads, kBinsOfThread <= 2 ? 5 : 2) sort_scatter_kernel(SortPass s, int passes) {
     extern __shared__ int places[];  // [kWarps][bins]
     __shared__ int warp_sums[kWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int* const place = places + warp * s.bins;
     let_next_start();
-    const int per = (s.bins + kThreads - 1) / kThreads, bin0 = threadIdx.x * per;
+    const int bin0 = threadIdx.x * kBinsOfThread;
     for (int pass = 0; pass < passes; ++pass) {
         for (int i = threadIdx.x; i < kWarps * s.bins; i += kThreads) places[i] = 0;
         __syncthreads();
@@ -243,7 +242,7 @@ __global__ void __launch_bounds__(kThreads) sort_scatter_kernel(SortPass s, int 
         if (!kAlone) {
 #pragma unroll
             for (int i = 0; i < kBinsOfThread; ++i) {
-                const bool in = i < per && bin0 + i < s.bins;
+                const bool in = bin0 + i < s.bins;
                 total[i] = in ? s.totals[bin0 + i] : 0;
                 start[i] = in ? s.counts[static_cast<size_t>(bin0 + i) * s.tiles + blockIdx.x] : 0;
             }
@@ -255,7 +254,9 @@ __global__ void __launch_bounds__(kThreads) sort_scatter_kernel(SortPass s, int 
             const int d = live ? s.digit(entry[j].x) : 0;
             unsigned peers = __ballot_sync(0xffffffffu, live);
             peers = live ? peers : ~peers;
-            for (int bit = 1; bit < s.bins; bit <<= 1) {
+#pragma unroll
+            for (int bit = 1; bit < kThreads * kBinsOfThread; bit <<= 1) {
+                if (bit >= s.bins) break;
                 const unsigned set = __ballot_sync(0xffffffffu, d & bit);
                 peers &= d & bit ? set : ~set;
             }
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(kThreads) sort_scatter_kernel(SortPass s, int 
         for (int i = 0; i < kBinsOfThread; ++i) {
             if (kAlone) {
                 start[i] = total[i] = 0;
-                if (i < per && bin0 + i < s.bins)
+                if (bin0 + i < s.bins)
                     for (int w = 0; w < kWarps; ++w) total[i] += places[w * s.bins + bin0 + i];
             }
             sum += total[i];
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(kThreads) sort_scatter_kernel(SortPass s, int 
         int at = block_exclusive(sum, warp_sums, &all);
 #pragma unroll
         for (int i = 0; i < kBinsOfThread; ++i) {
-            if (i < per && bin0 + i < s.bins) {
+            if (bin0 + i < s.bins) {
                 int next = at + start[i];
                 for (int w = 0; w < kWarps; ++w) {
                     const int c = places[w * s.bins + bin0 + i];
@@ -600,6 +601,15 @@ GradientPlan plan_gradient(const BulletOuCudaCppContext* ctx, int n, int vocab, 
     return p;
 }
 
+template <int kSteps, bool kAlone>
+int launch_scatter(BulletOuCudaCppContext* ctx, const LaunchShape& shape, const SortPass& s, int passes) {
+    auto with = [&](auto kernel) { return launch_kernel(ctx, "embedding sort launch", kernel, shape, s, passes); };
+    if (s.bins <= kThreads) return with(sort_scatter_kernel<kSteps, kAlone, 1>);
+    if (s.bins <= 2 * kThreads) return with(sort_scatter_kernel<kSteps, kAlone, 2>);
+    if (s.bins <= 4 * kThreads) return with(sort_scatter_kernel<kSteps, kAlone, 4>);
+    return with(sort_scatter_kernel<kSteps, kAlone, 8>);
+}
+
 // Sorts the tokens into the scratch at `base`.
 int sort_tokens(BulletOuCudaCppContext* ctx, const Tokens& tokens, const GradientPlan& plan, int* base, GradientArgs* out) {
     SortPass s{};
@@ -617,7 +627,7 @@ int sort_tokens(BulletOuCudaCppContext* ctx, const Tokens& tokens, const Gradien
     constexpr int kSteps = kMaxTile / kThreads;
     if (plan.tile == kMaxTile && plan.tiles == 1) {
         shape.smem = places;
-        if (launch_kernel(ctx, "embedding sort launch", sort_scatter_kernel<kSteps, true>, shape, s, plan.passes) != 0) return -1;
+        if (launch_scatter<kSteps, true>(ctx, shape, s, plan.passes) != 0) return -1;
         out->entries = plan.passes % 2 == 1 ? s.out : s.other;
         return 0;
     }
@@ -634,8 +644,7 @@ int sort_tokens(BulletOuCudaCppContext* ctx, const Tokens& tokens, const Gradien
         if (launch_kernel(ctx, "embedding sort launch", sort_scan_kernel, shape, s) != 0) return -1;
         shape.grid = dim3(plan.tiles);
         shape.smem = places;
-        if (launch_kernel(ctx, "embedding sort launch",
-                          large ? sort_scatter_kernel<kSteps, false> : sort_scatter_kernel<kSteps / 2, false>, shape, s, 1) != 0)
+        if ((large ? launch_scatter<kSteps, false>(ctx, shape, s, 1) : launch_scatter<kSteps / 2, false>(ctx, shape, s, 1)) != 0)
             return -1;
         s.in = s.out;
         std::swap(s.out, s.other);

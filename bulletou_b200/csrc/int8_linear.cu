@@ -22,46 +22,59 @@ __device__ __forceinline__ float row_factor(float top) { return 127.0f * __frcp_
 __device__ __forceinline__ float row_scale(float top) { return top * (1.0f / 127.0f); }
 __device__ __forceinline__ int quantised(float x, float factor) { return __float2int_rn(x * factor); }
 
-// ------------------------------------------------------------------ repacking
-// Rows of bytes into rows that start on 16 bytes, for the TMA.
-struct RepackArgs {
-    const int8_t* src;
-    size_t src_stride;
-    int8_t* dst;
-    size_t dst_stride;
+// ------------------------------------------------------------------ bytes
+// A matrix of bytes with rows of any alignment.
+struct Bytes {
+    const int8_t* data;
+    const int8_t* end;  // past the last row's last byte
+    size_t stride;
     int rows, cols;
+    bool vector;        // rows start on 16 bytes
 };
 
-constexpr int kRepackWords = 8;  // 4-byte words that a thread has in flight
+// 16 bytes of a row from column c on, zeros beyond its end.  An unaligned row is
+// read in the aligned words that cover it, wherever those lie inside the matrix.
+__device__ __forceinline__ uint4 load_bytes(const Bytes& m, const int8_t* row, int c) {
+    const int left = m.cols - c;
+    if (m.vector && left >= 16) return __ldg(reinterpret_cast<const uint4*>(row + c));
+    uint32_t out[4] = {};
+    if (left > 0) {
+        const int8_t* p = row + c;
+        const unsigned shift = reinterpret_cast<uintptr_t>(p) & 3u;
+        const int8_t* first = p - shift;
+        if (first >= m.data && first + 20 <= m.end) {
+            uint32_t w[5];
+#pragma unroll
+            for (int i = 0; i < 5; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(first) + i);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int keep = left - 4 * i;
+                const uint32_t v = __funnelshift_r(w[i], w[i + 1], 8 * shift);
+                out[i] = keep >= 4 ? v : keep > 0 ? v & ((1u << (8 * keep)) - 1) : 0u;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (j < left) out[j >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(p[j])) << (8 * (j & 3));
+        }
+    }
+    return make_uint4(out[0], out[1], out[2], out[3]);
+}
+
+// Rows of bytes into rows that start on 16 bytes, for the TMA; bytes up to the
+// next multiple of 16 become zeros.
+struct RepackArgs {
+    Bytes src;
+    int8_t* dst;
+    size_t dst_stride;
+};
 
 __device__ void repack_rows(const RepackArgs& a, unsigned block, unsigned blocks) {
-    const unsigned words = (a.cols + 3) / 4, parts = (words + kThreads - 1) / kThreads;
-    // a CTA takes kRepackWords neighbouring pieces of kThreads words
-    const int64_t pieces = static_cast<int64_t>(a.rows) * parts;
-    for (int64_t p0 = static_cast<int64_t>(block) * kRepackWords; p0 < pieces; p0 += static_cast<int64_t>(blocks) * kRepackWords) {
-        uint32_t word[kRepackWords];
-        int64_t row = p0 / parts;
-        unsigned part = static_cast<unsigned>(p0 - row * parts);
-        const int64_t row0 = row;
-        const unsigned part0 = part;
-#pragma unroll
-        for (int i = 0; i < kRepackWords; ++i) {
-            const int c = static_cast<int>(part * kThreads + threadIdx.x) * 4;
-            const int8_t* s = a.src + row * a.src_stride + c;
-            word[i] = 0;
-            if (row < a.rows)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (c + j < a.cols) word[i] |= static_cast<uint32_t>(static_cast<uint8_t>(s[j])) << (8 * j);
-            if (++part == parts) part = 0, ++row;
-        }
-        row = row0, part = part0;
-#pragma unroll
-        for (int i = 0; i < kRepackWords; ++i) {
-            const int c = static_cast<int>(part * kThreads + threadIdx.x) * 4;
-            if (row < a.rows && c < a.cols) *reinterpret_cast<uint32_t*>(a.dst + row * a.dst_stride + c) = word[i];
-            if (++part == parts) part = 0, ++row;
-        }
+    const int64_t units = (a.src.cols + 15) / 16, n = a.src.rows * units;
+    for (int64_t i = static_cast<int64_t>(block) * kThreads + threadIdx.x; i < n; i += static_cast<int64_t>(blocks) * kThreads) {
+        const int64_t r = i / units;
+        const int c = static_cast<int>(i - r * units) * 16;
+        *reinterpret_cast<uint4*>(a.dst + r * a.dst_stride + c) = load_bytes(a.src, a.src.data + r * a.src.stride, c);
     }
 }
 
@@ -184,12 +197,12 @@ __global__ void __launch_bounds__(kThreads, 4) quantize_kernel(const QuantizeArg
 }
 
 // ------------------------------------------------------------------ few rows
-// For up to kFewRows rows the weights' bytes are what counts: every warp takes
+// For one or two rows the weights' bytes are what counts: every warp takes
 // output channels one after the other, 16 bytes of a channel for each lane at
 // a time, against the rows' 8-bit values in shared memory.  Each CTA quantises
 // the rows itself (they are a few KB from L2), so the layer is one launch, and
 // the first channel's weights are on their way meanwhile.
-constexpr int kFewRows = 4;
+constexpr int kFewRows = 2;
 constexpr size_t kFewRowsBytes = 48 * 1024;  // shared memory for the rows
 
 struct FewRowsArgs {
@@ -197,19 +210,8 @@ struct FewRowsArgs {
     bool quantise;  // the rows are x; otherwise p.q and p.scales
     const void* x;
     size_t x_stride;
-    bool w_vector;  // 16-byte aligned rows of w
+    Bytes w;
 };
-
-// 16 bytes of a weight row from column c on, zeros beyond its end.
-__device__ __forceinline__ uint4 load_weights(const int8_t* w, int c, int cols, bool vector) {
-    if (vector && c + 16 <= cols) return __ldg(reinterpret_cast<const uint4*>(w + c));
-    uint4 packed = make_uint4(0, 0, 0, 0);
-    uint32_t* word = reinterpret_cast<uint32_t*>(&packed);
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-        if (c + j < cols) word[j >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(w[c + j])) << (8 * (j & 3));
-    return packed;
-}
 
 template <typename T, typename Out, int kRows>
 __global__ void __launch_bounds__(kThreads) few_rows_kernel(const FewRowsArgs a) {
@@ -226,7 +228,7 @@ __global__ void __launch_bounds__(kThreads) few_rows_kernel(const FewRowsArgs a)
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
         const int c = (i * 32 + lane) * 16;
-        ahead[i] = n < p.n && c < p.k ? load_weights(p.w + n * p.w_stride, c, p.k, a.w_vector) : make_uint4(0, 0, 0, 0);
+        ahead[i] = n < p.n ? load_bytes(a.w, p.w + n * p.w_stride, c) : make_uint4(0, 0, 0, 0);
     }
     float scale[kRows];
     if (a.quantise) {
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(kThreads) few_rows_kernel(const FewRowsArgs a)
             for (int i = 0; i < kAhead; ++i) {
                 const int c = c0 + i * 512;
                 const bool first = n < first_end && c0 == lane * 16;
-                v[i] = first ? ahead[i] : c < p.k ? load_weights(w, c, p.k, a.w_vector) : make_uint4(0, 0, 0, 0);
+                v[i] = first ? ahead[i] : load_bytes(a.w, w, c);
             }
 #pragma unroll
             for (int i = 0; i < kAhead; ++i)
@@ -308,16 +310,15 @@ __global__ void __launch_bounds__(kThreads) few_rows_kernel(const FewRowsArgs a)
 size_t padded(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
 unsigned repack_ctas(const BulletOuCudaCppContext* ctx, const RepackArgs& a) {
-    const int64_t words = (static_cast<int64_t>(a.cols) + 3) / 4;
-    const int64_t pieces = a.rows * ((words + kThreads - 1) / kThreads);
-    return static_cast<unsigned>(std::min<int64_t>((pieces + kRepackWords - 1) / kRepackWords, ctx->sm_count * 4));
+    const int64_t units = a.src.rows * ((static_cast<int64_t>(a.src.cols) + 15) / 16);
+    return static_cast<unsigned>(std::min<int64_t>((units + kThreads - 1) / kThreads, ctx->sm_count * 8));
 }
 
 template <typename T, int kRowThreads>
 int launch_quantize(BulletOuCudaCppContext* ctx, QuantizeArgs a) {
     constexpr int kRows = kThreads / kRowThreads;
     a.ctas = static_cast<unsigned>((static_cast<int64_t>(a.rows) + kRows - 1) / kRows);
-    const unsigned more = a.weights.rows > 0 ? repack_ctas(ctx, a.weights) : 0;
+    const unsigned more = a.weights.src.rows > 0 ? repack_ctas(ctx, a.weights) : 0;
     return launch_kernel(ctx, "int8 quantise launch", quantize_kernel<T, kRowThreads>, LaunchShape{dim3(a.ctas + more), kThreads}, a);
 }
 
@@ -330,7 +331,7 @@ int launch_quantize(BulletOuCudaCppContext* ctx, const QuantizeArgs& a) {
     return launch_quantize<T, 256>(ctx, a);
 }
 
-// `weights`: rows to repack in the same launch (none: rows == 0).
+// `weights`: rows to repack in the same launch (none: no rows).
 int quantize(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix& x, int8_t* q, size_t q_stride, int padded_cols,
              float* scales, const RepackArgs& weights) {
     QuantizeArgs a{};
@@ -357,12 +358,15 @@ int repack(BulletOuCudaCppContext* ctx, const RepackArgs& a) {
     return launch_kernel(ctx, "int8 repack launch", repack_kernel, LaunchShape{dim3(repack_ctas(ctx, a)), kThreads}, a);
 }
 
+Bytes bytes_of(const int8_t* data, size_t stride, int rows, int cols) {
+    return {data, data + (rows > 0 ? (rows - 1) * stride + cols : 0), stride, rows, cols, tma_rows(data, rows, stride)};
+}
+
 template <typename T, typename Out>
 void launch_few_rows(BulletOuCudaCppContext* ctx, const FewRowsArgs& a) {
     const int grid = std::min((a.p.n + kWarps - 1) / kWarps, ctx->sm_count * 4);
     const size_t row = padded(a.p.k, 16);
     if (a.p.m <= 1) few_rows_kernel<T, Out, 1><<<grid, kThreads, row, ctx->stream>>>(a);
-    else if (a.p.m <= 2) few_rows_kernel<T, Out, 2><<<grid, kThreads, 2 * row, ctx->stream>>>(a);
     else few_rows_kernel<T, Out, kFewRows><<<grid, kThreads, kFewRows * row, ctx->stream>>>(a);
 }
 
@@ -379,7 +383,7 @@ int product(BulletOuCudaCppContext* ctx, ProductArgs p, const BulletOuB200Matrix
     if (p.m <= kFewRows && kFewRows * padded(p.k, 16) <= kFewRowsBytes) {
         FewRowsArgs a{};
         a.p = p;
-        a.w_vector = tma_rows(p.w, p.n, p.w_stride);
+        a.w = bytes_of(p.w, p.w_stride, p.n, p.k);
         if (x != nullptr) {
             a.quantise = true;
             a.x = x->data;
@@ -401,7 +405,7 @@ int product(BulletOuCudaCppContext* ctx, ProductArgs p, const BulletOuB200Matrix
     int8_t* const w = q + q_bytes;
     RepackArgs weights{};
     if (own_w) {
-        if (p.k > 0) weights = {p.w, p.w_stride, w, pitch, p.n, p.k};
+        if (p.k > 0) weights = {bytes_of(p.w, p.w_stride, p.n, p.k), w, pitch};
         p.w = w;
         p.w_stride = pitch;
     }
@@ -409,8 +413,8 @@ int product(BulletOuCudaCppContext* ctx, ProductArgs p, const BulletOuB200Matrix
         if (quantize(ctx, *x, q, pitch, static_cast<int>(pitch), scales, weights) != 0) return -1;
         p.scales = scales;
     } else {
-        if (weights.rows > 0 && repack(ctx, weights) != 0) return -1;
-        if (own_q && p.k > 0 && repack(ctx, {p.q, p.q_stride, q, pitch, p.m, p.k}) != 0) return -1;
+        if (weights.src.rows > 0 && repack(ctx, weights) != 0) return -1;
+        if (own_q && p.k > 0 && repack(ctx, {bytes_of(p.q, p.q_stride, p.m, p.k), q, pitch}) != 0) return -1;
     }
     if (own_q) {
         p.q = q;
@@ -419,7 +423,7 @@ int product(BulletOuCudaCppContext* ctx, ProductArgs p, const BulletOuB200Matrix
     // a single row's stride is the caller's and may be anything
     if (p.m == 1) p.q_stride = pitch;
     if (p.n == 1) p.w_stride = pitch;
-    return launch_int8_mma(ctx, p, out_type, x != nullptr, weights.rows == 0);
+    return launch_int8_mma(ctx, p, out_type, x != nullptr, weights.src.rows == 0);
 }
 
 // The weight side's checks, shared by the two products.

@@ -141,8 +141,11 @@ template <int TN>
 struct TileShape {
     static constexpr uint32_t kStageBytes = kABytes + TN * kTileK;
     static constexpr int kStages = TN == 64 ? 4 : 3;  // 96 KB: two CTAs on an SM
+    // after the last MMA the stages hold the partial sums and the staged rows
+    static constexpr uint32_t kStagingAt = TN * kTileM * 4;
     static constexpr int kThreads = 128;
-    static constexpr uint32_t kSmem = kStages * kStageBytes + 4 * 32 * (32 + kStagePad) * 4 + 2 * TN * 4 + 256 + 1024;
+    static constexpr uint32_t kSmem = kStages * kStageBytes + 2 * TN * 4 + 256 + 1024;
+    static_assert(kStagingAt + 4 * 32 * (32 + kStagePad) * 4 <= kStages * kStageBytes);
 };
 
 // `splits` CTAs of a cluster share a tile and cut k; the grid is their tiles,
@@ -156,8 +159,8 @@ __global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ 
     const uint32_t raw_addr = smem_u32(raw);
     const uint32_t base = (raw_addr + 1023u) & ~1023u;  // swizzle atoms
     uint8_t* const stages = raw + (base - raw_addr);
-    float* const staging = reinterpret_cast<float*>(stages + S::kStages * S::kStageBytes);
-    float* const col_scale = staging + 4 * 32 * (32 + kStagePad);
+    float* const staging = reinterpret_cast<float*>(stages + S::kStagingAt);
+    float* const col_scale = reinterpret_cast<float*>(stages + S::kStages * S::kStageBytes);
     float* const col_bias = col_scale + TN;
     uint64_t* const bars = reinterpret_cast<uint64_t*>(col_bias + TN);  // full, empty, done
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S::kStages + 1);
@@ -485,7 +488,7 @@ template <typename Out>
 int launch_typed(BulletOuCudaCppContext* ctx, const ProductArgs& a, bool early, bool weights_ready) {
     const bool vector_ok = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && (a.m <= 1 || a.out_stride * sizeof(Out) % 16 == 0);
     const int64_t pairs = static_cast<int64_t>((a.m + 255) / 256) * ((a.n + 255) / 256);
-    if (pairs >= ctx->sm_count / 2 && pairs <= INT32_MAX)
+    if (pairs >= 32 && pairs <= INT32_MAX)
         return launch_pairs<Out>(ctx, a, static_cast<int>(pairs), vector_ok, early);
     const int64_t wide = static_cast<int64_t>((a.m + 127) / 128) * ((a.n + 127) / 128);
     return wide >= ctx->sm_count ? launch_tiles<128, Out>(ctx, a, vector_ok, early, weights_ready)

@@ -22,10 +22,13 @@ namespace bou {
 namespace {
 
 constexpr int kThreads = 256;
-// CTAs on an SM by the places of a lane: 64 registers for each thread, 80 for 16 places
+// By the places of a lane: CTAs on an SM of the backward pass, and threads of the
+// forward pass's one CTA on an SM (each CTA leaves sums to be joined): 64
+// registers for each thread, 80 for 16 places.
 template <int kPlaces>
 constexpr int kCtas = kPlaces > 12 ? 3 : 4;
-constexpr int kWarps = kThreads / 32;
+template <int kGroup, int kPlaces>  // (the sums of 512 experts for each warp fill the shared memory)
+constexpr int kForwardThreads = kThreads * (kGroup * kPlaces > 256 ? 2 : kCtas<kPlaces>);
 constexpr int kMaxExperts = BULLETOU_B200_ROUTER_MAX_EXPERTS;
 constexpr int kMaxTopK = BULLETOU_B200_ROUTER_MAX_TOP_K;
 constexpr int kJoinThreads = 1024;
@@ -164,7 +167,8 @@ __device__ void finish(const RouterArgs& a, const float* p_sums, const int* coun
 // kGroup lanes for each row (at least top_k), kPlaces experts in each lane.  One
 // CTA alone also finishes; otherwise the CTAs leave their sums to router_join_kernel.
 template <typename T, int kGroup, int kPlaces>
-__global__ void __launch_bounds__(kThreads, kCtas<kPlaces>) router_forward_kernel(const RouterArgs a) {
+__global__ void __launch_bounds__(kForwardThreads<kGroup, kPlaces>, 1) router_forward_kernel(const RouterArgs a) {
+    constexpr int kThreads = kForwardThreads<kGroup, kPlaces>, kWarps = kThreads / 32;
     __shared__ int count[kMaxExperts + 1];
     __shared__ float psum[kWarps][kGroup * kPlaces];
     const int lane = threadIdx.x & (kGroup - 1), warp = threadIdx.x >> 5;
@@ -378,18 +382,17 @@ int with_shape(const RouterArgs& a, F&& f) {
     return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 16>{});
 }
 
-// CTAs for the rows; up to four rounds of rows are left to one CTA, which then
+// CTAs for the rows; up to two rounds of rows are left to one CTA, which then
 // needs no second launch.
-int router_grid(const BulletOuCudaCppContext* ctx, int rows, int group, int resident) {
-    const int per = kThreads / group;
+int router_grid(const BulletOuCudaCppContext* ctx, int rows, int per) {
     const int64_t ctas = (static_cast<int64_t>(rows) + per - 1) / per;
-    return ctas <= 4 ? 1 : static_cast<int>(std::min<int64_t>(ctas, static_cast<int64_t>(ctx->sm_count) * resident));
+    return ctas <= 2 ? 1 : static_cast<int>(std::min<int64_t>(ctas, ctx->sm_count));
 }
 
 template <typename T>
 int forward(BulletOuCudaCppContext* ctx, RouterArgs a) {
     return with_shape(a, [&](auto group, auto places) {
-        const int grid = router_grid(ctx, a.rows, group, kCtas<places()>);
+        const int grid = router_grid(ctx, a.rows, kForwardThreads<group(), places()> / group());
         if (grid > 1) {
             void* p = nullptr;
             if (scratch_slot(ctx, kScratchRouter, static_cast<size_t>(grid) * (2 * a.experts + 1) * 4, &p,
@@ -398,7 +401,7 @@ int forward(BulletOuCudaCppContext* ctx, RouterArgs a) {
             a.part_p = static_cast<float*>(p);
             a.part_c = static_cast<int*>(p) + static_cast<size_t>(grid) * a.experts;
         }
-        LaunchShape shape{dim3(grid), kThreads};
+        LaunchShape shape{dim3(grid), kForwardThreads<group(), places()>};
         if (launch_kernel(ctx, "router forward launch", router_forward_kernel<T, group(), places()>, shape, a) != 0) return -1;
         if (grid == 1) return 0;
         LaunchShape join{dim3(1), kJoinThreads};
