@@ -96,6 +96,19 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
         : "memory");
 }
 
+// The results of 32 columns of a lane's row.
+__device__ __forceinline__ void results(const uint32_t* sum, float row_scale, const float* col_scale, const float* col_bias,
+                                        float* v) {
+#pragma unroll
+    for (int c = 0; c < 32; c += 4) {
+        const float4 s = *reinterpret_cast<const float4*>(col_scale + c), b = *reinterpret_cast<const float4*>(col_bias + c);
+        v[c] = int8_result(static_cast<int>(sum[c]), row_scale, s.x, b.x);
+        v[c + 1] = int8_result(static_cast<int>(sum[c + 1]), row_scale, s.y, b.y);
+        v[c + 2] = int8_result(static_cast<int>(sum[c + 2]), row_scale, s.z, b.z);
+        v[c + 3] = int8_result(static_cast<int>(sum[c + 3]), row_scale, s.w, b.w);
+    }
+}
+
 // A warp writes 32 rows x 32 columns, one row in each lane: through shared
 // memory, so that the global stores cover whole rows of the block.
 template <typename Out>
@@ -130,17 +143,22 @@ __device__ __forceinline__ void store_block(float* stage, const float* v, const 
             *reinterpret_cast<uint4*>(out + static_cast<size_t>(row0 + r) * a.out_stride + col0 + c) = packed;
         }
     } else if (col0 + lane < a.n) {
-        for (int r = 0; r < 32 && row0 + r < a.m; ++r)
-            out[static_cast<size_t>(row0 + r) * a.out_stride + col0 + lane] = from_f32<Out>(stage[r * kPitch + lane]);
+        Out* at = out + static_cast<size_t>(row0) * a.out_stride + col0 + lane;
+        const int rows = a.m - row0;
+#pragma unroll
+        for (int r = 0; r < 32; ++r, at += a.out_stride)
+            if (r < rows) *at = from_f32<Out>(stage[r * kPitch + lane]);
     }
     __syncwarp();
 }
 
 // ------------------------------------------------------------------ one tile for each CTA
-template <int TN>
+// kDeep: the SM's shared memory for one CTA, which has 1 KB of k of its tile on
+// the way at once; otherwise 96 KB, for two CTAs.
+template <int TN, bool kDeep>
 struct TileShape {
     static constexpr uint32_t kStageBytes = kABytes + TN * kTileK;
-    static constexpr int kStages = TN == 64 ? 4 : 3;  // 96 KB: two CTAs on an SM
+    static constexpr int kStages = kDeep ? 192 * 1024 / kStageBytes : 96 * 1024 / kStageBytes;
     // after the last MMA the stages hold the partial sums and the staged rows
     static constexpr uint32_t kStagingAt = TN * kTileM * 4;
     static constexpr int kThreads = 128;
@@ -150,11 +168,11 @@ struct TileShape {
 
 // `splits` CTAs of a cluster share a tile and cut k; the grid is their tiles,
 // the columns' tiles first.
-template <int TN, typename Out>
+template <int TN, bool kDeep, typename Out>
 __global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ CUtensorMap map_q,
                                                         const __grid_constant__ CUtensorMap map_w, const ProductArgs a,
-                                                        int splits, bool vector_ok, bool weights_ready) {
-    using S = TileShape<TN>;
+                                                        int splits, int box_rows, bool vector_ok, bool weights_ready) {
+    using S = TileShape<TN, kDeep>;
     extern __shared__ uint8_t raw[];
     const uint32_t raw_addr = smem_u32(raw);
     const uint32_t base = (raw_addr + 1023u) & ~1023u;  // swizzle atoms
@@ -165,7 +183,7 @@ __global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ 
     uint64_t* const bars = reinterpret_cast<uint64_t*>(col_bias + TN);  // full, empty, done
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S::kStages + 1);
     const uint32_t full = smem_u32(bars), empty = full + 8 * S::kStages, done = empty + 8 * S::kStages;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
 
     const int rank = splits > 1 ? static_cast<int>(cluster_rank()) : 0;
     const int tile = blockIdx.x / splits;
@@ -174,6 +192,7 @@ __global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ 
     const int blocks = (a.k + kTileK - 1) / kTileK;
     const int share = (blocks + splits - 1) / splits;
     const int k0 = min(blocks, rank * share), count = min(blocks, k0 + share) - k0;
+    const uint32_t stage_bytes = box_rows * kTileK + TN * kTileK;  // what a stage's loads bring
 
     if (tid == 0) {
         for (int s = 0; s < S::kStages; ++s) {
@@ -189,66 +208,74 @@ __global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ 
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    for (int c = tid; c < TN; c += S::kThreads) {
-        const bool in = col0 + c < a.n;
-        col_scale[c] = in ? a.w_scales[col0 + c] : 0.0f;
-        col_bias[c] = in && a.bias != nullptr ? a.bias[col0 + c] : 0.0f;
-    }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = uniform(*tmem_slot);
 
-    if (warp == 0 && lane == 0) {
-        // the weights of the first stages come while the rows are still being quantised
-        const int ahead = min(count, S::kStages);
-        if (!weights_ready) wait_for_previous();
-        for (int i = 0; i < ahead; ++i) {
-            mbar_expect_tx(full + 8 * i, S::kStageBytes);
-            tma_load_2d(base + i * S::kStageBytes + kABytes, &map_w, (k0 + i) * kTileK, col0, full + 8 * i);
-        }
-        wait_for_previous();
-        for (int i = 0; i < ahead; ++i) tma_load_2d(base + i * S::kStageBytes, &map_q, (k0 + i) * kTileK, row0, full + 8 * i);
-        for (int i = ahead; i < count; ++i) {
+    bool good = true;
+    if (warp == 0 || warp == 2) {
+        // One warp loads w, another q, since a load takes its time to issue.  The first
+        // weights come while the rows are still being quantised.
+        const bool rows = warp == 2;
+        if (rows || !weights_ready) wait_for_previous();
+        for (int i = 0; i < count && good; ++i) {
             const int s = i % S::kStages;
-            if (!mbar_wait(empty + 8 * s, (i / S::kStages - 1) & 1)) break;
-            mbar_expect_tx(full + 8 * s, S::kStageBytes);
-            tma_load_2d(base + s * S::kStageBytes, &map_q, (k0 + i) * kTileK, row0, full + 8 * s);
-            tma_load_2d(base + s * S::kStageBytes + kABytes, &map_w, (k0 + i) * kTileK, col0, full + 8 * s);
+            good = i < S::kStages || mbar_wait(empty + 8 * s, (i / S::kStages - 1) & 1);
+            if (good && elect_one()) {
+                const uint32_t stage = base + s * S::kStageBytes;
+                if (rows) {
+                    tma_load_2d(stage, &map_q, (k0 + i) * kTileK, row0, full + 8 * s);
+                } else {
+                    mbar_expect_tx(full + 8 * s, stage_bytes);
+                    tma_load_2d(stage + kABytes, &map_w, (k0 + i) * kTileK, col0, full + 8 * s);
+                }
+            }
+            __syncwarp();
         }
-    } else if (warp == 1 && lane == 0) {
-        bool good = true;
+    } else if (warp == 1) {
         for (int i = 0; i < count && good; ++i) {
             const int s = i % S::kStages;
             good = mbar_wait(full + 8 * s, (i / S::kStages) & 1);
-            if (!good) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t qa = base + s * S::kStageBytes, wa = qa + kABytes;
+            if (good && elect_one()) {
+                const uint64_t qd = k_major_desc(base + s * S::kStageBytes);
+                const uint64_t wd = k_major_desc(base + s * S::kStageBytes + kABytes);
 #pragma unroll
-            for (int j = 0; j < kTileK / 32; ++j)
-                mma_i8<1>(tmem, k_major_desc(qa + 32 * j), k_major_desc(wa + 32 * j), int8_idesc(kTileM, TN),
-                          (i | j) != 0 ? 1u : 0u);
-            commit_one(empty + 8 * s);
+                for (int j = 0; j < kTileK / 32; ++j)  // (a descriptor counts in 16 bytes)
+                    mma_i8<1>(tmem, qd + 2 * j, wd + 2 * j, int8_idesc(kTileM, TN), (i | j) != 0 ? 1u : 0u);
+                if (i + S::kStages < count) commit_one(empty + 8 * s);  // the stage is loaded again
+                if (i + 1 == count) commit_one(done);
+            }
+            __syncwarp();
         }
-        if (good && count > 0) commit_one(done);
+    } else {
+        for (int c = lane; c < TN; c += 32) {
+            const bool in = col0 + c < a.n;
+            col_scale[c] = in ? a.w_scales[col0 + c] : 0.0f;
+            col_bias[c] = in && a.bias != nullptr ? a.bias[col0 + c] : 0.0f;
+        }
     }
     __syncwarp();
-    const bool good = count == 0 || mbar_wait(done, 0);
+    wait_for_previous();  // the rows' scales
+    const int own_row = row0 + warp * 32 + lane;
+    const float own_scale = splits == 1 && own_row < a.m ? a.scales[own_row] : 0.0f;
+    good = count == 0 || mbar_wait(done, 0);
+    __syncthreads();  // the columns' scales
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    wait_for_previous();  // the scales
     float* const stage = staging + warp * 32 * (32 + kStagePad);
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
     if (splits == 1) {
-        const int row = row0 + warp * 32 + lane;
-        const float row_scale = row < a.m ? (good ? a.scales[row] : NAN) : 0.0f;
+        const float row_scale = good ? own_scale : NAN;
 #pragma unroll 1
         for (int c0 = 0; c0 < TN && col0 + c0 < a.n; c0 += 32) {
             uint32_t sum[32];
             float v[32];
             tmem_ld32(lanes + c0, sum);
+            if (count == 0)
 #pragma unroll
-            for (int c = 0; c < 32; ++c)
-                v[c] = int8_result(count > 0 ? static_cast<int>(sum[c]) : 0, row_scale, col_scale[c0 + c], col_bias[c0 + c]);
+                for (int c = 0; c < 32; ++c) sum[c] = 0;
+            results(sum, row_scale, col_scale + c0, col_bias + c0, v);
             store_block<Out>(stage, v, a, row0 + warp * 32, col0 + c0, vector_ok);
         }
     } else {
@@ -272,7 +299,7 @@ __global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ 
             const int group = job & 3, c0 = (job >> 2) * 32;
             const int row = row0 + group * 32 + lane;
             if (row0 + group * 32 >= a.m || col0 + c0 >= a.n) continue;
-            int sum[32] = {};
+            uint32_t sum[32] = {};
             bool broken = false;
             for (int r = 0; r < splits; ++r) {
                 const uint32_t from = map_rank(mine, r);
@@ -282,8 +309,7 @@ __global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ 
             }
             const float row_scale = row < a.m ? (broken ? NAN : a.scales[row]) : 0.0f;
             float v[32];
-#pragma unroll
-            for (int c = 0; c < 32; ++c) v[c] = int8_result(sum[c], row_scale, col_scale[c0 + c], col_bias[c0 + c]);
+            results(sum, row_scale, col_scale + c0, col_bias + c0, v);
             store_block<Out>(stage, v, a, row0 + group * 32, col0 + c0, vector_ok);
         }
         cluster_sync();  // no CTA leaves while another reads its sums
@@ -321,7 +347,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const uint32_t full = smem_u32(bars), empty = full + 8 * kPairStages, tile_full = empty + 8 * kPairStages,
                    tile_empty = tile_full + 16;
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kPairStages + 4);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
     const uint32_t rank = cluster_rank();
 
     if (tid == 0) {
@@ -345,7 +371,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     __syncthreads();
     cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = uniform(*tmem_slot);
     wait_for_previous();
 
     const int tiles_m = (a.m + 2 * kTileM - 1) / (2 * kTileM), tiles_n = (a.n + kPairN - 1) / kPairN;
@@ -360,48 +386,53 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     };
     const int first_tile = blockIdx.x >> 1, step = gridDim.x >> 1;
 
-    if (warp == 0 && lane == 0) {
+    bool good = true;
+    if (warp == 0) {
         int i = 0;
-        bool good = true;
         for (int t = first_tile; t < tiles && good; t += step) {
             int row0, col0;
             place(t, row0, col0);
-            for (int kb = 0; kb < blocks; ++kb, ++i) {
+            for (int kb = 0; kb < blocks && good; ++kb, ++i) {
                 const int s = i % kPairStages;
-                if (i >= kPairStages && !(good = mbar_wait(empty + 8 * s, (i / kPairStages - 1) & 1))) break;
-                if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * kPairStageBytes);
-                const uint32_t bar = map_rank(full + 8 * s, 0), dst = base + s * kPairStageBytes;
-                tma_load_pair(dst, &map_q, kb * kTileK, row0, bar);
-                tma_load_pair(dst + kABytes, &map_w, kb * kTileK, col0 + static_cast<int>(rank) * kTileM, bar);
+                good = i < kPairStages || mbar_wait(empty + 8 * s, (i / kPairStages - 1) & 1);
+                if (good && elect_one()) {
+                    if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * kPairStageBytes);
+                    const uint32_t bar = map_rank(full + 8 * s, 0), dst = base + s * kPairStageBytes;
+                    tma_load_pair(dst, &map_q, kb * kTileK, row0, bar);
+                    tma_load_pair(dst + kABytes, &map_w, kb * kTileK, col0 + static_cast<int>(rank) * kTileM, bar);
+                }
+                __syncwarp();
             }
         }
         // without a failure every copy was consumed; after one the last of each stage is waited for
         if (!good && rank == 0)
             for (int j = max(0, i - kPairStages); j < i; ++j) mbar_wait(full + 8 * (j % kPairStages), (j / kPairStages) & 1);
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+    } else if (warp == 1 && rank == 0) {
         int i = 0;
-        bool good = true;
         for (int t = first_tile, n = 0; t < tiles && good; t += step, ++n) {
             const int b = n & 1;
-            if (n >= 2 && !(good = mbar_wait(tile_empty + 8 * b, (n / 2 - 1) & 1))) break;
+            good = n < 2 || mbar_wait(tile_empty + 8 * b, (n / 2 - 1) & 1);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            for (int kb = 0; kb < blocks; ++kb, ++i) {
+            for (int kb = 0; kb < blocks && good; ++kb, ++i) {
                 const int s = i % kPairStages;
-                if (!(good = mbar_wait(full + 8 * s, (i / kPairStages) & 1))) break;
+                good = mbar_wait(full + 8 * s, (i / kPairStages) & 1);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t qa = base + s * kPairStageBytes, wa = qa + kABytes;
+                if (good && elect_one()) {
+                    const uint64_t qd = k_major_desc(base + s * kPairStageBytes);
+                    const uint64_t wd = k_major_desc(base + s * kPairStageBytes + kABytes);
 #pragma unroll
-                for (int j = 0; j < kTileK / 32; ++j)
-                    mma_i8<2>(tmem + b * kPairN, k_major_desc(qa + 32 * j), k_major_desc(wa + 32 * j),
-                              int8_idesc(2 * kTileM, kPairN), (kb | j) != 0 ? 1u : 0u);
-                commit_pair(empty + 8 * s);
+                    for (int j = 0; j < kTileK / 32; ++j)  // (a descriptor counts in 16 bytes)
+                        mma_i8<2>(tmem + b * kPairN, qd + 2 * j, wd + 2 * j, int8_idesc(2 * kTileM, kPairN),
+                                  (kb | j) != 0 ? 1u : 0u);
+                    commit_pair(empty + 8 * s);
+                    if (kb + 1 == blocks) commit_pair(tile_full + 8 * b);
+                }
+                __syncwarp();
             }
-            if (good) commit_pair(tile_full + 8 * b);
         }
     } else if (warp >= 2) {
         const int quarter = warp & 3;  // the TMEM lanes this warp may read
         float* const stage = staging + quarter * 32 * (32 + kStagePad);
-        bool good = true;
         for (int t = first_tile, n = 0; t < tiles; t += step, ++n) {
             const int b = n & 1;
             int row0, col0;
@@ -414,19 +445,18 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             }
             asm volatile("bar.sync 1, 128;" ::: "memory");
             const int row = row0 + quarter * 32 + lane;
+            const float own_scale = row < a.m ? a.scales[row] : 0.0f;
             good = good && mbar_wait(tile_full + 8 * b, (n / 2) & 1);
             good = __all_sync(0xffffffffu, good);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const float row_scale = row < a.m ? (good ? a.scales[row] : NAN) : 0.0f;
+            const float row_scale = good ? own_scale : NAN;
             const uint32_t lanes = tmem + b * kPairN + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll 1
             for (int c0 = 0; c0 < kPairN && col0 + c0 < a.n; c0 += 32) {
                 uint32_t sum[32];
                 float v[32];
                 tmem_ld32(lanes + c0, sum);
-#pragma unroll
-                for (int c = 0; c < 32; ++c)
-                    v[c] = int8_result(static_cast<int>(sum[c]), row_scale, col_scale[c0 + c], col_bias[c0 + c]);
+                results(sum, row_scale, col_scale + c0, col_bias + c0, v);
                 store_block<Out>(stage, v, a, row0 + quarter * 32, col0 + c0, vector_ok);
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -461,18 +491,28 @@ int operand_map(CUtensorMap* map, const int8_t* data, int rows, int k, size_t st
     return 0;
 }
 
+template <int TN, bool kDeep, typename Out>
+int launch_tiles(BulletOuCudaCppContext* ctx, const ProductArgs& a, int64_t tiles, int splits, bool vector_ok, bool early, bool weights_ready) {
+    using S = TileShape<TN, kDeep>;
+    CUtensorMap q, w;
+    // few rows are loaded as they are: the rest of the tile is what the stage
+    // held before and reaches no result
+    const int box_rows = std::min(kTileM, (a.m + 7) / 8 * 8);
+    if (operand_map(&q, a.q, a.m, a.k, a.q_stride, box_rows) != 0 || operand_map(&w, a.w, a.n, a.k, a.w_stride, TN) != 0)
+        return -1;
+    const LaunchShape shape{dim3(static_cast<unsigned>(tiles * splits)), S::kThreads, S::kSmem, splits, early};
+    return launch_kernel(ctx, "int8 product launch", int8_tile_kernel<TN, kDeep, Out>, shape, q, w, a, splits, box_rows, vector_ok, weights_ready);
+}
+
 template <int TN, typename Out>
 int launch_tiles(BulletOuCudaCppContext* ctx, const ProductArgs& a, bool vector_ok, bool early, bool weights_ready) {
     const int64_t tiles = static_cast<int64_t>((a.m + kTileM - 1) / kTileM) * ((a.n + TN - 1) / TN);
     const int blocks = (a.k + kTileK - 1) / kTileK;
     int splits = 1;
-    while (splits < 4 && tiles * splits * 2 <= ctx->sm_count && blocks >= 4 * splits) splits *= 2;
+    while (splits < 4 && tiles * splits * 2 <= ctx->sm_count && blocks >= 16 * splits) splits *= 2;
     if (tiles * splits > INT32_MAX) return fail_messagef("int8 product: %d x %d results are too many", a.m, a.n);
-    CUtensorMap q, w;
-    if (operand_map(&q, a.q, a.m, a.k, a.q_stride, kTileM) != 0 || operand_map(&w, a.w, a.n, a.k, a.w_stride, TN) != 0)
-        return -1;
-    const LaunchShape shape{dim3(static_cast<unsigned>(tiles * splits)), TileShape<TN>::kThreads, TileShape<TN>::kSmem, splits, early};
-    return launch_kernel(ctx, "int8 product launch", int8_tile_kernel<TN, Out>, shape, q, w, a, splits, vector_ok, weights_ready);
+    return tiles * splits <= ctx->sm_count ? launch_tiles<TN, true, Out>(ctx, a, tiles, splits, vector_ok, early, weights_ready)
+                                           : launch_tiles<TN, false, Out>(ctx, a, tiles, splits, vector_ok, early, weights_ready);
 }
 
 template <typename Out>

@@ -21,6 +21,23 @@ __device__ __forceinline__ uint64_t global_ns() {
     return t;
 }
 
+// One lane of a converged warp.  TMA and MMA instructions take their operands
+// from uniform registers; behind this predicate the compiler knows that one
+// lane runs them, behind a comparison of the lane's number it serialises over
+// the lanes (about 70 cycles for each instruction).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+    return one != 0;
+}
+
+// A value that is the same in the whole warp, as one that the compiler knows to
+// be so.
+template <typename T>
+__device__ __forceinline__ T uniform(T v) {
+    return __shfl_sync(0xffffffffu, v, 0);
+}
+
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
