@@ -20,20 +20,34 @@ constexpr int kThreads = 256;
 constexpr int kLanes = 8;  // elements of one Philox block
 constexpr int kCtas = 4;   // CTAs on an SM: 64 registers for each thread
 
+constexpr int kRounds = 10;
+
 struct Philox {
     uint32_t w[4];
 };
 
-__device__ __forceinline__ Philox philox_block(uint64_t block, uint2 offset, uint2 key) {
-    uint32_t x0 = static_cast<uint32_t>(block), x1 = static_cast<uint32_t>(block >> 32), x2 = offset.x, x3 = offset.y;
+struct PhiloxKeys {
+    uint2 offset;
+    uint2 round[kRounds];  // the key of each round
+};
+
+PhiloxKeys philox_keys(uint64_t seed, uint64_t offset) {
+    PhiloxKeys k{};
+    k.offset = make_uint2(static_cast<uint32_t>(offset), static_cast<uint32_t>(offset >> 32));
+    for (uint32_t r = 0; r < kRounds; ++r)
+        k.round[r] = make_uint2(static_cast<uint32_t>(seed) + 0x9e3779b9u * r, static_cast<uint32_t>(seed >> 32) + 0xbb67ae85u * r);
+    return k;
+}
+
+__device__ __forceinline__ Philox philox_block(uint64_t block, const PhiloxKeys& k) {
+    uint32_t x0 = static_cast<uint32_t>(block), x1 = static_cast<uint32_t>(block >> 32), x2 = k.offset.x, x3 = k.offset.y;
 #pragma unroll
-    for (int r = 0; r < 10; ++r) {
+    for (int r = 0; r < kRounds; ++r) {
         const uint64_t a = static_cast<uint64_t>(0xd2511f53u) * x0;
         const uint64_t b = static_cast<uint64_t>(0xcd9e8d57u) * x2;
-        const uint32_t k0 = key.x + 0x9e3779b9u * r, k1 = key.y + 0xbb67ae85u * r;
-        x0 = static_cast<uint32_t>(b >> 32) ^ x1 ^ k0;
+        x0 = static_cast<uint32_t>(b >> 32) ^ x1 ^ k.round[r].x;
         x1 = static_cast<uint32_t>(b);
-        x2 = static_cast<uint32_t>(a >> 32) ^ x3 ^ k1;
+        x2 = static_cast<uint32_t>(a >> 32) ^ x3 ^ k.round[r].y;
         x3 = static_cast<uint32_t>(a);
     }
     return {{x0, x1, x2, x3}};
@@ -47,7 +61,7 @@ struct DropoutArgs {
     size_t cols;
     bool flat;                        // no gaps between the rows of any operand
     size_t x_stride, residual_stride, out_stride;
-    uint2 key, offset;
+    PhiloxKeys keys;
     uint32_t threshold;               // dropped below; 65536: everything
     float factor;
 };
@@ -113,7 +127,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) dropout_vector_kernel(const D
         for (int i = 0; i < kBlocks; ++i) {
             const size_t b = b0 + i * step;
             if (b >= blocks) break;
-            const Philox random = philox_block(b, a.offset, a.key);
+            const Philox random = philox_block(b, a.keys);
 #pragma unroll
             for (int j = 0; j < kLanes; ++j) {
                 const float v = kept(random, j, a.threshold) ? x[i].get(j) : 0.0f;
@@ -125,51 +139,65 @@ __global__ void __launch_bounds__(kThreads, kCtas) dropout_vector_kernel(const D
     // the last elements of a flat vector
     if (kFlat && blockIdx.x == 0 && threadIdx.x < a.n - blocks * kLanes) {
         const size_t e = blocks * kLanes + threadIdx.x;
-        const Philox random = philox_block(blocks, a.offset, a.key);
+        const Philox random = philox_block(blocks, a.keys);
         const float v = kept(random, threadIdx.x, a.threshold) ? to_f32(static_cast<const T*>(a.x)[e]) : 0.0f;
         static_cast<T*>(a.out)[e] = from_f32<T>(kResidual ? __fmaf_rn(v, a.factor, to_f32(static_cast<const T*>(a.residual)[e]))
                                                           : v * a.factor);
     }
 }
 
-// Rows of any stride and alignment, wide ones: a warp takes a piece of a row, up
-// to kPiece elements, whose blocks its 32 lanes can compute wherever the piece
-// begins inside a block.  The elements are read and written 32 neighbours at a
-// time, each lane asking the lane that holds its element's block.
-constexpr int kPiece = 31 * kLanes;
+// Rows of any stride and alignment, wide ones: a warp takes pieces of 7 x 32
+// elements of a row, whose blocks its 32 lanes can compute wherever the piece
+// begins inside a block.  The lanes' decisions on each block's k-th element make
+// one word; a lane's elements are all the k-th of their blocks, 4 blocks apart,
+// so it picks its word once and tests a bit for each element.  The elements are
+// read and written 32 neighbours at a time.
+constexpr int kTurns = 7;
+constexpr int kPiece = kTurns * 32;
 constexpr int kWideRow = 64;  // columns from which a piece fills most of a warp's turns
+template <bool kResidual>
+constexpr int kRowCtas = kResidual ? 4 : 6;
+
+template <bool kFull, typename T, bool kResidual>
+__device__ __forceinline__ void dropout_piece(const DropoutArgs& a, size_t row, size_t col, int count) {
+    const int lane = threadIdx.x & 31;
+    const T* const x_at = static_cast<const T*>(a.x) + row * a.x_stride + col + lane;
+    const T* const r_at = kResidual ? static_cast<const T*>(a.residual) + row * a.residual_stride + col + lane : nullptr;
+    T* const out = static_cast<T*>(a.out) + row * a.out_stride + col + lane;
+    const int left = count - lane;
+    T x[kTurns], r[kTurns];
+#pragma unroll
+    for (int j = 0; j < kTurns; ++j)
+        if (kFull || j * 32 < left) {
+            x[j] = x_at[j * 32];
+            if (kResidual) r[j] = r_at[j * 32];
+        }
+    const size_t element = row * a.cols + col;
+    const Philox random = philox_block(element / kLanes + lane, a.keys);
+    const int place = static_cast<int>(element % kLanes) + lane;
+    uint32_t word = 0;
+#pragma unroll
+    for (int k = 0; k < kLanes; ++k) {
+        const uint32_t decisions = __ballot_sync(0xffffffffu, kept(random, k, a.threshold));
+        if ((place & (kLanes - 1)) == k) word = decisions;
+    }
+    word >>= place / kLanes;
+#pragma unroll
+    for (int j = 0; j < kTurns; ++j)
+        if (kFull || j * 32 < left) {
+            const float v = word & (1u << (4 * j)) ? to_f32(x[j]) : 0.0f;
+            out[j * 32] = from_f32<T>(kResidual ? __fmaf_rn(v, a.factor, to_f32(r[j])) : v * a.factor);
+        }
+}
 
 template <typename T, bool kResidual>
-__global__ void __launch_bounds__(kThreads, kCtas) dropout_row_kernel(const DropoutArgs a, int pieces, int piece) {
-    const int lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(kThreads, kRowCtas<kResidual>) dropout_row_kernel(const DropoutArgs a, int pieces) {
     const size_t rows = a.n / a.cols, step = static_cast<size_t>(gridDim.x) * (kThreads / 32);
     for (size_t row = static_cast<size_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); row < rows; row += step)
         for (int s = blockIdx.y; s < pieces; s += gridDim.y) {
-            const size_t col = static_cast<size_t>(s) * piece;
-            const int count = static_cast<int>(min(static_cast<size_t>(piece), a.cols - col));
-            const T* const x_at = static_cast<const T*>(a.x) + row * a.x_stride + col + lane;
-            const T* const r_at = kResidual ? static_cast<const T*>(a.residual) + row * a.residual_stride + col + lane : nullptr;
-            T* const out = static_cast<T*>(a.out) + row * a.out_stride + col + lane;
-            T x[kLanes], r[kLanes];
-#pragma unroll
-            for (int j = 0; j < kLanes; ++j)
-                if (j * 32 + lane < count) {
-                    x[j] = x_at[j * 32];
-                    if (kResidual) r[j] = r_at[j * 32];
-                }
-            const size_t element = row * a.cols + col;
-            const Philox random = philox_block(element / kLanes + lane, a.offset, a.key);
-            uint32_t mask = 0;
-#pragma unroll
-            for (int j = 0; j < kLanes; ++j) mask |= kept(random, j, a.threshold) ? 1u << j : 0u;
-            const int place = static_cast<int>(element % kLanes) + lane;
-#pragma unroll
-            for (int j = 0; j < kLanes; ++j) {
-                if (j * 32 >= count) break;  // for the whole warp
-                const uint32_t theirs = __shfl_sync(0xffffffffu, mask, (j * 32 + place) >> 3);
-                const float v = (theirs >> (place & 7)) & 1u ? to_f32(x[j]) : 0.0f;
-                if (j * 32 + lane < count) out[j * 32] = from_f32<T>(kResidual ? __fmaf_rn(v, a.factor, to_f32(r[j])) : v * a.factor);
-            }
+            const size_t col = static_cast<size_t>(s) * kPiece;
+            if (a.cols - col >= kPiece) dropout_piece<true, T, kResidual>(a, row, col, kPiece);
+            else dropout_piece<false, T, kResidual>(a, row, col, static_cast<int>(a.cols - col));
         }
 }
 
@@ -205,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) dropout_kernel(const DropoutA
             x_at += x_step + (wrap ? x_wrap : 0);
             if (kResidual) r_at += r_step + (wrap ? r_wrap : 0);
         }
-        const Philox random = philox_block(b0 + lane, a.offset, a.key);
+        const Philox random = philox_block(b0 + lane, a.keys);
         uint32_t mask = 0;
 #pragma unroll
         for (int j = 0; j < kLanes; ++j) mask |= kept(random, j, a.threshold) ? 1u << j : 0u;
@@ -228,11 +256,10 @@ int launch_dropout(BulletOuCudaCppContext* ctx, const DropoutArgs& a, bool vecto
     if (!vector && a.cols >= kWideRow) {
         const int64_t rows = static_cast<int64_t>(a.n / a.cols), row_ctas = (rows + kThreads / 32 - 1) / (kThreads / 32);
         const int pieces = static_cast<int>((a.cols + kPiece - 1) / kPiece);
-        const int piece = static_cast<int>((a.cols + pieces - 1) / pieces);
-        const int64_t resident = static_cast<int64_t>(ctx->sm_count) * kCtas;
+        const int64_t resident = static_cast<int64_t>(ctx->sm_count) * kRowCtas<kResidual>;
         const unsigned x = static_cast<unsigned>(std::min(row_ctas, resident));
         const unsigned y = static_cast<unsigned>(std::min<int64_t>(pieces, std::max<int64_t>(1, resident / x)));
-        return launch_kernel(ctx, "dropout launch", dropout_row_kernel<T, kResidual>, LaunchShape{dim3(x, y), kThreads}, a, pieces, piece);
+        return launch_kernel(ctx, "dropout launch", dropout_row_kernel<T, kResidual>, LaunchShape{dim3(x, y), kThreads}, a, pieces);
     }
     if (!vector) return launch_kernel(ctx, "dropout launch", dropout_kernel<T, kResidual>, shape, a);
     if (a.flat) return launch_kernel(ctx, "dropout launch", dropout_vector_kernel<T, kResidual, true>, shape, a);
@@ -273,8 +300,7 @@ int bulletou_b200_dropout_device(BulletOuCudaCppContext* ctx, const BulletOuB200
     a.x_stride = x->row_stride;
     a.residual_stride = residual != nullptr ? residual->row_stride : 0;
     a.out_stride = out->row_stride;
-    a.key = make_uint2(static_cast<uint32_t>(seed), static_cast<uint32_t>(seed >> 32));
-    a.offset = make_uint2(static_cast<uint32_t>(offset), static_cast<uint32_t>(offset >> 32));
+    a.keys = philox_keys(seed, offset);
     a.threshold = static_cast<uint32_t>(std::floor(static_cast<double>(probability) * 65536.0 + 0.5));
     a.factor = a.threshold < 65536u ? static_cast<float>(65536.0 / (65536.0 - a.threshold)) : 0.0f;
     // a vector where every eight is aligned: rows of whole eights, or no gaps between rows at all
