@@ -86,5 +86,6 @@ from .token_layers import (  # noqa: F401
     DeviceMatrix, dropout, dropout_backward, embedding_backward, embedding_forward, int8_linear, int8_matmul,
     int8_quantize_rows, router_backward, router_forward,
 )
+from .stack_router import StackRouter  # noqa: F401
 
 __version__ = "0.1.0"
