@@ -68,6 +68,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
+__device__ __forceinline__ float max_nan(float a, float2 b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b.x), "f"(b.y));
+    return y;
+}
 __device__ __forceinline__ float reciprocal_approx(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -95,44 +100,86 @@ __device__ __forceinline__ int group_min(int v) {
     return v;
 }
 
+// Two f32 operations in one instruction, each rounded as by itself.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 y;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(y))
+        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+    return y;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 y;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(y))
+        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+    return y;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 y;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t&>(y))
+        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
+          "l"(reinterpret_cast<const uint64_t&>(c)));
+    return y;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 // A row's logits and their exponentials: expert e in lane e % kGroup, place
-// e / kGroup; places past the last expert hold -inf and 0.  All lanes of a warp
-// come here together; a row past the end is one that is not alive.
+// e / kGroup; only the last two places may lie past the last expert, and hold
+// -inf and 0 there.  All lanes of a warp come here together; a row past the end
+// is one that is not alive.
 //
 // exp(z - top) is taken as 2^((z - top) log2 e): two roundings of 2^-24 relative
 // in an exponent below 20 wherever p > 10^-6.
 template <int kGroup, int kPlaces>
 struct Row {
-    float z[kPlaces];
-    float e[kPlaces];
+    static_assert(kPlaces % 2 == 0);
+    float2 z[kPlaces / 2];
+    float2 e[kPlaces / 2];
     float top, shift, inverse;  // p = e * inverse, e = exp(z - shift); shift is top where that is finite
     bool alive;                 // the largest logit is finite
 
+    __device__ __forceinline__ float& logit(int i) { return i % 2 == 0 ? z[i / 2].x : z[i / 2].y; }
+    __device__ __forceinline__ float largest() const {
+        float m = max_nan(z[0].x, z[0].y);
+#pragma unroll
+        for (int i = 1; i < kPlaces / 2; ++i) m = max_nan(m, z[i]);
+        return m;
+    }
     __device__ __forceinline__ float exponential(float logit) const { return exp2_approx((logit - shift) * kLog2E); }
 
+    // `src`: the row's logit in place 0 of this lane; `mine`: the places that it has, 0 in a row past the end.
     template <typename T>
-    __device__ __forceinline__ void load(const RouterArgs& a, int64_t t, int lane) {
-        const T* src = static_cast<const T*>(a.logits) + t * a.logit_stride + lane;
-        const int mine = t < a.rows ? a.experts - lane : 0;
+    __device__ __forceinline__ void load(const T* src, int mine) {
+        const bool valid = mine > 0;
 #pragma unroll
-        for (int i = 0; i < kPlaces; ++i) z[i] = kGroup * i < mine ? to_f32(src[kGroup * i]) : -INFINITY;
-        top = z[0];
-#pragma unroll
-        for (int i = 1; i < kPlaces; ++i) top = max_nan(top, z[i]);
-        top = group_max<kGroup>(top);
+        for (int i = 0; i < kPlaces; ++i)
+            logit(i) = (i < kPlaces - 2 ? valid : i < mine) ? to_f32(src[kGroup * i]) : -INFINITY;
+    }
+
+    __device__ __forceinline__ void normalise() {
+        top = group_max<kGroup>(largest());
         alive = top > -INFINITY && top < INFINITY;
         shift = alive ? top : 0.0f;
-        float sum = 0.0f;
+        float2 sum = both(0.0f);
 #pragma unroll
-        for (int i = 0; i < kPlaces; ++i) {
-            e[i] = exponential(z[i]);
-            sum += e[i];
+        for (int i = 0; i < kPlaces / 2; ++i) {
+            const float2 x = mul2(add2(z[i], both(-shift)), both(kLog2E));
+            e[i] = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+            sum = add2(sum, e[i]);
         }
-        sum = group_sum<kGroup>(sum);
+        const float total = group_sum<kGroup>(sum.x + sum.y);
         // a masked row's exponentials are zeros; a broken row is NaN
-        inverse = alive ? reciprocal_approx(sum) : top == -INFINITY ? 0.0f : NAN;
+        inverse = alive ? reciprocal_approx(total) : top == -INFINITY ? 0.0f : NAN;
     }
 };
+
+// The places that this lane has in a row of `experts`.
+template <int kGroup>
+__device__ __forceinline__ int places_of(int experts, int lane) {
+    return (experts - lane + kGroup - 1) / kGroup;
+}
 
 // Means and loss from the sums of the probabilities and the counts; every
 // thread of the CTA comes here.
@@ -175,15 +222,22 @@ __global__ void __launch_bounds__(kForwardThreads<kGroup, kPlaces>, 1) router_fo
     let_next_start();
     for (int i = threadIdx.x; i <= a.experts; i += kThreads) count[i] = 0;
     __syncthreads();
-    float acc[kPlaces] = {};
+    float2 acc[kPlaces / 2] = {};
     int alive = 0;
     constexpr int kRows = kThreads / kGroup;
-    for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * kRows; t0 < a.rows; t0 += static_cast<int64_t>(gridDim.x) * kRows) {
-        const int64_t t = t0 + threadIdx.x / kGroup;
+    const int places = places_of<kGroup>(a.experts, lane);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+    int64_t t = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kGroup;
+    const T* src = static_cast<const T*>(a.logits) + t * a.logit_stride + lane;
+    int* chosen = a.chosen + t * a.chosen_stride + lane;
+    float* gates = a.gates + t * a.gate_stride + lane;
+    // (the lanes of a warp stay together for the trees)
+    for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * kRows; t0 < a.rows; t0 += step, t += step) {
         Row<kGroup, kPlaces> r;
-        r.template load<T>(a, t, lane);
+        r.template load<T>(src, t < a.rows ? places : 0);
+        r.normalise();
 #pragma unroll
-        for (int i = 0; i < kPlaces; ++i) acc[i] = __fmaf_rn(r.e[i], r.inverse, acc[i]);
+        for (int i = 0; i < kPlaces / 2; ++i) acc[i] = fma2(r.e[i], both(r.inverse), acc[i]);
         alive += r.alive && lane == 0;
         float total = 0.0f, own = 0.0f;  // lane j keeps the j-th choice
         int pick = -1;
@@ -192,7 +246,7 @@ __global__ void __launch_bounds__(kForwardThreads<kGroup, kPlaces>, 1) router_fo
             int at = kMaxExperts;  // the lowest index that has the largest logit left
 #pragma unroll
             for (int i = kPlaces - 1; i >= 0; --i)
-                if (r.z[i] == best) at = lane + kGroup * i;
+                if (r.logit(i) == best) at = lane + kGroup * i;
             at = group_min<kGroup>(at);
             const bool some = r.alive && best > -INFINITY;
             const float gate = some ? r.exponential(best) * r.inverse : 0.0f;
@@ -204,24 +258,25 @@ __global__ void __launch_bounds__(kForwardThreads<kGroup, kPlaces>, 1) router_fo
             if (++j >= a.top_k) break;
 #pragma unroll
             for (int i = 0; i < kPlaces; ++i)
-                if (lane + kGroup * i == at) r.z[i] = -INFINITY;
-            best = r.z[0];
-#pragma unroll
-            for (int i = 1; i < kPlaces; ++i) best = fmaxf(best, r.z[i]);
-            best = group_max<kGroup>(best);
+                if (lane + kGroup * i == at) r.logit(i) = -INFINITY;
+            best = group_max<kGroup>(r.largest());
         }
         if (lane < a.top_k && t < a.rows) {
-            a.chosen[t * a.chosen_stride + lane] = pick;
-            a.gates[t * a.gate_stride + lane] = a.normalize && pick >= 0 ? own * reciprocal_approx(total) : own;
+            *chosen = pick;
+            *gates = a.normalize && pick >= 0 ? own * reciprocal_approx(total) : own;
             if (pick >= 0) atomicAdd(count + pick, 1);
         }
+        src += step * a.logit_stride;
+        chosen += step * a.chosen_stride;
+        gates += step * a.gate_stride;
     }
     if (alive != 0) atomicAdd(count + a.experts, alive);
 #pragma unroll
     for (int i = 0; i < kPlaces; ++i) {
+        float s = i % 2 == 0 ? acc[i / 2].x : acc[i / 2].y;
 #pragma unroll
-        for (int d = kGroup; d < 32; d <<= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], d);
-        if ((threadIdx.x & 31) < kGroup) psum[warp][lane + kGroup * i] = acc[i];
+        for (int d = kGroup; d < 32; d <<= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        if ((threadIdx.x & 31) < kGroup) psum[warp][lane + kGroup * i] = s;
     }
     __syncthreads();
     for (int e = threadIdx.x; e < a.experts; e += kThreads) {
@@ -293,48 +348,57 @@ __global__ void __launch_bounds__(kJoinThreads) router_join_kernel(const RouterA
 template <typename T, int kGroup, int kPlaces>
 __global__ void __launch_bounds__(kThreads, kCtas<kPlaces>) router_backward_kernel(const RouterArgs a) {
     __shared__ int choices;
+    __shared__ int shared_counts[kGroup * kPlaces];
     const int lane = threadIdx.x & (kGroup - 1);
     if (threadIdx.x == 0) choices = 0;
     __syncthreads();
     int c = 0;
-    for (int e = threadIdx.x; e < a.experts; e += kThreads) c += a.counts[e];
+    for (int e = threadIdx.x; e < kGroup * kPlaces; e += kThreads) {
+        shared_counts[e] = e < a.experts ? a.counts[e] : 0;
+        c += shared_counts[e];
+    }
     if (c != 0) atomicAdd(&choices, c);
     __syncthreads();
     // the balance loss's pull on every probability of an expert
-    float h[kPlaces];
+    float2 h[kPlaces / 2];
     const float unit = (a.loss_grad != nullptr ? a.loss_grad[0] : 0.0f) * a.balance * static_cast<float>(a.experts) /
                        static_cast<float>(max(a.counts[a.experts], 1)) / static_cast<float>(max(choices, 1));
+    auto pull_of = [&](int e) { return static_cast<float>(shared_counts[e]) * unit; };
 #pragma unroll
-    for (int i = 0; i < kPlaces; ++i) {
-        const int e = lane + kGroup * i;
-        h[i] = e < a.experts ? static_cast<float>(a.counts[e]) * unit : 0.0f;
-    }
-    const T* const logits = static_cast<const T*>(a.logits);
+    for (int i = 0; i < kPlaces / 2; ++i) h[i] = make_float2(pull_of(lane + kGroup * 2 * i), pull_of(lane + kGroup * (2 * i + 1)));
     constexpr int kRows = kThreads / kGroup;
-    for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * kRows; t0 < a.rows; t0 += static_cast<int64_t>(gridDim.x) * kRows) {
-        const int64_t t = t0 + threadIdx.x / kGroup;
-        // lane j holds the j-th choice: its logit, its pull and its gate's gradient
-        int pick = -1;
-        float up = 0.0f, z = -INFINITY, pull = 0.0f;
-        if (a.gate_grad != nullptr && lane < a.top_k && t < a.rows) {
-            pick = a.chosen[t * a.chosen_stride + lane];
-            if (pick >= 0 && pick < a.experts) {
-                up = a.gate_grad[t * a.gate_grad_stride + lane];
-                z = to_f32(logits[t * a.logit_stride + pick]);
-                pull = static_cast<float>(a.counts[pick]) * unit;
-            } else {
-                pick = -1;
-            }
-        }
+    const int places = places_of<kGroup>(a.experts, lane);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+    int64_t t = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kGroup;
+    const T* src = static_cast<const T*>(a.logits) + t * a.logit_stride + lane;
+    T* dst = static_cast<T*>(a.logit_grad) + t * a.logit_grad_stride + lane;
+    const int* chosen = a.chosen + t * a.chosen_stride + lane;
+    const float* gate_grad = a.gate_grad + t * a.gate_grad_stride + lane;
+    // lane j holds the j-th choice and its gate's gradient, of the next row already
+    const bool chooses = a.gate_grad != nullptr && lane < a.top_k;
+    int next_pick = chooses && t < a.rows ? *chosen : -1;
+    float next_up = chooses && t < a.rows ? *gate_grad : 0.0f;
+    for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * kRows; t0 < a.rows; t0 += step, t += step) {
+        const int mine = t < a.rows ? places : 0;
+        const int pick = next_pick >= 0 && next_pick < a.experts ? next_pick : -1;
+        const float up = pick >= 0 ? next_up : 0.0f;
         Row<kGroup, kPlaces> r;
-        r.template load<T>(a, t, lane);
+        r.template load<T>(src, mine);
+        const float z = pick >= 0 ? to_f32(src[pick - lane]) : -INFINITY;
+        const float pull = pick >= 0 ? static_cast<float>(shared_counts[pick]) * unit : 0.0f;
+        chosen += step * a.chosen_stride;
+        gate_grad += step * a.gate_grad_stride;
+        next_pick = chooses && t + step < a.rows ? *chosen : -1;
+        next_up = chooses && t + step < a.rows ? *gate_grad : 0.0f;
+        r.normalise();
         const float p = pick >= 0 ? r.exponential(z) * r.inverse : 0.0f;
-        float dot = 0.0f;
+        float2 dots = both(0.0f);
 #pragma unroll
-        for (int i = 0; i < kPlaces; ++i) {
-            r.e[i] *= r.inverse;
-            dot = __fmaf_rn(r.e[i], h[i], dot);
+        for (int i = 0; i < kPlaces / 2; ++i) {
+            r.e[i] = mul2(r.e[i], both(r.inverse));
+            dots = fma2(r.e[i], h[i], dots);
         }
+        float dot = group_sum<kGroup>(dots.x + dots.y);
         float direct = up;
         if (a.gate_grad != nullptr) {
             const float weighted = group_sum<kGroup>(p * up);
@@ -343,20 +407,20 @@ __global__ void __launch_bounds__(kThreads, kCtas<kPlaces>) router_backward_kern
                 const float total = group_sum<kGroup>(p);
                 const float scale = total > 0.0f ? reciprocal_approx(total) : 0.0f;
                 direct = (up - weighted * scale) * scale;
-                dot = group_sum<kGroup>(dot);
             } else {
-                dot = group_sum<kGroup>(dot) + weighted;
+                dot += weighted;
             }
-        } else {
-            dot = group_sum<kGroup>(dot);
         }
-        T* const dst = static_cast<T*>(a.logit_grad) + t * a.logit_grad_stride;
-        const int mine = t < a.rows ? a.experts - lane : 0;
 #pragma unroll
-        for (int i = 0; i < kPlaces; ++i)
-            if (kGroup * i < mine) dst[lane + kGroup * i] = from_f32<T>(r.e[i] * (h[i] - dot));
+        for (int i = 0; i < kPlaces / 2; ++i) {
+            const float2 g = mul2(r.e[i], add2(h[i], both(-dot)));
+            if (2 * i < kPlaces - 2 ? mine > 0 : 2 * i < mine) dst[kGroup * 2 * i] = from_f32<T>(g.x);
+            if (2 * i < kPlaces - 2 ? mine > 0 : 2 * i + 1 < mine) dst[kGroup * (2 * i + 1)] = from_f32<T>(g.y);
+        }
         __syncwarp();  // the chosen ones are written again, after the lane that had them
-        if (pick >= 0) dst[pick] = from_f32<T>(p * (pull + direct - dot));
+        if (pick >= 0) dst[pick - lane] = from_f32<T>(p * (pull + direct - dot));
+        src += step * a.logit_stride;
+        dst += step * a.logit_grad_stride;
     }
 }
 
@@ -370,16 +434,20 @@ int validate_counts(const RouterArgs& a) {
 }
 
 // The lanes of a row: few enough that a lane has several experts and the trees
-// over lanes stay short, and one for every choice.
+// over lanes stay short, and one for every choice; and the places of a lane, two
+// more at most than the experts need.
+template <int kGroup, int kPlaces, typename F>
+int with_places(const RouterArgs& a, F&& f) {
+    if constexpr (kPlaces > 2)
+        if (a.experts <= kGroup * (kPlaces - 2)) return with_places<kGroup, kPlaces - 2>(a, f);
+    return f(std::integral_constant<int, kGroup>{}, std::integral_constant<int, kPlaces>{});
+}
 template <typename F>
 int with_shape(const RouterArgs& a, F&& f) {
-    if (a.experts <= 16 && a.top_k <= 4) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
-    if (a.experts <= 32 && a.top_k <= 4) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 8>{});
-    if (a.experts <= 64) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 8>{});
-    if (a.experts <= 96) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 12>{});
-    if (a.experts <= 128) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 16>{});
-    if (a.experts <= 256) return f(std::integral_constant<int, 16>{}, std::integral_constant<int, 16>{});
-    return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 16>{});
+    if (a.experts <= 32 && a.top_k <= 4) return with_places<4, 8>(a, f);
+    if (a.experts <= 128) return with_places<8, 16>(a, f);
+    if (a.experts <= 256) return with_places<16, 16>(a, f);
+    return with_places<32, 16>(a, f);
 }
 
 // CTAs for the rows; up to two rounds of rows are left to one CTA, which then
