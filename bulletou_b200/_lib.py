@@ -16,6 +16,7 @@ P = ctypes.c_void_p
 Z = ctypes.c_size_t
 I = ctypes.c_int
 F = ctypes.c_float
+D = ctypes.c_double
 U64 = ctypes.c_uint64
 
 PACKAGE_DIR = Path(__file__).resolve().parent
@@ -200,7 +201,7 @@ SIGNATURES: dict[str, list] = {
     "bulletou_b200_hcpe_to_psv_device": [P, P, Z, P, P, P],
     "bulletou_b200_embedding_forward_device": [P, P, P, F, P],
     "bulletou_b200_embedding_backward_device": [P, P, P, F, P],
-    "bulletou_b200_dropout_device": [P, P, P, F, U64, U64, P],
+    "bulletou_b200_dropout_device": [P, P, P, D, U64, U64, P],
     "bulletou_b200_router_forward_device": [P, P, F, I, P, P, P, P, P],
     "bulletou_b200_router_backward_device": [P, P, P, P, P, P, F, I, P],
     "bulletou_b200_int8_quantize_rows_device": [P, P, P, P],

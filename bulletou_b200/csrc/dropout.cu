@@ -279,7 +279,7 @@ using namespace bou;
 extern "C" {
 
 int bulletou_b200_dropout_device(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix* x,
-                                 const BulletOuB200Matrix* residual, float probability, unsigned long long seed,
+                                 const BulletOuB200Matrix* residual, double probability, unsigned long long seed,
                                  unsigned long long offset, const BulletOuB200Matrix* out) {
     if (set_device(ctx) != 0 || validate_matrix(x, kTypeFloat, "dropout x") != 0) return -1;
     const unsigned type = 1u << x->type;
@@ -288,8 +288,8 @@ int bulletou_b200_dropout_device(BulletOuCudaCppContext* ctx, const BulletOuB200
         validate_disjoint(out, "dropout out", x, "x", true) != 0 ||
         validate_disjoint(out, "dropout out", residual, "residual", true) != 0)
         return -1;
-    if (!(probability >= 0.0f && probability <= 1.0f))
-        return fail_messagef("dropout probability must be in [0, 1], got %g", static_cast<double>(probability));
+    if (!(probability >= 0.0 && probability <= 1.0))
+        return fail_messagef("dropout probability must be in [0, 1], got %g", probability);
     DropoutArgs a{};
     a.n = x->rows * x->cols;
     if (a.n == 0) return ok();
@@ -301,7 +301,7 @@ int bulletou_b200_dropout_device(BulletOuCudaCppContext* ctx, const BulletOuB200
     a.residual_stride = residual != nullptr ? residual->row_stride : 0;
     a.out_stride = out->row_stride;
     a.keys = philox_keys(seed, offset);
-    a.threshold = static_cast<uint32_t>(std::floor(static_cast<double>(probability) * 65536.0 + 0.5));
+    a.threshold = static_cast<uint32_t>(std::floor(probability * 65536.0 + 0.5));
     a.factor = a.threshold < 65536u ? static_cast<float>(65536.0 / (65536.0 - a.threshold)) : 0.0f;
     // a vector where every eight is aligned: rows of whole eights, or no gaps between rows at all
     a.flat = is_flat(*x) && is_flat(*out) && (residual == nullptr || is_flat(*residual));

@@ -697,7 +697,7 @@ int gradient(BulletOuCudaCppContext* ctx, const Tokens& t, GradientArgs a, bool 
     }
     a.chunk = p.chunk;
     a.chunks = p.chunks;
-    a.row_blocks = (a.vocab + kEmptyRows - 1) / kEmptyRows;
+    a.row_blocks = static_cast<int>((static_cast<int64_t>(a.vocab) + kEmptyRows - 1) / kEmptyRows);
     return vector ? launch_gradient_unit<In, Out, kVectorUnit<In, Out>>(ctx, a, p) : launch_gradient_unit<In, Out, 1>(ctx, a, p);
 }
 

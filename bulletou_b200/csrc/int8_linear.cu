@@ -3,7 +3,7 @@
 //
 //   s_m = max_k |x_mk| * (1/127),   q_mk = rint(x_mk * (127 * (1 / max_k |x_mk|)))
 //   y_mn = (sum_k q_mk w_nk) * (s_m * w_scale_n) + bias_n
-// The sum is exact in 32-bit integers for K <= 131072 (127^2 K < 2^31), so it
+// The sum is exact in 32-bit integers for K <= 131071 (128^2 K < 2^31), so it
 // may be cut and joined in any order.
 #include <algorithm>
 #include <cmath>

@@ -593,13 +593,14 @@ typedef struct BulletOuB200Matrix {
 
 /* out[n][:] = scale * table[token n][:], tokens in row-major order.  A token
  * outside the table (-1: padding) gives a row of zeros.  table and out: f32 or
- * bf16 each; tokens: i32 with rows * cols = out's rows. */
+ * bf16 each; tokens: i32 with rows * cols = out's rows, below 2^31 - 2048. */
 int bulletou_b200_embedding_forward_device(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix* table,
     const BulletOuB200Matrix* tokens, float scale, const BulletOuB200Matrix* out);
 
 /* table_gradients[v][:] = scale * sum of out_gradients[n][:] over the tokens n
  * that name row v, in an order that the tokens alone fix; rows that none names
- * are zeroed.  f32 or bf16 each; the sums are f32. */
+ * are zeroed, and the gradient of a padded token is not read.  f32 or bf16 each;
+ * the sums are f32. */
 int bulletou_b200_embedding_backward_device(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix* tokens,
     const BulletOuB200Matrix* out_gradients, float scale, const BulletOuB200Matrix* table_gradients);
 
@@ -611,7 +612,7 @@ int bulletou_b200_embedding_backward_device(BulletOuCudaCppContext* ctx, const B
  * same call on the gradient of out.  A dropped element is 0 whatever x holds
  * there.  out may be x or residual itself. */
 int bulletou_b200_dropout_device(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix* x,
-    const BulletOuB200Matrix* residual, float probability, unsigned long long seed, unsigned long long offset,
+    const BulletOuB200Matrix* residual, double probability, unsigned long long seed, unsigned long long offset,
     const BulletOuB200Matrix* out);
 
 #define BULLETOU_B200_ROUTER_MAX_EXPERTS 512
@@ -640,8 +641,9 @@ int bulletou_b200_router_backward_device(BulletOuCudaCppContext* ctx, const Bull
     const BulletOuB200Matrix* loss_gradient, float balance, int normalize_gates,
     const BulletOuB200Matrix* logit_gradients);
 
-/* Inner size at which a sum of 8-bit products could leave 32 bits. */
-#define BULLETOU_B200_INT8_MAX_INNER 131072
+/* The largest inner size at which every sum of 8-bit products fits 32 bits:
+ * 131071 * 128 * 128 < 2^31. */
+#define BULLETOU_B200_INT8_MAX_INNER 131071
 
 /* Row by row: m = max |x|, q = round-to-even(x * (127 * (1 / m))), scales =
  * m * (1 / 127), each operation rounded to f32.  A row with m < 2^-100 gives

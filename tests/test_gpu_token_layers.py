@@ -145,6 +145,21 @@ def test_lookup_gradient_against_differences(tctx):
             assert abs(host(got)[v, c] - diff) <= 40 * U32 * np.abs(up).sum()
 
 
+def test_lookup_gradient_of_padded_tokens_is_not_read(tctx):
+    """NaN and infinities in the gradients of tokens outside the table reach no row."""
+    rng = np.random.default_rng(9)
+    for n in (40, 5000):
+        tokens = rng.integers(0, 30, n).astype(np.int32)
+        outside = rng.random(n) < 0.3
+        tokens[outside] = rng.choice([-1, 30, 2**31 - 1, -2**31], outside.sum())
+        grad = rng.standard_normal((n, 24)).astype(np.float32)
+        grad[outside] = np.where(rng.random((outside.sum(), 24)) < 0.5, np.nan, np.inf)
+        got = device(np.full((30, 24), 5.0))
+        bo.embedding_backward(tctx, device(tokens), device(grad), got)
+        want, mag, terms = embedding_grad(tokens, grad, 30, 1.0)
+        assert (np.abs(host(got) - want) <= (terms[:, None] + 2) * U32 * mag).all()
+
+
 @pytest.mark.parametrize("n", [1, 31, 4097, 100003])
 def test_lookup_gradient_of_one_token(tctx, n):
     """Every entry in one row: the longest sum, far from the other rows' sizes."""
@@ -420,17 +435,19 @@ def test_int8(tctx, rows, inner, outer, t_in, t_out, bias, pad, shift):
 
 @pytest.mark.parametrize("rows", [1, 40, 300])
 def test_int8_extreme_sums_are_exact(tctx, rows):
-    """The largest products of the longest rows: sums near 2^31 that f32 could not hold."""
-    inner = 131072
-    q = device(np.full((rows, inner), 127, np.int8))
-    w = np.full((3, inner), 127, np.int8)
-    w[1] = -127
-    w[2, ::2] = -127
-    w[2, 0] = 126
-    out = device(np.zeros((rows, 3)))
-    bo.int8_matmul(tctx, q, device(np.ones(rows)), device(w), device(np.ones(3)), out)
-    acc = np.array([127 * 127 * inner, -127 * 127 * inner, 127 * 253], np.int64)
-    assert np.array_equal(host(out), np.broadcast_to(acc.astype(np.float32).astype(np.float64), (rows, 3)))
+    """The largest products of the longest rows: sums up to 2^31 that f32 could not hold on the way."""
+    inner = 131071
+    q = np.full((rows, inner), -128, np.int8)
+    w = np.full((4, inner), -128, np.int8)
+    w[1] = 127
+    w[2, ::2] = 127
+    w[3] = 0
+    w[3, 5] = 1
+    out = device(np.zeros((rows, 4)))
+    bo.int8_matmul(tctx, device(q), device(np.ones(rows)), device(w), device(np.ones(4)), out)
+    acc = q[:1].astype(np.int64) @ w.astype(np.int64).T
+    assert acc.max() == 2**31 - 16384
+    assert np.array_equal(host(out), np.broadcast_to(acc.astype(np.float32).astype(np.float64), (rows, 4)))
 
 
 def test_int8_rows_of_zeros_infinities_and_nan(tctx):
@@ -547,7 +564,7 @@ def test_refusals(tctx):
         ("router counts", lambda: bo.router_forward(tctx, f(4, 3), i32(4, 1), f(4, 1), i32(3), f(3), f(1), balance=1.0)),
         ("router loss", lambda: bo.router_forward(tctx, f(4, 3), i32(4, 1), f(4, 1), i32(4), f(3), f(2), balance=1.0)),
         ("logit gradients", lambda: bo.router_backward(tctx, f(4, 8), i32(4, 1), i32(9), None, None, bf, balance=1.0)),
-        ("at most", lambda: bo.int8_matmul(tctx, i8(1, 131073), f(1), i8(1, 131073), f(1), f(1, 1))),
+        ("at most", lambda: bo.int8_matmul(tctx, i8(1, 131072), f(1), i8(1, 131072), f(1), f(1, 1))),
         ("expected", lambda: bo.int8_linear(tctx, f(4, 8), i8(3, 9), f(3), f(4, 3))),
         ("expected", lambda: bo.int8_linear(tctx, f(4, 8), i8(3, 8), f(4), f(4, 3))),
         ("expected", lambda: bo.int8_linear(tctx, f(4, 8), i8(3, 8), f(3), f(4, 4))),
