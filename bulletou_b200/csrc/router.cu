@@ -181,18 +181,24 @@ __device__ __forceinline__ int places_of(int experts, int lane) {
     return (experts - lane + kGroup - 1) / kGroup;
 }
 
+// The choices of all experts, by the CTA's first warp.
+__device__ __forceinline__ void sum_choices(const int* counts, int experts, int64_t* choices) {
+    if (threadIdx.x >= 32) return;
+    int64_t c = 0;
+    for (int e = threadIdx.x; e < experts; e += 32) c += counts[e];
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) c += __shfl_xor_sync(0xffffffffu, c, d);
+    if (threadIdx.x == 0) *choices = c;
+}
+
 // Means and loss from the sums of the probabilities and the counts; every
 // thread of the CTA comes here.
 __device__ void finish(const RouterArgs& a, const float* p_sums, const int* counts) {
-    __shared__ unsigned long long choices;
+    __shared__ int64_t choices;
     __shared__ float warp_terms[32];
-    if (threadIdx.x == 0) choices = 0;
+    sum_choices(counts, a.experts, &choices);
     __syncthreads();
-    unsigned long long c = 0;
-    for (int e = threadIdx.x; e < a.experts; e += blockDim.x) c += counts[e];
-    if (c != 0) atomicAdd(&choices, c);
-    __syncthreads();
-    const float rows = static_cast<float>(max(counts[a.experts], 1)), all = static_cast<float>(max(choices, 1ull));
+    const float rows = static_cast<float>(max(counts[a.experts], 1)), all = static_cast<float>(max(choices, static_cast<int64_t>(1)));
     float s = 0.0f;
     for (int e = threadIdx.x; e < a.experts; e += blockDim.x) {
         const float mean = p_sums[e] / rows;
@@ -347,22 +353,17 @@ __global__ void __launch_bounds__(kJoinThreads) router_join_kernel(const RouterA
 
 template <typename T, int kGroup, int kPlaces>
 __global__ void __launch_bounds__(kThreads, kCtas<kPlaces>) router_backward_kernel(const RouterArgs a) {
-    __shared__ unsigned long long choices;
+    __shared__ int64_t choices;
     __shared__ int shared_counts[kGroup * kPlaces];
     const int lane = threadIdx.x & (kGroup - 1);
-    if (threadIdx.x == 0) choices = 0;
+    for (int e = threadIdx.x; e < kGroup * kPlaces; e += kThreads) shared_counts[e] = e < a.experts ? a.counts[e] : 0;
     __syncthreads();
-    unsigned long long c = 0;
-    for (int e = threadIdx.x; e < kGroup * kPlaces; e += kThreads) {
-        shared_counts[e] = e < a.experts ? a.counts[e] : 0;
-        c += shared_counts[e];
-    }
-    if (c != 0) atomicAdd(&choices, c);
+    sum_choices(shared_counts, a.experts, &choices);
     __syncthreads();
     // the balance loss's pull on every probability of an expert
     float2 h[kPlaces / 2];
     const float unit = (a.loss_grad != nullptr ? a.loss_grad[0] : 0.0f) * a.balance * static_cast<float>(a.experts) /
-                       static_cast<float>(max(a.counts[a.experts], 1)) / static_cast<float>(max(choices, 1ull));
+                       static_cast<float>(max(a.counts[a.experts], 1)) / static_cast<float>(max(choices, static_cast<int64_t>(1)));
     auto pull_of = [&](int e) { return static_cast<float>(shared_counts[e]) * unit; };
 #pragma unroll
     for (int i = 0; i < kPlaces / 2; ++i) h[i] = make_float2(pull_of(lane + kGroup * 2 * i), pull_of(lane + kGroup * (2 * i + 1)));
