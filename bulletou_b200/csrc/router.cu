@@ -24,9 +24,9 @@ namespace {
 constexpr int kThreads = 256;
 // By the places of a lane: CTAs on an SM of the backward pass, and threads of the
 // forward pass's one CTA on an SM (each CTA leaves sums to be joined): 64
-// registers for each thread, 80 for 16 places.
+// registers for each thread, 80 for 16 places, up to 128 beyond.
 template <int kPlaces>
-constexpr int kCtas = kPlaces > 12 ? 3 : 4;
+constexpr int kCtas = kPlaces > 16 ? 2 : kPlaces > 12 ? 3 : 4;
 template <int kGroup, int kPlaces>  // (the sums of 512 experts for each warp fill the shared memory)
 constexpr int kForwardThreads = kThreads * (kGroup * kPlaces > 256 ? 2 : kCtas<kPlaces>);
 constexpr int kMaxExperts = BULLETOU_B200_ROUTER_MAX_EXPERTS;
@@ -434,9 +434,12 @@ int validate_counts(const RouterArgs& a) {
     return 0;
 }
 
-// The lanes of a row: few enough that a lane has several experts and the trees
-// over lanes stay short, and one for every choice; and the places of a lane, two
-// more at most than the experts need.
+// The lanes of a row, at least one for every choice, and the places of a lane, at
+// most two more than the experts need.  Forward, few lanes: the trees over lanes
+// are short and the rest is a lane's own work (262144 x 81, top 2: 4 lanes 27 us,
+// 8 lanes 32 us).  Backward, every place is a store, whose sectors the lanes of a
+// row should fill (4 lanes 45 us, 8 lanes 36 us, 16 lanes 44 us; at 128 experts 8
+// lanes 13.5 us, 16 lanes 12.3 us for 65536 rows).
 template <int kGroup, int kPlaces, typename F>
 int with_places(const RouterArgs& a, F&& f) {
     if constexpr (kPlaces > 2)
@@ -444,10 +447,17 @@ int with_places(const RouterArgs& a, F&& f) {
     return f(std::integral_constant<int, kGroup>{}, std::integral_constant<int, kPlaces>{});
 }
 template <typename F>
-int with_shape(const RouterArgs& a, F&& f) {
-    if (a.experts <= 32 && a.top_k <= 4) return with_places<4, 8>(a, f);
+int with_forward_shape(const RouterArgs& a, F&& f) {
+    if (a.experts <= 96 && a.top_k <= 4) return with_places<4, 24>(a, f);
     if (a.experts <= 128) return with_places<8, 16>(a, f);
     if (a.experts <= 256) return with_places<16, 16>(a, f);
+    return with_places<32, 16>(a, f);
+}
+template <typename F>
+int with_backward_shape(const RouterArgs& a, F&& f) {
+    if (a.experts <= 16 && a.top_k <= 4) return with_places<4, 4>(a, f);
+    if (a.experts <= 96) return with_places<8, 12>(a, f);
+    if (a.experts <= 128) return with_places<16, 8>(a, f);
     return with_places<32, 16>(a, f);
 }
 
@@ -460,7 +470,7 @@ int router_grid(const BulletOuCudaCppContext* ctx, int rows, int per) {
 
 template <typename T>
 int forward(BulletOuCudaCppContext* ctx, RouterArgs a) {
-    return with_shape(a, [&](auto group, auto places) {
+    return with_forward_shape(a, [&](auto group, auto places) {
         const int grid = router_grid(ctx, a.rows, kForwardThreads<group(), places()> / group());
         if (grid > 1) {
             void* p = nullptr;
@@ -481,7 +491,7 @@ int forward(BulletOuCudaCppContext* ctx, RouterArgs a) {
 
 template <typename T>
 int backward(BulletOuCudaCppContext* ctx, const RouterArgs& a) {
-    return with_shape(a, [&](auto group, auto places) {
+    return with_backward_shape(a, [&](auto group, auto places) {
         const int64_t ctas = (static_cast<int64_t>(a.rows) * group + kThreads - 1) / kThreads;
         const LaunchShape shape{dim3(static_cast<unsigned>(std::min<int64_t>(ctas, static_cast<int64_t>(ctx->sm_count) * kCtas<places()>))), kThreads};
         return launch_kernel(ctx, "router backward launch", router_backward_kernel<T, group(), places()>, shape, a);
