@@ -101,6 +101,10 @@ struct LookupArgs {
 // (at most a row for each lane): each lane fetches one row's token, and the
 // rows' units are then loaded kRows at a time, all in flight together.  The
 // stores stream past L2, which keeps the table.
+//
+// Bound by the stores: 655360 rows of 256 bf16 take 71 us, 5.3 TB/s of which
+// 4.7 are written (torch's fill of that output alone takes 89 us).  With rows
+// held as f32, 70 registers and 24 warps on an SM it took 109 us.
 template <typename In, typename Out, int kUnit>
 __global__ void __launch_bounds__(kThreads, kLookupCtas) lookup_kernel(const LookupArgs a, int group, int span) {
     constexpr int kRows = 4;
@@ -144,7 +148,9 @@ __global__ void __launch_bounds__(kThreads, kLookupCtas) lookup_kernel(const Loo
 // Least-significant-digit radix sort of (token, position), tokens outside the
 // table as the largest key.  Digits of up to 11 bits: fewer passes save three
 // launches each, which is what a sort of 10^5 tokens costs, and 2048 counters
-// for each of 8 warps still fit the shared memory twice.
+// for each of 8 warps still fit the shared memory twice.  1310720 tokens of a
+// 17-bit table (two passes) take about 45 us, 68438 of an 11-bit one about 15:
+// launches, and scattered 8-byte stores.
 constexpr int kMaxDigitBits = 11;
 constexpr int kMaxBins = 1 << kMaxDigitBits;
 constexpr int kMaxTile = 2048;
@@ -311,6 +317,11 @@ __global__ void __launch_bounds__(kThreads, kBinsOfThread <= 2 ? 5 : 2) sort_sca
 // sums its chunk's runs of equal tokens in order.  A run inside the chunk is a
 // row's gradient and is written; a run that goes on beyond the chunk leaves a
 // partial row, and joined_rows_kernel adds those up in the order of the chunks.
+//
+// Bound by reading the gradients once: 1310720 rows of 256 f32 take 225 us, 6.3
+// TB/s (97 % of a copy), with 4 rows in flight for each of 24 warps on an SM; 8
+// rows in flight needed 142 registers, left 8 warps and took 309 us.  Rows of an
+// odd width go one element at a time: 68438 of 257 f32 in 21 us, 3.4 TB/s.
 struct GradientArgs {
     const int2* entries;   // (token, position), sorted by token
     int n, chunk, chunks;
@@ -449,7 +460,9 @@ __global__ void __launch_bounds__(kThreads, 3) gradient_kernel(const GradientArg
 // it.  Runs over up to kShortRun more chunks take a warp each; longer ones are
 // shared by the CTA's warps, each a run of consecutive chunks, and joined in
 // that order.  A lane takes eight columns at a time, two 16-byte loads of every
-// partial row.
+// partial row.  Bound by latency: the run's end is searched 32 chunks at a time
+// (a binary search of 20 steps made it 37 us for 10240 chunks of 256 columns, of
+// which the longest run covers 245; now 15).
 template <typename Out, bool kVector>
 __global__ void __launch_bounds__(kThreads, 4) joined_rows_kernel(const GradientArgs a) {
     constexpr int kShortRun = 8, kQuads = 2, kBlock = 128 * kQuads;

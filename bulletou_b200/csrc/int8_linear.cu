@@ -143,6 +143,9 @@ struct Group {
 // kRowThreads threads for each row, which hold its values in registers between
 // the maximum and the rounding: x is read once.  Rows longer than 2 * kGroup *
 // kRowThreads (only with kRowThreads == kThreads) read the rest again, from L2.
+// 16384 x 4096 bf16: 38 us, 5.2 TB/s, bound by memory and the conversions together
+// (54 % of the issue slots); with the values held as f32, 92 registers and 16
+// warps on an SM it took 67 us.
 template <typename T, int kRowThreads>
 __global__ void __launch_bounds__(kThreads, 4) quantize_kernel(const QuantizeArgs a) {
     constexpr int kHeld = 2, kRowWarps = kRowThreads / 32;
@@ -201,7 +204,9 @@ __global__ void __launch_bounds__(kThreads, 4) quantize_kernel(const QuantizeArg
 // output channels one after the other, 16 bytes of a channel for each lane at
 // a time, against the rows' 8-bit values in shared memory.  Each CTA quantises
 // the rows itself (they are a few KB from L2), so the layer is one launch, and
-// the first channel's weights are on their way meanwhile.
+// the first channel's weights are on their way meanwhile.  One row of 1536 x 2048
+// takes 3.8 us, which is the launch and one chain of latencies; two rows of 4096
+// x 4096 8.2 us against 9.2 on the tensor cores, four were 16 against 9.
 constexpr int kFewRows = 2;
 constexpr size_t kFewRowsBytes = 48 * 1024;  // shared memory for the rows
 

@@ -11,10 +11,16 @@
 // two single CTAs would load for the same products, and what L2 can deliver
 // per SM is the limit of a 128 x 256 tile.  Persistent; the 512 TMEM columns
 // hold two accumulators, so a tile's epilogue runs under the next tile's MMAs.
+// 16384 x 4096 x 4096: 165 us, 3.3 POP/s, the tensor pipe busy in 94 % of the
+// cycles at the clock that the power limit leaves.
 //
 // int8_tile_kernel, where there are too few 256 x 256 tiles for the SMs: one
-// 128 x TN tile for each CTA, with k cut over a cluster of up to four CTAs; the
-// partial integer sums meet through distributed shared memory.
+// 128 x 64 tile for each CTA, with k cut over a cluster of up to four CTAs where
+// that is long; the partial integer sums meet through distributed shared memory.
+// Bound by latency: 8 x 1536 x 2048 takes 5.8 us, of which 0.2 us for each 128 of
+// k (an MMA takes 64 cycles to issue whatever its N, and a wait between) and 3.4
+// us for the launch, the first load and the epilogue.  Meeting in a cluster costs
+// about 2 us, so k is cut from 16 blocks of 128 on.
 //
 // Every wait on an mbarrier is bounded (2 s); where one runs out the CTA's
 // remaining results are NaN.  No multicast loads.
@@ -28,6 +34,7 @@ namespace bou {
 namespace {
 
 constexpr int kTileM = 128;                 // rows of q for each CTA (MMA M of one CTA)
+constexpr int kTileN = 64;                  // rows of w for a tile of one CTA
 constexpr int kTileK = 128;                 // bytes of k in a stage: one swizzle atom
 constexpr uint32_t kABytes = kTileM * kTileK;
 constexpr int kStagePad = 4;                // floats between staged rows: 16-byte accesses without bank conflicts
@@ -153,46 +160,47 @@ __device__ __forceinline__ void store_block(float* stage, const float* v, const 
 }
 
 // ------------------------------------------------------------------ one tile for each CTA
-// kDeep: the SM's shared memory for one CTA, which has 1 KB of k of its tile on
-// the way at once; otherwise 96 KB, for two CTAs.
-template <int TN, bool kDeep>
+// kDeep, where every CTA has an SM to itself: all of the shared memory, so that 1
+// KB of k of the tile is on the way at once (512 x 512 x 512: 5.9 us, 6.8 without);
+// otherwise 96 KB, for two CTAs.
+template <bool kDeep>
 struct TileShape {
-    static constexpr uint32_t kStageBytes = kABytes + TN * kTileK;
+    static constexpr uint32_t kStageBytes = kABytes + kTileN * kTileK;
     static constexpr int kStages = kDeep ? 192 * 1024 / kStageBytes : 96 * 1024 / kStageBytes;
     // after the last MMA the stages hold the partial sums and the staged rows
-    static constexpr uint32_t kStagingAt = TN * kTileM * 4;
+    static constexpr uint32_t kStagingAt = kTileN * kTileM * 4;
     static constexpr int kThreads = 128;
-    static constexpr uint32_t kSmem = kStages * kStageBytes + 2 * TN * 4 + 256 + 1024;
+    static constexpr uint32_t kSmem = kStages * kStageBytes + 2 * kTileN * 4 + 256 + 1024;
     static_assert(kStagingAt + 4 * 32 * (32 + kStagePad) * 4 <= kStages * kStageBytes);
 };
 
 // `splits` CTAs of a cluster share a tile and cut k; the grid is their tiles,
 // the columns' tiles first.
-template <int TN, bool kDeep, typename Out>
+template <bool kDeep, typename Out>
 __global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ CUtensorMap map_q,
                                                         const __grid_constant__ CUtensorMap map_w, const ProductArgs a,
                                                         int splits, int box_rows, bool vector_ok, bool weights_ready) {
-    using S = TileShape<TN, kDeep>;
+    using S = TileShape<kDeep>;
     extern __shared__ uint8_t raw[];
     const uint32_t raw_addr = smem_u32(raw);
     const uint32_t base = (raw_addr + 1023u) & ~1023u;  // swizzle atoms
     uint8_t* const stages = raw + (base - raw_addr);
     float* const staging = reinterpret_cast<float*>(stages + S::kStagingAt);
     float* const col_scale = reinterpret_cast<float*>(stages + S::kStages * S::kStageBytes);
-    float* const col_bias = col_scale + TN;
-    uint64_t* const bars = reinterpret_cast<uint64_t*>(col_bias + TN);  // full, empty, done
+    float* const col_bias = col_scale + kTileN;
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(col_bias + kTileN);  // full, empty, done
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S::kStages + 1);
     const uint32_t full = smem_u32(bars), empty = full + 8 * S::kStages, done = empty + 8 * S::kStages;
     const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
 
     const int rank = splits > 1 ? static_cast<int>(cluster_rank()) : 0;
     const int tile = blockIdx.x / splits;
-    const int tiles_n = (a.n + TN - 1) / TN;
-    const int row0 = tile / tiles_n * kTileM, col0 = tile % tiles_n * TN;
+    const int tiles_n = (a.n + kTileN - 1) / kTileN;
+    const int row0 = tile / tiles_n * kTileM, col0 = tile % tiles_n * kTileN;
     const int blocks = (a.k + kTileK - 1) / kTileK;
     const int share = (blocks + splits - 1) / splits;
     const int k0 = min(blocks, rank * share), count = min(blocks, k0 + share) - k0;
-    const uint32_t stage_bytes = box_rows * kTileK + TN * kTileK;  // what a stage's loads bring
+    const uint32_t stage_bytes = box_rows * kTileK + kTileN * kTileK;  // what a stage's loads bring
 
     if (tid == 0) {
         for (int s = 0; s < S::kStages; ++s) {
@@ -204,7 +212,7 @@ __global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ 
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                     "r"(static_cast<uint32_t>(TN))
+                     "r"(static_cast<uint32_t>(kTileN))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -243,14 +251,14 @@ __global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ 
                 const uint64_t wd = k_major_desc(base + s * S::kStageBytes + kABytes);
 #pragma unroll
                 for (int j = 0; j < kTileK / 32; ++j)  // (a descriptor counts in 16 bytes)
-                    mma_i8<1>(tmem, qd + 2 * j, wd + 2 * j, int8_idesc(kTileM, TN), (i | j) != 0 ? 1u : 0u);
+                    mma_i8<1>(tmem, qd + 2 * j, wd + 2 * j, int8_idesc(kTileM, kTileN), (i | j) != 0 ? 1u : 0u);
                 if (i + S::kStages < count) commit_one(empty + 8 * s);  // the stage is loaded again
                 if (i + 1 == count) commit_one(done);
             }
             __syncwarp();
         }
     } else {
-        for (int c = lane; c < TN; c += 32) {
+        for (int c = lane; c < kTileN; c += 32) {
             const bool in = col0 + c < a.n;
             col_scale[c] = in ? a.w_scales[col0 + c] : 0.0f;
             col_bias[c] = in && a.bias != nullptr ? a.bias[col0 + c] : 0.0f;
@@ -268,7 +276,7 @@ __global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ 
     if (splits == 1) {
         const float row_scale = good ? own_scale : NAN;
 #pragma unroll 1
-        for (int c0 = 0; c0 < TN && col0 + c0 < a.n; c0 += 32) {
+        for (int c0 = 0; c0 < kTileN && col0 + c0 < a.n; c0 += 32) {
             uint32_t sum[32];
             float v[32];
             tmem_ld32(lanes + c0, sum);
@@ -282,7 +290,7 @@ __global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ 
         // partial sums as [column][row], over the stages that are no longer needed
         int* const part = reinterpret_cast<int*>(stages);
 #pragma unroll 1
-        for (int c0 = 0; c0 < TN; c0 += 32) {
+        for (int c0 = 0; c0 < kTileN; c0 += 32) {
             uint32_t sum[32];
             tmem_ld32(lanes + c0, sum);
 #pragma unroll
@@ -293,9 +301,9 @@ __global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ 
         __syncthreads();
         if (!good) *failed = 1;
         cluster_sync();
-        // the tile's 4 row groups x TN / 32 column groups, dealt out over the cluster's warps
+        // the tile's 4 row groups x kTileN / 32 column groups, dealt out over the cluster's warps
         const uint32_t mine = smem_u32(part), flag = smem_u32(failed);
-        for (int job = rank * 4 + warp; job < 4 * (TN / 32); job += 4 * splits) {
+        for (int job = rank * 4 + warp; job < 4 * (kTileN / 32); job += 4 * splits) {
             const int group = job & 3, c0 = (job >> 2) * 32;
             const int row = row0 + group * 32 + lane;
             if (row0 + group * 32 >= a.m || col0 + c0 >= a.n) continue;
@@ -320,7 +328,7 @@ __global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ 
         for (int s = 0; s < min(count, S::kStages); ++s) mbar_wait(full + 8 * s, ((count - 1 - s) / S::kStages) & 1);
     __syncthreads();
     if (warp == 1)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(static_cast<uint32_t>(TN))
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(static_cast<uint32_t>(kTileN))
                      : "memory");
 }
 
@@ -491,28 +499,28 @@ int operand_map(CUtensorMap* map, const int8_t* data, int rows, int k, size_t st
     return 0;
 }
 
-template <int TN, bool kDeep, typename Out>
+template <bool kDeep, typename Out>
 int launch_tiles(BulletOuCudaCppContext* ctx, const ProductArgs& a, int64_t tiles, int splits, bool vector_ok, bool early, bool weights_ready) {
-    using S = TileShape<TN, kDeep>;
+    using S = TileShape<kDeep>;
     CUtensorMap q, w;
     // few rows are loaded as they are: the rest of the tile is what the stage
     // held before and reaches no result
     const int box_rows = std::min(kTileM, (a.m + 7) / 8 * 8);
-    if (operand_map(&q, a.q, a.m, a.k, a.q_stride, box_rows) != 0 || operand_map(&w, a.w, a.n, a.k, a.w_stride, TN) != 0)
+    if (operand_map(&q, a.q, a.m, a.k, a.q_stride, box_rows) != 0 || operand_map(&w, a.w, a.n, a.k, a.w_stride, kTileN) != 0)
         return -1;
     const LaunchShape shape{dim3(static_cast<unsigned>(tiles * splits)), S::kThreads, S::kSmem, splits, early};
-    return launch_kernel(ctx, "int8 product launch", int8_tile_kernel<TN, kDeep, Out>, shape, q, w, a, splits, box_rows, vector_ok, weights_ready);
+    return launch_kernel(ctx, "int8 product launch", int8_tile_kernel<kDeep, Out>, shape, q, w, a, splits, box_rows, vector_ok, weights_ready);
 }
 
-template <int TN, typename Out>
+template <typename Out>
 int launch_tiles(BulletOuCudaCppContext* ctx, const ProductArgs& a, bool vector_ok, bool early, bool weights_ready) {
-    const int64_t tiles = static_cast<int64_t>((a.m + kTileM - 1) / kTileM) * ((a.n + TN - 1) / TN);
+    const int64_t tiles = static_cast<int64_t>((a.m + kTileM - 1) / kTileM) * ((a.n + kTileN - 1) / kTileN);
     const int blocks = (a.k + kTileK - 1) / kTileK;
     int splits = 1;
     while (splits < 4 && tiles * splits * 2 <= ctx->sm_count && blocks >= 16 * splits) splits *= 2;
     if (tiles * splits > INT32_MAX) return fail_messagef("int8 product: %d x %d results are too many", a.m, a.n);
-    return tiles * splits <= ctx->sm_count ? launch_tiles<TN, true, Out>(ctx, a, tiles, splits, vector_ok, early, weights_ready)
-                                           : launch_tiles<TN, false, Out>(ctx, a, tiles, splits, vector_ok, early, weights_ready);
+    return tiles * splits <= ctx->sm_count ? launch_tiles<true, Out>(ctx, a, tiles, splits, vector_ok, early, weights_ready)
+                                           : launch_tiles<false, Out>(ctx, a, tiles, splits, vector_ok, early, weights_ready);
 }
 
 template <typename Out>
@@ -527,12 +535,12 @@ int launch_pairs(BulletOuCudaCppContext* ctx, const ProductArgs& a, int tiles, b
 template <typename Out>
 int launch_typed(BulletOuCudaCppContext* ctx, const ProductArgs& a, bool early, bool weights_ready) {
     const bool vector_ok = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && (a.m <= 1 || a.out_stride * sizeof(Out) % 16 == 0);
+    // Pairs as soon as they fill 64 SMs: 512 x 4096 x 4096 (32 tiles) takes 18 us in
+    // pairs and 27 in single tiles, 256 x 4096 x 4096 (16) 16.5 and 11.8.
     const int64_t pairs = static_cast<int64_t>((a.m + 255) / 256) * ((a.n + 255) / 256);
     if (pairs >= 32 && pairs <= INT32_MAX)
         return launch_pairs<Out>(ctx, a, static_cast<int>(pairs), vector_ok, early);
-    const int64_t wide = static_cast<int64_t>((a.m + 127) / 128) * ((a.n + 127) / 128);
-    return wide >= ctx->sm_count ? launch_tiles<128, Out>(ctx, a, vector_ok, early, weights_ready)
-                                 : launch_tiles<64, Out>(ctx, a, vector_ok, early, weights_ready);
+    return launch_tiles<Out>(ctx, a, vector_ok, early, weights_ready);
 }
 
 }  // namespace

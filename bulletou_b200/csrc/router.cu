@@ -12,6 +12,11 @@
 // are trees over the lanes that share it; the sums over rows are added up per
 // lane, warp and CTA and joined in a fixed order, so no result depends on
 // timing.  Counts are integers.
+//
+// 262144 rows of 81 with their top 2: forward 27 us (bound by the comparisons of
+// the maximum and the choices, which run at half rate), backward 36 us (170 MB,
+// 4.7 TB/s).  A lane for each row, the rows in shared memory, took 38 and 57 us:
+// 20 warps fit an SM, and the shared memory's bandwidth bounds them.
 #include <algorithm>
 #include <type_traits>
 

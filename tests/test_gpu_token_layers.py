@@ -401,7 +401,7 @@ def test_router_gradient_skips_foreign_experts(tctx):
 INT8 = [  # rows, inner, outer
     (1, 1, 1), (1, 16, 8), (1, 1536, 2048), (2, 1000, 9), (3, 333, 77), (8, 128, 130), (9, 4096, 33), (16, 64, 257), (17, 100, 16),
     (64, 256, 128), (65, 257, 129), (128, 2560, 9), (129, 512, 300), (300, 1537, 1001), (513, 96, 520), (1025, 144, 257),
-    (2, 0, 5), (9, 0, 5), (0, 8, 5), (4, 8, 0), (5, 8192, 3), (33, 20001, 7), (2000, 96, 1300), (4700, 200, 1100), (300, 260, 20000),
+    (2, 0, 5), (9, 0, 5), (0, 8, 5), (4, 8, 0), (5, 8192, 3), (33, 20001, 7), (2000, 96, 1300), (4700, 200, 1100), (300, 260, 20000), (130, 200, 7000), (5, 5000, 70),
 ]
 
 
