@@ -83,6 +83,8 @@ __device__ __forceinline__ float reciprocal_approx(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// A gate's part of its row's; exactly one where it is the only one.
+__device__ __forceinline__ float share_of(float p, float total) { return p == total ? 1.0f : p * reciprocal_approx(total); }
 constexpr float kLog2E = 1.4426950408889634f;
 
 // Over the kGroup lanes that share a row.
@@ -274,7 +276,7 @@ __global__ void __launch_bounds__(kForwardThreads<kGroup, kPlaces>, 1) router_fo
         }
         if (lane < a.top_k && t < a.rows) {
             *chosen = pick;
-            *gates = a.normalize && pick >= 0 ? own * reciprocal_approx(total) : own;
+            *gates = a.normalize && pick >= 0 ? share_of(own, total) : own;
             if (pick >= 0) atomicAdd(count + pick, 1);
         }
         src += step * a.logit_stride;
@@ -405,16 +407,17 @@ __global__ void __launch_bounds__(kThreads, kCtas<kPlaces>) router_backward_kern
             dots = fma2(r.e[i], h[i], dots);
         }
         float dot = group_sum<kGroup>(dots.x + dots.y);
-        float direct = up;
+        float direct = 0.0f;  // what the choice's gate adds to its logit's gradient
         if (a.gate_grad != nullptr) {
-            const float weighted = group_sum<kGroup>(p * up);
             if (a.normalize) {
-                // p (u - sum g u) / sum p: gates that sum to one take no part in the mean
+                // g (u - sum g u): gates that sum to one take no part in the mean, and a
+                // single one adds nothing
                 const float total = group_sum<kGroup>(p);
-                const float scale = total > 0.0f ? reciprocal_approx(total) : 0.0f;
-                direct = (up - weighted * scale) * scale;
+                const float gate = total > 0.0f ? share_of(p, total) : 0.0f;
+                direct = gate * (up - group_sum<kGroup>(gate * up));
             } else {
-                dot += weighted;
+                direct = p * up;
+                dot += group_sum<kGroup>(direct);
             }
         }
 #pragma unroll
@@ -424,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<kPlaces>) router_backward_kern
             if (2 * i < kPlaces - 2 ? mine > 0 : 2 * i + 1 < mine) dst[kGroup * (2 * i + 1)] = from_f32<T>(g.y);
         }
         __syncwarp();  // the chosen ones are written again, after the lane that had them
-        if (pick >= 0) dst[pick - lane] = from_f32<T>(p * (pull + direct - dot));
+        if (pick >= 0) dst[pick - lane] = from_f32<T>(__fmaf_rn(p, pull - dot, direct));
         src += step * a.logit_stride;
         dst += step * a.logit_grad_stride;
     }

@@ -387,6 +387,21 @@ def test_router_gradient_in_place_and_without_parts(tctx):
     assert np.array_equal(host(z), parts[2])
 
 
+@pytest.mark.parametrize("experts", [2, 9, 81, 300])
+def test_router_single_normalised_gate_is_one_and_adds_nothing(tctx, experts):
+    """softmax over one choice: the gate is 1, and however large its gradient, the logits' is the balance loss's alone."""
+    rng = np.random.default_rng(experts)
+    z = device(rng.standard_normal((70, experts)))
+    out = run_router(tctx, z, 1, 0.1, True)
+    assert (host(out["gates"]) == 1).all()
+    got, alone = device(np.ones((70, experts))), device(np.ones((70, experts)))
+    bo.router_backward(tctx, z, out["experts"], out["counts"], device(np.full((70, 1), 1e6)), device([1.0]), got, balance=0.1,
+                       normalize_gates=True)
+    bo.router_backward(tctx, z, out["experts"], out["counts"], None, device([1.0]), alone, balance=0.1, normalize_gates=True)
+    # the chosen logit goes through its own product: one rounding of the difference apart
+    assert np.abs(host(got) - host(alone)).max() <= 4 * U32 * 0.1 * experts / 70
+
+
 def test_router_gradient_skips_foreign_experts(tctx):
     """Expert indexes outside the range (a caller's own padding) take no gradient and read nothing."""
     z = device(np.zeros((2, 4)))
