@@ -592,7 +592,7 @@ GradientPlan plan_gradient(const BulletOuCudaCppContext* ctx, int n, int vocab, 
     p.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
     p.digit_bits = (bits + p.passes - 1) / p.passes;
     // a CTA for every SM while there are tokens enough; one alone where it can hold them all
-    p.tile = n <= kMaxTile || n >= kMaxTile * ctx->sm_count ? kMaxTile : kMaxTile / 2;
+    p.tile = n <= kMaxTile || n > kMaxTile / 2 * ctx->sm_count ? kMaxTile : n > kMaxTile / 4 * ctx->sm_count ? kMaxTile / 2 : kMaxTile / 4;
     p.tiles = (n + p.tile - 1) / p.tile;
     p.row = (static_cast<size_t>(n) + 63) / 64 * 64;
     p.counts = ((static_cast<size_t>(1) << p.digit_bits) * p.tiles + 63) / 64 * 64;
@@ -605,11 +605,12 @@ GradientPlan plan_gradient(const BulletOuCudaCppContext* ctx, int n, int vocab, 
     const int most = p.unit == 1 ? 5 : 8 / p.unit;
     const int parts = (units + p.lanes * most - 1) / (p.lanes * most);
     p.units = (units + p.lanes * parts - 1) / (p.lanes * parts);
-    // Chunks long enough that the two partial rows of each cost little, short
-    // enough that every SM has the 24 warps that fit it.
+    // Chunks of up to 128 entries (each leaves up to two partial rows), as many as
+    // fill the 24 warps that fit an SM a whole number of times.
     const int64_t groups = static_cast<int64_t>(ctx->sm_count) * 24 * 32 / p.lanes;
-    p.chunk = 128;
-    while (p.chunk > 16 && static_cast<int64_t>(n / p.chunk) * parts < groups) p.chunk /= 2;
+    const int64_t work = static_cast<int64_t>(n) * parts;
+    const int64_t turns = (work + 128 * groups - 1) / (128 * groups);
+    p.chunk = std::max(16, static_cast<int>((work + turns * groups - 1) / std::max<int64_t>(1, turns * groups) + 3) / 4 * 4);
     p.chunks = (n + p.chunk - 1) / p.chunk;
     return p;
 }
@@ -644,20 +645,25 @@ int sort_tokens(BulletOuCudaCppContext* ctx, const Tokens& tokens, const Gradien
         out->entries = plan.passes % 2 == 1 ? s.out : s.other;
         return 0;
     }
-    const bool large = plan.tile == kMaxTile;
+    const int part = kMaxTile / plan.tile;  // the steps of a tile are those of the largest, or a half or a quarter of them
     for (int pass = 0; pass < plan.passes; ++pass) {
         s.shift = pass * plan.digit_bits;
         shape.chained = pass > 0;
         shape.smem = 0;
         shape.grid = dim3(plan.tiles);
-        if (launch_kernel(ctx, "embedding sort launch", large ? sort_count_kernel<kSteps> : sort_count_kernel<kSteps / 2>, shape, s) != 0)
+        if (launch_kernel(ctx, "embedding sort launch", part == 1   ? sort_count_kernel<kSteps>
+                          : part == 2 ? sort_count_kernel<kSteps / 2>
+                                      : sort_count_kernel<kSteps / 4>,
+                          shape, s) != 0)
             return -1;
         shape.chained = true;
         shape.grid = dim3(s.bins);
         if (launch_kernel(ctx, "embedding sort launch", sort_scan_kernel, shape, s) != 0) return -1;
         shape.grid = dim3(plan.tiles);
         shape.smem = places;
-        if ((large ? launch_scatter<kSteps, false>(ctx, shape, s, 1) : launch_scatter<kSteps / 2, false>(ctx, shape, s, 1)) != 0)
+        if ((part == 1   ? launch_scatter<kSteps, false>(ctx, shape, s, 1)
+             : part == 2 ? launch_scatter<kSteps / 2, false>(ctx, shape, s, 1)
+                         : launch_scatter<kSteps / 4, false>(ctx, shape, s, 1)) != 0)
             return -1;
         s.in = s.out;
         std::swap(s.out, s.other);
