@@ -56,32 +56,26 @@ class DeviceMatrix:
         self.packed = _pack(self.data, _TYPE_IDS[type], 0, rows, cols, stride)
 
 
-def _tensor(t, device: int) -> bytes:
-    """A torch tensor of one (a row) or two dimensions."""
-    kind = _TORCH_TYPES.get(t.dtype)
+def _matrix(x, ctx: Context):
+    """The C view of an operand (None stays None)."""
+    kind = _TORCH_TYPES.get(getattr(x, "dtype", None))
     if kind is None:
-        if _TORCH_TYPES:
-            raise CudaCppError(f"tensor type {t.dtype} is not supported")
-        import torch
-
-        _TORCH_TYPES.update({torch.float32: 0, torch.bfloat16: 1, torch.int8: 2, torch.int32: 3})
-        return _tensor(t, device)
-    if t.get_device() != device:
-        raise CudaCppError(f"tensor is on {t.device}, the context on cuda:{device}")
-    shape, stride = t.shape, t.stride()
+        return _other_matrix(x, ctx)
+    if x.get_device() != ctx.device:
+        raise CudaCppError(f"tensor is on {x.device}, the context on cuda:{ctx.device}")
+    shape, stride = x.shape, x.stride()
     if len(shape) == 2:
         rows, cols = shape
         if stride[1] != 1 and cols > 1 and rows:
             raise CudaCppError(f"tensor of strides {stride}: its last dimension must be contiguous")
-        return _pack(t.data_ptr(), kind, 0, rows, cols, stride[0])
+        return _pack(x.data_ptr(), kind, 0, rows, cols, stride[0])
     if len(shape) != 1 or (stride[0] != 1 and shape[0] > 1):
         raise CudaCppError(f"tensor of shape {tuple(shape)} and strides {stride}: one or two dimensions, the last one "
                            "contiguous, are supported")
-    return _pack(t.data_ptr(), kind, 0, 1, shape[0], shape[0])
+    return _pack(x.data_ptr(), kind, 0, 1, shape[0], shape[0])
 
 
-def _matrix(x, ctx: Context):
-    """The C view of an operand (None stays None)."""
+def _other_matrix(x, ctx: Context):
     if x is None:
         return None
     if isinstance(x, DeviceMatrix):
@@ -89,10 +83,15 @@ def _matrix(x, ctx: Context):
             raise CudaCppError(f"matrix is on device {x.device}, the context on {ctx.device}")
         return x.packed
     if isinstance(x, (F32Buffer, I32Buffer)):
-        return _matrix(DeviceMatrix(x, 1, len(x)), ctx)
+        return _other_matrix(DeviceMatrix(x, 1, len(x)), ctx)
     if not hasattr(x, "data_ptr"):
         raise CudaCppError(f"a matrix is expected, got {type(x).__name__}")
-    return _tensor(x, ctx.device)
+    if _TORCH_TYPES:
+        raise CudaCppError(f"tensor type {x.dtype} is not supported")
+    import torch
+
+    _TORCH_TYPES.update({torch.float32: 0, torch.bfloat16: 1, torch.int8: 2, torch.int32: 3})
+    return _matrix(x, ctx)
 
 
 def embedding_forward(ctx: Context, table, tokens, out, *, scale: float = 1.0) -> None:
