@@ -677,7 +677,9 @@ int launch_gradient(BulletOuCudaCppContext* ctx, const GradientArgs& a) {
     const int per_block = kThreads / kLanes;
     const int64_t blocks = static_cast<int64_t>(a.row_blocks) + (a.chunks + per_block - 1) / per_block;
     if (blocks > INT32_MAX) return fail_message("embedding gradient: too many tokens and rows");
-    LaunchShape shape{dim3(static_cast<unsigned>(blocks), (a.width / kUnit + kLanes * kUnits - 1) / (kLanes * kUnits)), kThreads};
+    const int parts = (a.width / kUnit + kLanes * kUnits - 1) / (kLanes * kUnits);
+    if (parts > 65535) return fail_messagef("embedding gradient: rows of %d are too wide", a.width);
+    LaunchShape shape{dim3(static_cast<unsigned>(blocks), parts), kThreads};
     shape.chained = a.n > 0;
     if (launch_kernel(ctx, "embedding gradient launch", gradient_kernel<In, Out, kUnit, kLanes, kUnits>, shape, a) != 0) return -1;
     if (a.chunks <= 1) return 0;

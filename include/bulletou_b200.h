@@ -582,7 +582,9 @@ int bulletou_b200_hcpe_to_psv_device(BulletOuCudaCppContext* ctx, const BulletOu
 
 /* rows x cols elements; element (r, c) at data + (r * row_stride + c) elements.
  * A vector of n is 1 x n.  row_stride counts only where rows > 1, and is then
- * at least cols.  The memory belongs to the caller. */
+ * at least cols.  rows and cols are at most 2^31 - 2^16.  The memory belongs to
+ * the caller.  An output shares no element with an input, except where an entry
+ * says that it may be the input itself. */
 typedef struct BulletOuB200Matrix {
     void* data;
     int type;           /* BULLETOU_B200_TYPE_* */

@@ -552,6 +552,22 @@ def test_scratch_grows_between_sizes(tctx):
     assert all(np.array_equal(a, b) for a, b in zip(small, again))
 
 
+# --------------------------------------------------------------------------- columns of one matrix
+def test_operands_that_are_columns_of_one_matrix(tctx):
+    """Slices of a wider matrix share its memory's span, but no element."""
+    rng = np.random.default_rng(31)
+    wide = torch.from_numpy(rng.standard_normal((20, 48)).astype(np.float32)).cuda()
+    before = wide.clone()
+    for x, out in ((wide[:, :16], wide[:, 16:32]), (wide[:, 32:], wide[:, 16:32])):
+        bo.dropout(tctx, x, out, probability=0.5, seed=4)
+        keep, factor = dropout_keep(0, 320, 0.5, 4, 0)
+        assert np.array_equal(host(out), np.where(keep.reshape(20, 16), host(x) * factor, 0.0))
+    assert torch.equal(wide[:, :16], before[:, :16]) and torch.equal(wide[:, 32:], before[:, 32:])
+    for x, out in ((wide[:, :16], wide[:, 8:24]), (wide[1:, :16], wide[:-1, 15:31])):  # they share a column
+        with pytest.raises(bo.CudaCppError, match="overlap"):
+            bo.dropout(tctx, x, out, probability=0.5, seed=4)
+
+
 # --------------------------------------------------------------------------- refusals
 def test_refusals(tctx):
     f, i8, i32 = (lambda *s: torch.zeros(*s, device="cuda")), (lambda *s: torch.zeros(*s, device="cuda", dtype=torch.int8)), \
