@@ -8,8 +8,8 @@
 // bound bf16 rows.  The threshold T = round(p * 2^16) is the probability that
 // is used, and f = 2^16 / (2^16 - T), so E[y] = x holds exactly.
 //
-// Aligned rows are bound by memory: 655360 x 256 bf16 with a residual take 152
-// us, 6.6 TB/s (101 % of a copy).  Unaligned ones by the integer pipe, which runs
+// Aligned rows are bound by memory: 655360 x 256 bf16 with a residual take 152 to
+// 164 us, 6.2 to 6.6 TB/s (a copy: 6.5).  Unaligned ones by the integer pipe, which runs
 // the logic and comparisons at half rate: 20011 x 769 f32 out of rows of 800 take
 // 31 us, 3.9 TB/s, 228 instructions for each piece of up to 224 elements.
 #include <algorithm>

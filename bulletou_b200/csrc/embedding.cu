@@ -102,8 +102,8 @@ struct LookupArgs {
 // rows' units are then loaded kRows at a time, all in flight together.  The
 // stores stream past L2, which keeps the table.
 //
-// Bound by the stores: 655360 rows of 256 bf16 take 71 us, 5.3 TB/s of which
-// 4.7 are written (torch's fill of that output alone takes 89 us).  With rows
+// Bound by the stores: 655360 rows of 256 bf16 take 71 to 74 us, 5.2 TB/s of which
+// 4.6 are written (torch's fill of that output alone takes 89 us).  With rows
 // held as f32, 70 registers and 24 warps on an SM it took 109 us.
 template <typename In, typename Out, int kUnit>
 __global__ void __launch_bounds__(kThreads, kLookupCtas) lookup_kernel(const LookupArgs a, int group, int span) {
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, kBinsOfThread <= 2 ? 5 : 2) sort_sca
 // Bound by reading the gradients once: 1310720 rows of 256 f32 take 225 us, 6.3
 // TB/s (97 % of a copy), with 4 rows in flight for each of 24 warps on an SM; 8
 // rows in flight needed 142 registers, left 8 warps and took 309 us.  Rows of an
-// odd width go one element at a time: 68438 of 257 f32 in 21 us, 3.4 TB/s.
+// odd width go one element at a time: 68438 of 257 f32 in 16 us, 4.4 TB/s.
 struct GradientArgs {
     const int2* entries;   // (token, position), sorted by token
     int n, chunk, chunks;
