@@ -67,12 +67,15 @@ struct DropoutArgs {
     bool flat;                        // no gaps between the rows of any operand
     size_t x_stride, residual_stride, out_stride;
     PhiloxKeys keys;
-    uint32_t threshold;               // dropped below; 65536: everything
+    uint32_t most_dropped;            // (T << 16) - 1: 16 bits below T, with whatever bits below them
+    bool keep_all;                    // T == 0
     float factor;
 };
 
-__device__ __forceinline__ bool kept(const Philox& r, int j, uint32_t threshold) {
-    return ((r.w[j >> 1] >> (16 * (j & 1))) & 0xffffu) >= threshold;
+// Lane j (16 bits) is not below T: compared in the upper half of a word, where the
+// odd lanes are already and a multiplication brings the even ones.
+__device__ __forceinline__ bool kept(const DropoutArgs& a, const Philox& r, int j) {
+    return a.keep_all || (j & 1 ? r.w[j >> 1] : r.w[j >> 1] << 16) > a.most_dropped;
 }
 
 // Eight neighbouring elements as 16 bytes of bf16 or 32 bytes of f32.
@@ -135,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) dropout_vector_kernel(const D
             const Philox random = philox_block(b, a.keys);
 #pragma unroll
             for (int j = 0; j < kLanes; ++j) {
-                const float v = kept(random, j, a.threshold) ? x[i].get(j) : 0.0f;
+                const float v = kept(a, random, j) ? x[i].get(j) : 0.0f;
                 x[i].set(j, kResidual ? __fmaf_rn(v, a.factor, r[i].get(j)) : v * a.factor);
             }
             x[i].store(out[i]);
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) dropout_vector_kernel(const D
     if (kFlat && blockIdx.x == 0 && threadIdx.x < a.n - blocks * kLanes) {
         const size_t e = blocks * kLanes + threadIdx.x;
         const Philox random = philox_block(blocks, a.keys);
-        const float v = kept(random, threadIdx.x, a.threshold) ? to_f32(static_cast<const T*>(a.x)[e]) : 0.0f;
+        const float v = kept(a, random, threadIdx.x) ? to_f32(static_cast<const T*>(a.x)[e]) : 0.0f;
         static_cast<T*>(a.out)[e] = from_f32<T>(kResidual ? __fmaf_rn(v, a.factor, to_f32(static_cast<const T*>(a.residual)[e]))
                                                           : v * a.factor);
     }
@@ -183,7 +186,7 @@ __device__ __forceinline__ void dropout_piece(const DropoutArgs& a, size_t row, 
     uint32_t word = 0;
 #pragma unroll
     for (int k = 0; k < kLanes; ++k) {
-        const uint32_t decisions = __ballot_sync(0xffffffffu, kept(random, k, a.threshold));
+        const uint32_t decisions = __ballot_sync(0xffffffffu, kept(a, random, k));
         if ((place & (kLanes - 1)) == k) word = decisions;
     }
     word >>= place / kLanes;
@@ -241,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) dropout_kernel(const DropoutA
         const Philox random = philox_block(b0 + lane, a.keys);
         uint32_t mask = 0;
 #pragma unroll
-        for (int j = 0; j < kLanes; ++j) mask |= kept(random, j, a.threshold) ? 1u << j : 0u;
+        for (int j = 0; j < kLanes; ++j) mask |= kept(a, random, j) ? 1u << j : 0u;
         T* out = static_cast<T*>(a.out) + row * a.out_stride + (e - row * cols);
 #pragma unroll
         for (int j = 0; j < kLanes; ++j) {
@@ -306,8 +309,10 @@ int bulletou_b200_dropout_device(BulletOuCudaCppContext* ctx, const BulletOuB200
     a.residual_stride = residual != nullptr ? residual->row_stride : 0;
     a.out_stride = out->row_stride;
     a.keys = philox_keys(seed, offset);
-    a.threshold = static_cast<uint32_t>(std::floor(probability * 65536.0 + 0.5));
-    a.factor = a.threshold < 65536u ? static_cast<float>(65536.0 / (65536.0 - a.threshold)) : 0.0f;
+    const uint32_t threshold = static_cast<uint32_t>(std::floor(probability * 65536.0 + 0.5));
+    a.keep_all = threshold == 0;
+    a.most_dropped = static_cast<uint32_t>((static_cast<uint64_t>(threshold) << 16) - 1);  // 65536: every word
+    a.factor = threshold < 65536u ? static_cast<float>(65536.0 / (65536.0 - threshold)) : 0.0f;
     // a vector where every eight is aligned: rows of whole eights, or no gaps between rows at all
     a.flat = is_flat(*x) && is_flat(*out) && (residual == nullptr || is_flat(*residual));
     const size_t unit = kLanes * type_bytes(x->type);

@@ -531,6 +531,64 @@ def test_library_buffers_streams_and_graphs():
     ctx.close()
 
 
+def test_all_operators_in_one_graph():
+    """Captured once after their sizes have run; the replay reads what the buffers hold then."""
+    stream = torch.cuda.Stream()
+    ctx = bo.Context(0, stream=stream.cuda_stream)
+    with torch.cuda.stream(stream):
+        rng = np.random.default_rng(6)
+        tokens = device(rng.integers(-1, 40, 3000).astype(np.int32))
+        table, weights = device(rng.standard_normal((40, 32))), device(rng.integers(-127, 128, (9, 32)).astype(np.int8))
+        hidden, d_table = device(np.zeros((3000, 32))), device(np.zeros((40, 32)))
+        logits, d_logits = device(np.zeros((3000, 9))), device(np.zeros((3000, 9)))
+        out = {"experts": device(np.zeros((3000, 2), np.int32)), "gates": device(np.zeros((3000, 2))),
+               "counts": device(np.zeros(10, np.int32)), "mean": device(np.zeros(9)), "loss": device([0.0])}
+        scales, one, gate_grad = device(np.full(9, 0.01)), device([1.0]), device(rng.standard_normal((3000, 2)))
+
+        def everything():
+            bo.embedding_forward(ctx, table, tokens, hidden, scale=0.5)
+            bo.dropout(ctx, hidden, hidden, probability=0.2, seed=8)
+            bo.int8_linear(ctx, hidden, weights, scales, logits)
+            bo.router_forward(ctx, logits, out["experts"], out["gates"], out["counts"], out["mean"], out["loss"], balance=0.1)
+            bo.router_backward(ctx, logits, out["experts"], out["counts"], gate_grad, one, d_logits, balance=0.1)
+            bo.embedding_backward(ctx, tokens, hidden, d_table, scale=2.0)
+
+        everything()
+        bo.GraphExec.begin_capture(ctx)
+        everything()
+        graph = bo.GraphExec.end_capture(ctx)
+        tokens.copy_(device(rng.integers(-1, 40, 3000).astype(np.int32)))
+        table.mul_(-0.75)
+        everything()
+        want = [t.clone() for t in (hidden, logits, d_logits, d_table, *out.values())]
+        for t in (hidden, logits, d_logits, d_table, *out.values()):
+            t.fill_(3)
+        graph.launch(ctx)
+        stream.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, (hidden, logits, d_logits, d_table, *out.values())))
+    graph.close()
+    ctx.close()
+
+
+def test_tensors_of_another_stream_are_ordered_by_events():
+    """The context has a stream of its own: torch's work and the library's wait for one another by events."""
+    import ctypes
+
+    ctx = bo.Context(0)
+    p = ctypes.c_void_p()
+    ctx.lib.call("bulletou_b200_context_stream", ctx.as_ptr(), ctypes.byref(p))
+    theirs, ours = torch.cuda.current_stream(), torch.cuda.ExternalStream(p.value)
+    x, y = torch.zeros(2048, 4096, device="cuda"), torch.zeros(2048, 4096, device="cuda")
+    for round_ in range(1, 6):
+        for _ in range(20):
+            x.add_(1.0)  # work that the library has to wait for
+        ours.wait_stream(theirs)
+        bo.dropout(ctx, x, y, probability=0.0, seed=1)
+        theirs.wait_stream(ours)
+        assert bool((y == 20.0 * round_).all())
+    ctx.close()
+
+
 def test_scratch_grows_between_sizes(tctx):
     """Small, large, small again: scratch that grew in between changes nothing."""
     rng = np.random.default_rng(3)
