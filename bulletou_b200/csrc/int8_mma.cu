@@ -535,10 +535,13 @@ int launch_pairs(BulletOuCudaCppContext* ctx, const ProductArgs& a, int tiles, b
 template <typename Out>
 int launch_typed(BulletOuCudaCppContext* ctx, const ProductArgs& a, bool early, bool weights_ready) {
     const bool vector_ok = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && (a.m <= 1 || a.out_stride * sizeof(Out) % 16 == 0);
-    // Pairs as soon as they fill 64 SMs: 512 x 4096 x 4096 (32 tiles) takes 18 us in
-    // pairs and 27 in single tiles, 256 x 4096 x 4096 (16) 16.5 and 11.8.
+    // Single tiles while they all run at once, two on an SM: 512 x 4096 x 4096 (256 of
+    // them) takes 15 us, in pairs 18; 8192 x 640 x 256 (256) 6.0 and 9.0.  Beyond,
+    // pairs, unless most of their columns are empty: 16384 x 2560 x 256 (512) takes
+    // 13 us in pairs, 17 singly, but 65536 x 640 x 64 16 and 10.
     const int64_t pairs = static_cast<int64_t>((a.m + 255) / 256) * ((a.n + 255) / 256);
-    if (pairs >= 32 && pairs <= INT32_MAX)
+    const int64_t singles = static_cast<int64_t>((a.m + 127) / 128) * ((a.n + 63) / 64);
+    if (a.n > 64 && singles > 2 * ctx->sm_count && pairs <= INT32_MAX)
         return launch_pairs<Out>(ctx, a, static_cast<int>(pairs), vector_ok, early);
     return launch_tiles<Out>(ctx, a, vector_ok, early, weights_ready);
 }
