@@ -9,6 +9,7 @@
 // order: no floating atomics, the same bits from call to call, every row of
 // out_gradients read once and every row of the table written once.
 #include <algorithm>
+#include <climits>
 #include <utility>
 
 #include "device_matrix.cuh"
@@ -159,10 +160,9 @@ struct SortPass {
     Tokens tokens;           // keys of the first pass
     const int2* in;          // (token, position); null: the tokens themselves, at positions 0..n-1
     int2* out;
-    int2* other;             // where the pass after this one goes
     int* counts;             // [bins][tiles], turned into starts inside a bin
     int* totals;             // [bins]
-    int n, tiles, shift, digit_bits, bins;
+    int n, tiles, shift, bins;
     __device__ __forceinline__ int2 entry(int i) const { return in != nullptr ? in[i] : make_int2(tokens(i), i); }
     __device__ __forceinline__ int digit(int k) const { return (k >> shift) & (bins - 1); }
 };
@@ -206,10 +206,10 @@ __device__ __forceinline__ int block_exclusive(int v, int* warp_sums, int* total
     return before + incl - v;
 }
 
-// CTA per bin: where each tile's keys of the bin start inside the bin.
+// CTA per bin: where each tile's keys of the bin start inside the bin.  It does
+// not let the scatter start early: that cost 8 us of 39 for 68438 tokens.
 __global__ void __launch_bounds__(kThreads) sort_scan_kernel(const SortPass s) {
     __shared__ int warp_sums[kWarps];
-    let_next_start();
     wait_for_previous();
     int* counts = s.counts + static_cast<size_t>(blockIdx.x) * s.tiles;
     int run = 0;
@@ -225,89 +225,114 @@ __global__ void __launch_bounds__(kThreads) sort_scan_kernel(const SortPass s) {
 
 // CTA per tile, each warp a run of consecutive entries: an entry's place is the
 // start of its bin, its tile's start in the bin, the entries of earlier warps,
-// and its rank among the equal digits of its warp.  kAlone: one tile holds all
-// entries, so its own counts are all there is and the CTA runs every pass.
-template <int kSteps, bool kAlone, int kBinsOfThread>
-__global__ void __launch_bounds__(kThreads, kBinsOfThread <= 2 ? 5 : 2) sort_scatter_kernel(SortPass s, int passes) {
+// and its rank among the equal digits of its warp.
+template <int kSteps, int kBinsOfThread>
+__global__ void __launch_bounds__(kThreads, kBinsOfThread <= 2 ? 5 : 2) sort_scatter_kernel(const SortPass s) {
     extern __shared__ int places[];  // [kWarps][bins]
     __shared__ int warp_sums[kWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int* const place = places + warp * s.bins;
     let_next_start();
     const int bin0 = threadIdx.x * kBinsOfThread;
-    for (int pass = 0; pass < passes; ++pass) {
-        for (int i = threadIdx.x; i < kWarps * s.bins; i += kThreads) places[i] = 0;
-        __syncthreads();
-        if (pass == 0) wait_for_previous();
-        const int first = blockIdx.x * (kSteps * kThreads) + warp * (kSteps * 32) + lane;
-        int2 entry[kSteps];
-        int rank[kSteps];
+    for (int i = threadIdx.x; i < kWarps * s.bins; i += kThreads) places[i] = 0;
+    __syncthreads();
+    wait_for_previous();
+    const int first = blockIdx.x * (kSteps * kThreads) + warp * (kSteps * 32) + lane;
+    int2 entry[kSteps];
+    int rank[kSteps];
 #pragma unroll
-        for (int j = 0; j < kSteps; ++j) entry[j] = first + j * 32 < s.n ? s.entry(first + j * 32) : make_int2(-1, 0);
-        int total[kBinsOfThread], start[kBinsOfThread];
-        if (!kAlone) {
+    for (int j = 0; j < kSteps; ++j) entry[j] = first + j * 32 < s.n ? s.entry(first + j * 32) : make_int2(-1, 0);
+    int total[kBinsOfThread], start[kBinsOfThread];
 #pragma unroll
-            for (int i = 0; i < kBinsOfThread; ++i) {
-                const bool in = bin0 + i < s.bins;
-                total[i] = in ? s.totals[bin0 + i] : 0;
-                start[i] = in ? s.counts[static_cast<size_t>(bin0 + i) * s.tiles + blockIdx.x] : 0;
+    for (int i = 0; i < kBinsOfThread; ++i) {
+        const bool in = bin0 + i < s.bins;
+        total[i] = in ? s.totals[bin0 + i] : 0;
+        start[i] = in ? s.counts[static_cast<size_t>(bin0 + i) * s.tiles + blockIdx.x] : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+        // the lanes with this lane's digit; those past the last entry go by themselves
+        const bool live = entry[j].x >= 0;
+        const int d = live ? s.digit(entry[j].x) : 0;
+        unsigned peers = __ballot_sync(0xffffffffu, live);
+        peers = live ? peers : ~peers;
+#pragma unroll
+        for (int bit = 1; bit < kThreads * kBinsOfThread; bit <<= 1) {
+            if (bit >= s.bins) break;
+            const unsigned set = __ballot_sync(0xffffffffu, d & bit);
+            peers &= d & bit ? set : ~set;
+        }
+        const int before = live ? place[d] : 0;
+        __syncwarp();  // every lane has read it
+        rank[j] = before + __popc(peers & ((1u << lane) - 1));
+        if (live && lane == 31 - __clz(peers)) place[d] = before + __popc(peers);
+        __syncwarp();
+    }
+    __syncthreads();
+    int sum = 0;
+#pragma unroll
+    for (int i = 0; i < kBinsOfThread; ++i) sum += total[i];
+    int all;
+    int at = block_exclusive(sum, warp_sums, &all);
+#pragma unroll
+    for (int i = 0; i < kBinsOfThread; ++i) {
+        if (bin0 + i < s.bins) {
+            int next = at + start[i];
+            for (int w = 0; w < kWarps; ++w) {
+                const int c = places[w * s.bins + bin0 + i];
+                places[w * s.bins + bin0 + i] = next;
+                next += c;
             }
         }
+        at += total[i];
+    }
+    __syncthreads();
 #pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-            // the lanes with this lane's digit; those past the last entry go by themselves
-            const bool live = entry[j].x >= 0;
-            const int d = live ? s.digit(entry[j].x) : 0;
-            unsigned peers = __ballot_sync(0xffffffffu, live);
-            peers = live ? peers : ~peers;
-#pragma unroll
-            for (int bit = 1; bit < kThreads * kBinsOfThread; bit <<= 1) {
-                if (bit >= s.bins) break;
-                const unsigned set = __ballot_sync(0xffffffffu, d & bit);
-                peers &= d & bit ? set : ~set;
-            }
-            const int before = live ? place[d] : 0;
-            __syncwarp();  // every lane has read it
-            rank[j] = before + __popc(peers & ((1u << lane) - 1));
-            if (live && lane == 31 - __clz(peers)) place[d] = before + __popc(peers);
-            __syncwarp();
+    for (int j = 0; j < kSteps; ++j)
+        if (entry[j].x >= 0) s.out[place[s.digit(entry[j].x)] + rank[j]] = entry[j];
+}
+
+// Few tokens are ranked instead, in one launch: a token's place is the number of
+// tokens that are smaller, or equal and earlier.  A CTA ranks kRankTokens of
+// them, kRankParts threads for each, against all n in shared memory.  The gradient
+// of 4096 tokens x 64 takes 18 us with it and 23 with the radix sort, of 8192 25
+// and 24, of 24 tokens 7 and 16.
+constexpr int kRankMost = 4096;
+constexpr int kRankTokens = 64;
+constexpr int kRankParts = kThreads / kRankTokens;
+
+__global__ void __launch_bounds__(kThreads) rank_tokens_kernel(const Tokens tokens, int2* out) {
+    extern __shared__ int4 shared_tokens[];
+    __shared__ int ranks[kRankParts][kRankTokens];
+    int* const all = reinterpret_cast<int*>(shared_tokens);
+    const int n = tokens.n, padded = (n + 3) / 4 * 4;
+    let_next_start();
+    for (int i = threadIdx.x; i < padded; i += kThreads) all[i] = i < n ? tokens(i) : INT_MAX;
+    __syncthreads();
+    const int slot = threadIdx.x % kRankTokens, part = threadIdx.x / kRankTokens;
+    const int first = blockIdx.x * kRankTokens, i = first + slot;
+    const int mine = i < n ? all[i] : INT_MAX;
+    // four tokens at a time; those before this CTA's come first among equals, those after it do not
+    int rank = 0;
+    const int quads = padded / 4, q0 = first / 4, q1 = min(quads, q0 + kRankTokens / 4);
+    for (int q = part; q < q0; q += kRankParts) {
+        const int4 t = shared_tokens[q];
+        rank += (t.x <= mine) + (t.y <= mine) + (t.z <= mine) + (t.w <= mine);
+    }
+    for (int q = q0 + part; q < q1; q += kRankParts)
+        for (int j = 0; j < 4; ++j) {
+            const int other = 4 * q + j;
+            rank += all[other] < mine || (all[other] == mine && other < i);
         }
-        __syncthreads();
-        int sum = 0;
-#pragma unroll
-        for (int i = 0; i < kBinsOfThread; ++i) {
-            if (kAlone) {
-                start[i] = total[i] = 0;
-                if (bin0 + i < s.bins)
-                    for (int w = 0; w < kWarps; ++w) total[i] += places[w * s.bins + bin0 + i];
-            }
-            sum += total[i];
-        }
-        int all;
-        int at = block_exclusive(sum, warp_sums, &all);
-#pragma unroll
-        for (int i = 0; i < kBinsOfThread; ++i) {
-            if (bin0 + i < s.bins) {
-                int next = at + start[i];
-                for (int w = 0; w < kWarps; ++w) {
-                    const int c = places[w * s.bins + bin0 + i];
-                    places[w * s.bins + bin0 + i] = next;
-                    next += c;
-                }
-            }
-            at += total[i];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < kSteps; ++j)
-            if (entry[j].x >= 0) s.out[place[s.digit(entry[j].x)] + rank[j]] = entry[j];
-        if (kAlone) {
-            __syncthreads();
-            s.in = s.out;
-            s.out = s.other;
-            s.other = const_cast<int2*>(s.in);
-            s.shift += s.digit_bits;
-        }
+    for (int q = q1 + part; q < quads; q += kRankParts) {
+        const int4 t = shared_tokens[q];
+        rank += (t.x < mine) + (t.y < mine) + (t.z < mine) + (t.w < mine);
+    }
+    ranks[part][slot] = rank;
+    __syncthreads();
+    if (part == 0 && i < n) {
+        for (int p = 1; p < kRankParts; ++p) rank += ranks[p][slot];
+        out[rank] = make_int2(mine, i);
     }
 }
 
@@ -376,7 +401,7 @@ __device__ void write_empty_rows(const GradientArgs& a, int block) {
 // kLanes lanes hold kUnits units of a row each; blockIdx.y cuts wider rows.
 template <typename In, typename Out, int kUnit, int kLanes, int kUnits>
 __global__ void __launch_bounds__(kThreads, 3) gradient_kernel(const GradientArgs a) {
-    constexpr int kBatch = 4;  // rows in flight
+    constexpr int kBatch = kUnit * kUnits > 4 ? 4 : kUnit * kUnits > 1 ? 8 : 16;  // rows in flight
     let_next_start();
     wait_for_previous();
     if (static_cast<int>(blockIdx.x) < a.row_blocks) {
@@ -591,8 +616,8 @@ GradientPlan plan_gradient(const BulletOuCudaCppContext* ctx, int n, int vocab, 
     while (static_cast<int64_t>(vocab) >> bits != 0) ++bits;
     p.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
     p.digit_bits = (bits + p.passes - 1) / p.passes;
-    // a CTA for every SM while there are tokens enough; one alone where it can hold them all
-    p.tile = n <= kMaxTile || n > kMaxTile / 2 * ctx->sm_count ? kMaxTile : n > kMaxTile / 4 * ctx->sm_count ? kMaxTile / 2 : kMaxTile / 4;
+    // a CTA for every SM while there are tokens enough
+    p.tile = n > kMaxTile / 2 * ctx->sm_count ? kMaxTile : n > kMaxTile / 4 * ctx->sm_count ? kMaxTile / 2 : kMaxTile / 4;
     p.tiles = (n + p.tile - 1) / p.tile;
     p.row = (static_cast<size_t>(n) + 63) / 64 * 64;
     p.counts = ((static_cast<size_t>(1) << p.digit_bits) * p.tiles + 63) / 64 * 64;
@@ -615,13 +640,13 @@ GradientPlan plan_gradient(const BulletOuCudaCppContext* ctx, int n, int vocab, 
     return p;
 }
 
-template <int kSteps, bool kAlone>
-int launch_scatter(BulletOuCudaCppContext* ctx, const LaunchShape& shape, const SortPass& s, int passes) {
-    auto with = [&](auto kernel) { return launch_kernel(ctx, "embedding sort launch", kernel, shape, s, passes); };
-    if (s.bins <= kThreads) return with(sort_scatter_kernel<kSteps, kAlone, 1>);
-    if (s.bins <= 2 * kThreads) return with(sort_scatter_kernel<kSteps, kAlone, 2>);
-    if (s.bins <= 4 * kThreads) return with(sort_scatter_kernel<kSteps, kAlone, 4>);
-    return with(sort_scatter_kernel<kSteps, kAlone, 8>);
+template <int kSteps>
+int launch_scatter(BulletOuCudaCppContext* ctx, const LaunchShape& shape, const SortPass& s) {
+    auto with = [&](auto kernel) { return launch_kernel(ctx, "embedding sort launch", kernel, shape, s); };
+    if (s.bins <= kThreads) return with(sort_scatter_kernel<kSteps, 1>);
+    if (s.bins <= 2 * kThreads) return with(sort_scatter_kernel<kSteps, 2>);
+    if (s.bins <= 4 * kThreads) return with(sort_scatter_kernel<kSteps, 4>);
+    return with(sort_scatter_kernel<kSteps, 8>);
 }
 
 // Sorts the tokens into the scratch at `base`.
@@ -633,40 +658,34 @@ int sort_tokens(BulletOuCudaCppContext* ctx, const Tokens& tokens, const Gradien
     s.bins = 1 << plan.digit_bits;
     s.totals = base + 4 * plan.row;
     s.counts = s.totals + kMaxBins;
-    s.digit_bits = plan.digit_bits;
     s.out = reinterpret_cast<int2*>(base);
-    s.other = s.out + plan.row;
-    LaunchShape shape{dim3(plan.tiles), kThreads};
-    const size_t places = static_cast<size_t>(kWarps) * s.bins * sizeof(int);
-    constexpr int kSteps = kMaxTile / kThreads;
-    if (plan.tile == kMaxTile && plan.tiles == 1) {
-        shape.smem = places;
-        if (launch_scatter<kSteps, true>(ctx, shape, s, plan.passes) != 0) return -1;
-        out->entries = plan.passes % 2 == 1 ? s.out : s.other;
-        return 0;
+    if (tokens.n <= kRankMost) {
+        const LaunchShape shape{dim3((tokens.n + kRankTokens - 1) / kRankTokens), kThreads, (static_cast<size_t>(tokens.n) + 3) / 4 * 16};
+        out->entries = s.out;
+        return launch_kernel(ctx, "embedding sort launch", rank_tokens_kernel, shape, tokens, s.out);
     }
+    int2* other = s.out + plan.row;
+    LaunchShape shape{dim3(plan.tiles), kThreads};
+    constexpr int kSteps = kMaxTile / kThreads;
     const int part = kMaxTile / plan.tile;  // the steps of a tile are those of the largest, or a half or a quarter of them
     for (int pass = 0; pass < plan.passes; ++pass) {
         s.shift = pass * plan.digit_bits;
         shape.chained = pass > 0;
         shape.smem = 0;
         shape.grid = dim3(plan.tiles);
-        if (launch_kernel(ctx, "embedding sort launch", part == 1   ? sort_count_kernel<kSteps>
-                          : part == 2 ? sort_count_kernel<kSteps / 2>
-                                      : sort_count_kernel<kSteps / 4>,
-                          shape, s) != 0)
-            return -1;
+        auto* const count = part == 1 ? sort_count_kernel<kSteps> : part == 2 ? sort_count_kernel<kSteps / 2> : sort_count_kernel<kSteps / 4>;
+        if (launch_kernel(ctx, "embedding sort launch", count, shape, s) != 0) return -1;
         shape.chained = true;
         shape.grid = dim3(s.bins);
         if (launch_kernel(ctx, "embedding sort launch", sort_scan_kernel, shape, s) != 0) return -1;
         shape.grid = dim3(plan.tiles);
-        shape.smem = places;
-        if ((part == 1   ? launch_scatter<kSteps, false>(ctx, shape, s, 1)
-             : part == 2 ? launch_scatter<kSteps / 2, false>(ctx, shape, s, 1)
-                         : launch_scatter<kSteps / 4, false>(ctx, shape, s, 1)) != 0)
+        shape.smem = static_cast<size_t>(kWarps) * s.bins * sizeof(int);
+        if ((part == 1   ? launch_scatter<kSteps>(ctx, shape, s)
+             : part == 2 ? launch_scatter<kSteps / 2>(ctx, shape, s)
+                         : launch_scatter<kSteps / 4>(ctx, shape, s)) != 0)
             return -1;
         s.in = s.out;
-        std::swap(s.out, s.other);
+        std::swap(s.out, other);
     }
     out->entries = s.in;
     return 0;
