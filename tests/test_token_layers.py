@@ -61,6 +61,7 @@ def test_entries_refuse_a_null_context(lib):
     for name in ("embedding_forward", "embedding_backward", "dropout", "router_forward", "router_backward",
                  "int8_quantize_rows", "int8_matmul", "int8_linear"):
         full = f"bulletou_b200_{name}_device"
-        args = [a(0) if a in (ctypes.c_float, ctypes.c_int, ctypes.c_uint64) else None for a in SIGNATURES[full]]
+        values = (ctypes.c_float, ctypes.c_double, ctypes.c_int, ctypes.c_uint64)
+        args = [a(0) if a in values else None for a in SIGNATURES[full]]
         assert lib.fn(full)(*args) == -1
         assert "context must not be null" in lib.last_error()
