@@ -362,18 +362,23 @@ template <typename T, int kGroup, int kPlaces>
 __global__ void __launch_bounds__(kThreads, kCtas<kPlaces>) router_backward_kernel(const RouterArgs a) {
     __shared__ int64_t choices;
     __shared__ int shared_counts[kGroup * kPlaces];
+    __shared__ float shared_pull[kGroup * kPlaces];
     const int lane = threadIdx.x & (kGroup - 1);
     for (int e = threadIdx.x; e < kGroup * kPlaces; e += kThreads) shared_counts[e] = e < a.experts ? a.counts[e] : 0;
     __syncthreads();
     sum_choices(shared_counts, a.experts, &choices);
     __syncthreads();
-    // the balance loss's pull on every probability of an expert
+    // The balance loss's pull on every probability of an expert, h_e less the mean
+    // of h: the probabilities sum to one, so what all h share cancels, and experts
+    // nearly in balance would leave only its rounding.  E c_e - sum c is exact.
+    const float unit = (a.loss_grad != nullptr ? a.loss_grad[0] : 0.0f) * a.balance / static_cast<float>(max(a.counts[a.experts], 1)) /
+                       static_cast<float>(max(choices, static_cast<int64_t>(1)));
+    for (int e = threadIdx.x; e < kGroup * kPlaces; e += kThreads)
+        shared_pull[e] = e < a.experts ? static_cast<float>(static_cast<int64_t>(shared_counts[e]) * a.experts - choices) * unit : 0.0f;
+    __syncthreads();
     float2 h[kPlaces / 2];
-    const float unit = (a.loss_grad != nullptr ? a.loss_grad[0] : 0.0f) * a.balance * static_cast<float>(a.experts) /
-                       static_cast<float>(max(a.counts[a.experts], 1)) / static_cast<float>(max(choices, static_cast<int64_t>(1)));
-    auto pull_of = [&](int e) { return static_cast<float>(shared_counts[e]) * unit; };
 #pragma unroll
-    for (int i = 0; i < kPlaces / 2; ++i) h[i] = make_float2(pull_of(lane + kGroup * 2 * i), pull_of(lane + kGroup * (2 * i + 1)));
+    for (int i = 0; i < kPlaces / 2; ++i) h[i] = make_float2(shared_pull[lane + kGroup * 2 * i], shared_pull[lane + kGroup * (2 * i + 1)]);
     constexpr int kRows = kThreads / kGroup;
     const int places = places_of<kGroup>(a.experts, lane);
     const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
@@ -393,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<kPlaces>) router_backward_kern
         Row<kGroup, kPlaces> r;
         r.template load<T>(src, mine);
         const float z = pick >= 0 ? to_f32(src[pick - lane]) : -INFINITY;
-        const float pull = pick >= 0 ? static_cast<float>(shared_counts[pick]) * unit : 0.0f;
+        const float pull = pick >= 0 ? shared_pull[pick] : 0.0f;
         chosen += step * a.chosen_stride;
         gate_grad += step * a.gate_grad_stride;
         next_pick = chooses && t + step < a.rows ? *chosen : -1;

@@ -307,6 +307,24 @@ def test_router(tctx, rows, experts, k, t, pad, normalize):
         assert torch.equal(out[name], again[name])
 
 
+@pytest.mark.parametrize("counts", [[500, 500], [12800, 12754], [3, 4, 3, 4, 3], [2**31 - 1, 2**31 - 2], [7] * 128])
+def test_router_balance_gradient_of_experts_nearly_in_balance(tctx, counts):
+    # what all experts' pulls share cancels: the error is measured by how far they differ
+    rng = np.random.default_rng(len(counts))
+    experts = len(counts)
+    z = rng.uniform(-3, 3, (301, experts)).astype(np.float32).astype(np.float64)
+    p = np.exp(z - z.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    pull = 0.5 * np.float32(0.9) / 301 * ((experts * np.array(counts, np.int64) - sum(counts)) / sum(counts))
+    want = p * (pull - (p * pull).sum(1, keepdims=True))
+    got = device(np.full((301, experts), 9.0))
+    bo.router_backward(tctx, device(z), device(np.zeros((301, 1), np.int32)), device(np.array([counts + [301]], np.int32)), None,
+                       device([np.float32(0.9)]), got, balance=0.5)
+    # a probability: the rounding of its exponent (6 log2 e) and of its operations and the sum's; then the pull's and the dot's
+    bound = (2 * 6 * 1.4427 + 64 + experts) * U32 * p * np.abs(pull).max() + 1e-45
+    assert (np.abs(host(got) - want) <= bound).all()
+
+
 @pytest.mark.parametrize("normalize", [False, True])
 def test_router_gradient_formula_against_differences(tctx, normalize):
     rng = np.random.default_rng(4)
