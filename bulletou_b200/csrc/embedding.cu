@@ -105,10 +105,15 @@ struct LookupArgs {
 //
 // Bound by the stores: 655360 rows of 256 bf16 take 71 to 74 us, 5.2 TB/s of which
 // 4.6 are written (torch's fill of that output alone takes 89 us).  With rows
-// held as f32, 70 registers and 24 warps on an SM it took 109 us.
-template <typename In, typename Out, int kUnit>
-__global__ void __launch_bounds__(kThreads, kLookupCtas) lookup_kernel(const LookupArgs a, int group, int span) {
+// held as f32, 70 registers and 24 warps on an SM it took 109 us.  Units of one or
+// two elements are bound by latency: rows of more than 32 of them have kCols
+// units of each row in flight in a lane, 155642 rows of 257 f32 46 us instead of
+// 66, 600000 of 63 bf16 37 instead of 55.  Aligned 16-byte blocks shifted into
+// place took 79 us there: all lanes go through the rows' ends element by element.
+template <typename In, typename Out, int kUnit, int kCols>
+__global__ void __launch_bounds__(kThreads, kLookupCtas) lookup_kernel(const LookupArgs a, int any_group, int span) {
     constexpr int kRows = 4;
+    const int group = kCols > 1 ? 32 : any_group;  // with a group known only at run time the columns' offsets cost 100 bytes of spills
     const int lane = threadIdx.x & (group - 1);
     // blockIdx.y cuts the columns
     const int share = (a.width / kUnit + gridDim.y - 1) / gridDim.y;
@@ -125,20 +130,28 @@ __global__ void __launch_bounds__(kThreads, kLookupCtas) lookup_kernel(const Loo
             int token[kRows];
 #pragma unroll
             for (int i = 0; i < kRows; ++i) token[i] = __shfl_sync(0xffffffffu, own, i0 + i, group);
-            for (int u = unit0 + lane; u < units; u += group) {
-                Raw<In, kUnit> v[kRows];
+            for (int u = unit0 + lane; u < units; u += group * kCols) {
+                Raw<In, kUnit> v[kRows][kCols];
 #pragma unroll
                 for (int i = 0; i < kRows; ++i) {
-                    if (i0 + i < rows && token[i] < a.tokens.vocab) v[i].load(table + token[i] * a.table_stride + u * kUnit);
-                    else v[i].clear();
+                    const In* const row = table + token[i] * a.table_stride + u * kUnit;
+#pragma unroll
+                    for (int k = 0; k < kCols; ++k) {
+                        if (i0 + i < rows && token[i] < a.tokens.vocab && (k == 0 || u + k * group < units)) v[i][k].load(row + k * group * kUnit);
+                        else v[i][k].clear();
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < kRows; ++i) {
                     if (i0 + i >= rows) break;
-                    Raw<Out, kUnit> y;
+                    Out* const row = out + (i0 + i) * a.out_stride + u * kUnit;
 #pragma unroll
-                    for (int j = 0; j < kUnit; ++j) y.set(j, v[i].get(j) * a.scale);
-                    y.store(out + (i0 + i) * a.out_stride + u * kUnit);
+                    for (int k = 0; k < kCols; ++k) {
+                        Raw<Out, kUnit> y;
+#pragma unroll
+                        for (int j = 0; j < kUnit; ++j) y.set(j, v[i][k].get(j) * a.scale);
+                        if (k == 0 || u + k * group < units) y.store(row + k * group * kUnit);
+                    }
                 }
             }
         }
@@ -748,7 +761,7 @@ bool rows_of_units(const BulletOuB200Matrix& a, const BulletOuB200Matrix& b) {
            rows_aligned(b, std::min<size_t>(16, kUnit * sizeof(B)));
 }
 
-template <typename In, typename Out, int kUnit>
+template <typename In, typename Out, int kUnit, int kCols>
 int launch_lookup(BulletOuCudaCppContext* ctx, const LookupArgs& a) {
     const int units = a.width / kUnit;
     int group = 1;
@@ -761,14 +774,16 @@ int launch_lookup(BulletOuCudaCppContext* ctx, const LookupArgs& a) {
     const int64_t blocks = ((static_cast<int64_t>(a.tokens.n) + span - 1) / span * group + kThreads - 1) / kThreads;
     const unsigned x = static_cast<unsigned>(std::min(blocks, resident));
     const unsigned y = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(units / 64, resident / x)));
-    return launch_kernel(ctx, "embedding lookup launch", lookup_kernel<In, Out, kUnit>, LaunchShape{dim3(x, y), kThreads}, a, group, span);
+    return launch_kernel(ctx, "embedding lookup launch", lookup_kernel<In, Out, kUnit, kCols>, LaunchShape{dim3(x, y), kThreads}, a, group, span);
 }
 
 template <typename In, typename Out>
 int lookup(BulletOuCudaCppContext* ctx, const LookupArgs& a, const BulletOuB200Matrix& table, const BulletOuB200Matrix& out) {
-    if (rows_of_units<In, Out, kVectorUnit<In, Out>>(table, out)) return launch_lookup<In, Out, kVectorUnit<In, Out>>(ctx, a);
-    if (rows_of_units<In, Out, 2>(table, out)) return launch_lookup<In, Out, 2>(ctx, a);
-    return launch_lookup<In, Out, 1>(ctx, a);
+    if (rows_of_units<In, Out, kVectorUnit<In, Out>>(table, out)) return launch_lookup<In, Out, kVectorUnit<In, Out>, 1>(ctx, a);
+    if (rows_of_units<In, Out, 2>(table, out))
+        return a.width > 64 ? launch_lookup<In, Out, 2, 2>(ctx, a) : launch_lookup<In, Out, 2, 1>(ctx, a);
+    if (a.width > 64) return launch_lookup<In, Out, 1, 4>(ctx, a);
+    return a.width > 32 ? launch_lookup<In, Out, 1, 2>(ctx, a) : launch_lookup<In, Out, 1, 1>(ctx, a);
 }
 
 }  // namespace
