@@ -54,7 +54,8 @@ struct Raw {
     }
     __device__ __forceinline__ void load(const T* p) {
         if constexpr (kUnit == 1) {
-            *reinterpret_cast<T*>(w) = *p;
+            if constexpr (sizeof(T) == 2) w[0] = *reinterpret_cast<const unsigned short*>(p);  // the whole word, so that none is merged
+            else w[0] = *reinterpret_cast<const uint32_t*>(p);
         } else if constexpr (kWords == 1) {
             w[0] = *reinterpret_cast<const uint32_t*>(p);
         } else if constexpr (kWords == 2) {
@@ -414,7 +415,7 @@ __device__ void write_empty_rows(const GradientArgs& a, int block) {
 // kLanes lanes hold kUnits units of a row each; blockIdx.y cuts wider rows.
 template <typename In, typename Out, int kUnit, int kLanes, int kUnits>
 __global__ void __launch_bounds__(kThreads, 3) gradient_kernel(const GradientArgs a) {
-    constexpr int kBatch = kUnit * kUnits > 4 ? 4 : kUnit * kUnits > 1 ? 8 : 16;  // rows in flight
+    constexpr int kBatch = kUnit * kUnits > 4 ? 4 : 8;  // rows in flight
     let_next_start();
     wait_for_previous();
     if (static_cast<int>(blockIdx.x) < a.row_blocks) {
