@@ -497,8 +497,8 @@ __global__ void __launch_bounds__(kThreads, 3) gradient_kernel(const GradientArg
 
 // CTA for kWarps chunks: the rows whose run begins in a chunk and goes on after
 // it.  Runs over up to kShortRun more chunks take a warp each; longer ones are
-// shared by the CTA's warps, each a run of consecutive chunks, and joined in
-// that order.  A lane takes eight columns at a time, two 16-byte loads of every
+// shared by strands of the CTA's lanes, each a run of consecutive chunks, and
+// joined in a fixed order.  A lane takes eight columns at a time, two 16-byte loads of every
 // partial row.  Bound by latency: the run's end is searched 32 chunks at a time
 // (a binary search of 20 steps made it 37 us for 10240 chunks of 256 columns, of
 // which the longest run covers 245; now 15).
@@ -541,18 +541,18 @@ __global__ void __launch_bounds__(kThreads, 4) joined_rows_kernel(const Gradient
     }
     __syncthreads();
     auto add = [](float4& s, const float4& v) { s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w; };
-    auto add_heads = [&](int first, int count, int base, float4* s) {
-        const float* row = a.heads + first * a.part_stride + base + lane * 4;
+    auto add_heads = [&](int first, int count, int column, float4* s) {
+        const float* row = a.heads + first * a.part_stride + column;
 #pragma unroll 4
         for (int i = 0; i < count; ++i, row += a.part_stride)
 #pragma unroll
             for (int j = 0; j < kQuads; ++j)
-                if (base + lane * 4 + 128 * j < a.width) add(s[j], *reinterpret_cast<const float4*>(row + 128 * j));
+                if (column + 128 * j < a.width) add(s[j], *reinterpret_cast<const float4*>(row + 128 * j));
     };
-    auto finish = [&](int c, int key, int base, float4* s) {
+    auto finish = [&](int c, int key, int first_column, float4* s) {
 #pragma unroll
         for (int j = 0; j < kQuads; ++j) {
-            const int column = base + lane * 4 + 128 * j;
+            const int column = first_column + 128 * j;
             if (column >= a.width) continue;
             add(s[j], *reinterpret_cast<const float4*>(a.tails + c * a.part_stride + column));
             const float v[4] = {s[j].x, s[j].y, s[j].z, s[j].w};
@@ -572,26 +572,35 @@ __global__ void __launch_bounds__(kThreads, 4) joined_rows_kernel(const Gradient
     if (first_key[warp] >= 0 && more[warp] <= kShortRun)
         for (int base = 0; base < a.width; base += kBlock) {
             float4 s[kQuads] = {};
-            add_heads(c0 + warp + 1, more[warp], base, s);
-            finish(c0 + warp, first_key[warp], base, s);
+            add_heads(c0 + warp + 1, more[warp], base + lane * 4, s);
+            finish(c0 + warp, first_key[warp], base + lane * 4, s);
         }
     for (int w = 0; w < kWarps; ++w) {
         if (first_key[w] < 0 || more[w] <= kShortRun) continue;
-        const int share = (more[w] + kWarps - 1) / kWarps;
-        const int first = min(more[w], warp * share), count = min(more[w], first + share) - first;
         for (int base = 0; base < a.width; base += kBlock) {
+            // `side` lanes hold a row's columns, so narrow rows have more strands
+            int side = 1;
+            while (side < 32 && side * 4 < a.width - base) side *= 2;
+            const int strands = kThreads / side, strand = threadIdx.x / side;
+            const int share = (more[w] + strands - 1) / strands;
+            const int first = min(more[w], strand * share), count = min(more[w], first + share) - first;
             float4 s[kQuads] = {};
-            add_heads(c0 + w + 1 + first, count, base, s);
+            add_heads(c0 + w + 1 + first, count, base + (lane & (side - 1)) * 4, s);
+            for (int d = side; d < 32; d *= 2)
+#pragma unroll
+                for (int j = 0; j < kQuads; ++j)
+                    add(s[j], make_float4(__shfl_down_sync(0xffffffffu, s[j].x, d), __shfl_down_sync(0xffffffffu, s[j].y, d),
+                                          __shfl_down_sync(0xffffffffu, s[j].z, d), __shfl_down_sync(0xffffffffu, s[j].w, d)));
 #pragma unroll
             for (int j = 0; j < kQuads; ++j) part[warp][lane + 32 * j] = s[j];
             __syncthreads();
-            if (warp == 0) {
+            if (warp == 0 && lane < side) {
 #pragma unroll
                 for (int j = 0; j < kQuads; ++j) {
                     s[j] = part[0][lane + 32 * j];
                     for (int x = 1; x < kWarps; ++x) add(s[j], part[x][lane + 32 * j]);
                 }
-                finish(c0 + w, first_key[w], base, s);
+                finish(c0 + w, first_key[w], base + lane * 4, s);
             }
             __syncthreads();
         }
