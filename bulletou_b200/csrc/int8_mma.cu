@@ -12,7 +12,13 @@
 // per SM is the limit of a 128 x 256 tile.  Persistent; the 512 TMEM columns
 // hold two accumulators, so a tile's epilogue runs under the next tile's MMAs.
 // 16384 x 4096 x 4096: 165 us, 3.3 POP/s, the tensor pipe busy in 94 % of the
-// cycles at the clock that the power limit leaves.
+// cycles at the clock that the power limit leaves.  Where k is short the epilogue
+// is the bound, by the shared memory that it shares with the operands: results
+// staged as they are stored and fetched from there by TMA, eight warps for them
+// and five stages: 8192 x 1024 x 4096 with bf16 results 33 us and f32 43, where
+// four warps that staged f32 and stored it themselves took 43 and 47 (lanes
+// that store their own rows 44 and 74).  Six stages and four such warps take 35
+// and 47; with k = 4096 they are equal.
 //
 // int8_tile_kernel, where there are too few 256 x 256 tiles for the SMs: one
 // 128 x 64 tile for each CTA, with k cut over a cluster of up to four CTAs where
@@ -333,23 +339,58 @@ __global__ void __launch_bounds__(128) int8_tile_kernel(const __grid_constant__ 
 }
 
 // ------------------------------------------------------------------ a pair of CTAs on 256 x 256 tiles
+// The lane's row of a block that leaves by TMA, columns h .. h + 31: 16-byte units
+// in the 128-byte swizzle, which keeps 8 lanes of a store on different banks.
+template <typename Out>
+__device__ __forceinline__ void stage_row(uint8_t* stage, int h, const float* v) {
+    constexpr int kVec = 16 / sizeof(Out);
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int c = 0; c < 32; c += kVec) {
+        uint4 unit;
+        if constexpr (sizeof(Out) == 4) {
+            unit = make_uint4(__float_as_uint(v[c]), __float_as_uint(v[c + 1]), __float_as_uint(v[c + 2]), __float_as_uint(v[c + 3]));
+        } else {
+            uint32_t* const p = reinterpret_cast<uint32_t*>(&unit);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __nv_bfloat162 b = __floats2bfloat162_rn(v[c + 2 * i], v[c + 2 * i + 1]);
+                p[i] = *reinterpret_cast<const uint32_t*>(&b);
+            }
+        }
+        *reinterpret_cast<uint4*>(stage + lane * 128 + (((h + c) / kVec) ^ (lane & 7)) * 16) = unit;
+    }
+}
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n cp.async.bulk.commit_group;" ::"l"(
+            reinterpret_cast<uint64_t>(map)),
+        "r"(x), "r"(y), "r"(src)
+        : "memory");
+}
+__device__ __forceinline__ void wait_for_stores_to_be_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+
 constexpr int kPairN = 256;
-constexpr int kPairStages = 6;
+constexpr int kPairStages = 5;
 constexpr uint32_t kPairStageBytes = 2 * kABytes;  // 128 rows of q, 128 rows of w
-constexpr int kPairThreads = 192;                  // TMA, MMA, 4 x epilogue
+constexpr int kEpilogueWarps = 8;                  // two for each quarter of the TMEM lanes, half of the columns each
+constexpr int kPairThreads = 64 + 32 * kEpilogueWarps;  // TMA, MMA, epilogue
+constexpr int kWarpCols = kPairN * 4 / kEpilogueWarps;
+constexpr uint32_t kWarpStaging = 5 * 1024;        // of an epilogue warp: 32 rows of 128 bytes, or of 32 + kStagePad floats
 constexpr int kGroupM = 8;                         // tiles of rows that run next to one another, for L2
-constexpr uint32_t kPairSmem = kPairStages * kPairStageBytes + 4 * 32 * (32 + kStagePad) * 4 + 2 * kPairN * 4 + 256 + 1024;
+constexpr uint32_t kPairSmem = kPairStages * kPairStageBytes + kEpilogueWarps * kWarpStaging + 2 * kPairN * 4 + 256 + 1024;
 
 template <typename Out>
 __global__ void __launch_bounds__(kPairThreads, 1)
     int8_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_w,
-                     const ProductArgs a, bool vector_ok) {
+                     const __grid_constant__ CUtensorMap map_out, const ProductArgs a, bool out_by_tma) {
     extern __shared__ uint8_t raw[];
     const uint32_t raw_addr = smem_u32(raw);
     const uint32_t base = (raw_addr + 1023u) & ~1023u;
     uint8_t* const stages = raw + (base - raw_addr);
-    float* const staging = reinterpret_cast<float*>(stages + kPairStages * kPairStageBytes);
-    float* const col_scale = staging + 4 * 32 * (32 + kStagePad);
+    uint8_t* const staging = stages + kPairStages * kPairStageBytes;
+    float* const col_scale = reinterpret_cast<float*>(staging + kEpilogueWarps * kWarpStaging);
     float* const col_bias = col_scale + kPairN;
     uint64_t* const bars = reinterpret_cast<uint64_t*>(col_bias + kPairN);
     const uint32_t full = smem_u32(bars), empty = full + 8 * kPairStages, tile_full = empty + 8 * kPairStages,
@@ -365,7 +406,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(tile_full + 8 * b, 1);
-            mbar_init(tile_empty + 8 * b, 8);  // 4 epilogue warps in each CTA
+            mbar_init(tile_empty + 8 * b, 2 * kEpilogueWarps);  // of both CTAs
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -440,18 +481,21 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
     } else if (warp >= 2) {
         const int quarter = warp & 3;  // the TMEM lanes this warp may read
-        float* const stage = staging + quarter * 32 * (32 + kStagePad);
+        const int first_col = (warp - 2) / 4 * kWarpCols;
+        uint8_t* const stage = staging + (warp - 2) * kWarpStaging;
+        const uint32_t stage_address = smem_u32(stage);
+        constexpr int kBlockCols = 128 / sizeof(Out);  // a block that leaves by TMA: 32 rows of 128 bytes
         for (int t = first_tile, n = 0; t < tiles; t += step, ++n) {
             const int b = n & 1;
             int row0, col0;
             place(t, row0, col0);
-            asm volatile("bar.sync 1, 128;" ::: "memory");  // the last tile's scales are read
-            for (int c = tid - 64; c < kPairN; c += 128) {
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogueWarps) : "memory");  // the last tile's scales are read
+            for (int c = tid - 64; c < kPairN; c += 32 * kEpilogueWarps) {
                 const bool in = col0 + c < a.n;
                 col_scale[c] = in ? a.w_scales[col0 + c] : 0.0f;
                 col_bias[c] = in && a.bias != nullptr ? a.bias[col0 + c] : 0.0f;
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogueWarps) : "memory");
             const int row = row0 + quarter * 32 + lane;
             const float own_scale = row < a.m ? a.scales[row] : 0.0f;
             good = good && mbar_wait(tile_full + 8 * b, (n / 2) & 1);
@@ -460,12 +504,26 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             const float row_scale = good ? own_scale : NAN;
             const uint32_t lanes = tmem + b * kPairN + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll 1
-            for (int c0 = 0; c0 < kPairN && col0 + c0 < a.n; c0 += 32) {
+            for (int c0 = first_col; c0 < first_col + kWarpCols && col0 + c0 < a.n; c0 += out_by_tma ? kBlockCols : 32) {
                 uint32_t sum[32];
                 float v[32];
-                tmem_ld32(lanes + c0, sum);
-                results(sum, row_scale, col_scale + c0, col_bias + c0, v);
-                store_block<Out>(stage, v, a, row0 + quarter * 32, col0 + c0, vector_ok);
+                if (!out_by_tma) {
+                    tmem_ld32(lanes + c0, sum);
+                    results(sum, row_scale, col_scale + c0, col_bias + c0, v);
+                    store_block<Out>(reinterpret_cast<float*>(stage), v, a, row0 + quarter * 32, col0 + c0, false);
+                    continue;
+                }
+                wait_for_stores_to_be_read();  // of the block before
+                __syncwarp();
+#pragma unroll
+                for (int h = 0; h < kBlockCols; h += 32) {
+                    tmem_ld32(lanes + c0 + h, sum);
+                    results(sum, row_scale, col_scale + c0 + h, col_bias + c0 + h, v);
+                    stage_row<Out>(stage, h, v);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0 && row0 + quarter * 32 < a.m) tma_store_2d(&map_out, stage_address, col0 + c0, row0 + quarter * 32);
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
@@ -474,6 +532,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                                  map_rank(tile_empty + 8 * b, 0))
                              : "memory");
         }
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -495,6 +554,23 @@ int operand_map(CUtensorMap* map, const int8_t* data, int rows, int k, size_t st
     const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(data), dims, strides, box, estride,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail_messagef("cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+    return 0;
+}
+
+// The results in blocks of 32 rows x 128 bytes; the columns and rows beyond are not written.
+template <typename Out>
+int result_map(CUtensorMap* map, const ProductArgs& a) {
+    const EncodeTiled fn = encode_tiled();
+    if (fn == nullptr) return fail_message("cuTensorMapEncodeTiled is unavailable");
+    const size_t stride = a.m > 1 ? a.out_stride * sizeof(Out) : (a.n * sizeof(Out) + 15) / 16 * 16;  // of one row: any
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.n), static_cast<cuuint64_t>(a.m)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride)};
+    const cuuint32_t box[2] = {128 / sizeof(Out), 32};
+    const cuuint32_t estride[2] = {1, 1};
+    const CUresult r = fn(map, sizeof(Out) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.out, dims,
+                          strides, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail_messagef("cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
     return 0;
 }
@@ -525,11 +601,12 @@ int launch_tiles(BulletOuCudaCppContext* ctx, const ProductArgs& a, bool vector_
 
 template <typename Out>
 int launch_pairs(BulletOuCudaCppContext* ctx, const ProductArgs& a, int tiles, bool vector_ok, bool early) {
-    CUtensorMap q, w;
+    CUtensorMap q, w, out{};
     if (operand_map(&q, a.q, a.m, a.k, a.q_stride, kTileM) != 0 || operand_map(&w, a.w, a.n, a.k, a.w_stride, kTileM) != 0)
         return -1;
+    if (vector_ok && result_map<Out>(&out, a) != 0) return -1;
     const LaunchShape shape{dim3(2 * std::min(tiles, ctx->sm_count / 2)), kPairThreads, kPairSmem, 2, early};
-    return launch_kernel(ctx, "int8 product launch", int8_pair_kernel<Out>, shape, q, w, a, vector_ok);
+    return launch_kernel(ctx, "int8 product launch", int8_pair_kernel<Out>, shape, q, w, out, a, vector_ok);
 }
 
 template <typename Out>
