@@ -14,8 +14,8 @@
 // 16384 x 4096 x 4096: 165 us, 3.3 POP/s, the tensor pipe busy in 94 % of the
 // cycles at the clock that the power limit leaves.  Where k is short the epilogue
 // is the bound, by the shared memory that it shares with the operands: results
-// staged as they are stored and fetched from there by TMA, eight warps for them
-// and five stages: 8192 x 1024 x 4096 with bf16 results 33 us and f32 43, where
+// staged as they are stored and fetched from there by TMA, with eight warps for
+// them and five stages: 8192 x 1024 x 4096 with bf16 results 33 us and f32 43, where
 // four warps that staged f32 and stored it themselves took 43 and 47 (lanes
 // that store their own rows 44 and 74).  Six stages and four such warps take 35
 // and 47; with k = 4096 they are equal.
@@ -372,19 +372,26 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t sr
 __device__ __forceinline__ void wait_for_stores_to_be_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 
 constexpr int kPairN = 256;
-constexpr int kPairStages = 5;
 constexpr uint32_t kPairStageBytes = 2 * kABytes;  // 128 rows of q, 128 rows of w
-constexpr int kEpilogueWarps = 8;                  // two for each quarter of the TMEM lanes, half of the columns each
-constexpr int kPairThreads = 64 + 32 * kEpilogueWarps;  // TMA, MMA, epilogue
-constexpr int kWarpCols = kPairN * 4 / kEpilogueWarps;
 constexpr uint32_t kWarpStaging = 5 * 1024;        // of an epilogue warp: 32 rows of 128 bytes, or of 32 + kStagePad floats
 constexpr int kGroupM = 8;                         // tiles of rows that run next to one another, for L2
-constexpr uint32_t kPairSmem = kPairStages * kPairStageBytes + kEpilogueWarps * kWarpStaging + 2 * kPairN * 4 + 256 + 1024;
+// kManyLong, for tiles of long k that come one after the other: as many stages as
+// fit, and the four epilogue warps that the MMAs hide; otherwise eight.
+template <bool kManyLong>
+struct PairShape {
+    static constexpr int kStages = kManyLong ? 6 : 5;
+    static constexpr int kEpilogueWarps = kManyLong ? 4 : 8;  // for each quarter of the TMEM lanes one, or two with half of the columns each
+    static constexpr int kWarpCols = kPairN * 4 / kEpilogueWarps;
+    static constexpr int kThreads = 64 + 32 * kEpilogueWarps;  // TMA, MMA, epilogue
+    static constexpr uint32_t kSmem = kStages * kPairStageBytes + kEpilogueWarps * kWarpStaging + 2 * kPairN * 4 + 256 + 1024;
+};
 
-template <typename Out>
-__global__ void __launch_bounds__(kPairThreads, 1)
+template <bool kManyLong, typename Out>
+__global__ void __launch_bounds__(PairShape<kManyLong>::kThreads, 1)
     int8_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_w,
                      const __grid_constant__ CUtensorMap map_out, const ProductArgs a, bool out_by_tma) {
+    using S = PairShape<kManyLong>;
+    constexpr int kPairStages = S::kStages, kEpilogueWarps = S::kEpilogueWarps, kWarpCols = S::kWarpCols;
     extern __shared__ uint8_t raw[];
     const uint32_t raw_addr = smem_u32(raw);
     const uint32_t base = (raw_addr + 1023u) & ~1023u;
@@ -504,17 +511,21 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             const float row_scale = good ? own_scale : NAN;
             const uint32_t lanes = tmem + b * kPairN + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll 1
-            for (int c0 = first_col; c0 < first_col + kWarpCols && col0 + c0 < a.n; c0 += out_by_tma ? kBlockCols : 32) {
+            for (int c0 = first_col; c0 < first_col + kWarpCols && col0 + c0 < a.n; c0 += kBlockCols) {
                 uint32_t sum[32];
                 float v[32];
-                if (!out_by_tma) {
-                    tmem_ld32(lanes + c0, sum);
-                    results(sum, row_scale, col_scale + c0, col_bias + c0, v);
-                    store_block<Out>(reinterpret_cast<float*>(stage), v, a, row0 + quarter * 32, col0 + c0, false);
-                    continue;
-                }
                 wait_for_stores_to_be_read();  // of the block before
                 __syncwarp();
+                // a TMA store writes whole 16-byte units, so the last columns go by it only where they fill theirs
+                if (!out_by_tma || (col0 + c0 + kBlockCols > a.n && a.n % (16 / sizeof(Out)) != 0)) {
+#pragma unroll 1
+                    for (int h = 0; h < kBlockCols && col0 + c0 + h < a.n; h += 32) {
+                        tmem_ld32(lanes + c0 + h, sum);
+                        results(sum, row_scale, col_scale + c0 + h, col_bias + c0 + h, v);
+                        store_block<Out>(reinterpret_cast<float*>(stage), v, a, row0 + quarter * 32, col0 + c0 + h, out_by_tma);
+                    }
+                    continue;
+                }
 #pragma unroll
                 for (int h = 0; h < kBlockCols; h += 32) {
                     tmem_ld32(lanes + c0 + h, sum);
@@ -558,7 +569,7 @@ int operand_map(CUtensorMap* map, const int8_t* data, int rows, int k, size_t st
     return 0;
 }
 
-// The results in blocks of 32 rows x 128 bytes; the columns and rows beyond are not written.
+// The results in blocks of 32 rows x 128 bytes; the rows and 16-byte units beyond are not written.
 template <typename Out>
 int result_map(CUtensorMap* map, const ProductArgs& a) {
     const EncodeTiled fn = encode_tiled();
@@ -599,14 +610,14 @@ int launch_tiles(BulletOuCudaCppContext* ctx, const ProductArgs& a, bool vector_
                                            : launch_tiles<false, Out>(ctx, a, tiles, splits, vector_ok, early, weights_ready);
 }
 
-template <typename Out>
+template <bool kManyLong, typename Out>
 int launch_pairs(BulletOuCudaCppContext* ctx, const ProductArgs& a, int tiles, bool vector_ok, bool early) {
     CUtensorMap q, w, out{};
     if (operand_map(&q, a.q, a.m, a.k, a.q_stride, kTileM) != 0 || operand_map(&w, a.w, a.n, a.k, a.w_stride, kTileM) != 0)
         return -1;
     if (vector_ok && result_map<Out>(&out, a) != 0) return -1;
-    const LaunchShape shape{dim3(2 * std::min(tiles, ctx->sm_count / 2)), kPairThreads, kPairSmem, 2, early};
-    return launch_kernel(ctx, "int8 product launch", int8_pair_kernel<Out>, shape, q, w, out, a, vector_ok);
+    const LaunchShape shape{dim3(2 * std::min(tiles, ctx->sm_count / 2)), PairShape<kManyLong>::kThreads, PairShape<kManyLong>::kSmem, 2, early};
+    return launch_kernel(ctx, "int8 product launch", int8_pair_kernel<kManyLong, Out>, shape, q, w, out, a, vector_ok);
 }
 
 template <typename Out>
@@ -619,7 +630,10 @@ int launch_typed(BulletOuCudaCppContext* ctx, const ProductArgs& a, bool early, 
     const int64_t pairs = static_cast<int64_t>((a.m + 255) / 256) * ((a.n + 255) / 256);
     const int64_t singles = static_cast<int64_t>((a.m + 127) / 128) * ((a.n + 63) / 64);
     if (a.n > 64 && singles > 2 * ctx->sm_count && pairs <= INT32_MAX)
-        return launch_pairs<Out>(ctx, a, static_cast<int>(pairs), vector_ok, early);
+        // 16384 x 4096 x 4096 takes 202 us with six stages, 206 with five; 4096 x 8192 x
+        // 2048 (two tiles for each pair) 67 and 66, 8192 x 1024 x 4096 44 and 41
+        return a.k >= 2048 && pairs >= 4 * ctx->sm_count / 2 ? launch_pairs<true, Out>(ctx, a, static_cast<int>(pairs), vector_ok, early)
+                                                             : launch_pairs<false, Out>(ctx, a, static_cast<int>(pairs), vector_ok, early);
     return launch_tiles<Out>(ctx, a, vector_ok, early, weights_ready);
 }
 

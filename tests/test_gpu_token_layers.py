@@ -503,6 +503,22 @@ def test_int8_rows_of_zeros_infinities_and_nan(tctx):
     assert (y[[0, 3, 4]] == bias).all() and np.isnan(y[1:3]).all() and np.isfinite(y[5]).all()
 
 
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("pad", [0, 8, 1])  # results that leave in blocks, into padded rows, and element by element
+def test_int8_of_many_tiles_of_long_rows(tctx, t, pad):
+    rows, inner, outer = 4700, 2100, 3990
+    g = torch.Generator(device="cuda").manual_seed(7)
+    q = torch.randint(-127, 128, (rows, inner), generator=g, device="cuda", dtype=torch.int8)
+    w = torch.randint(-127, 128, (outer, inner), generator=g, device="cuda", dtype=torch.int8)
+    scales, ws = torch.rand(rows, generator=g, device="cuda"), torch.rand(outer, generator=g, device="cuda")
+    wide = torch.full((rows, outer + 10 + pad), 9.0, device="cuda", dtype=kind(t))
+    bo.int8_matmul(tctx, q, scales, w, ws, wide[:, :outer])
+    assert (wide[:, outer:] == 9.0).all()
+    want = (q.double() @ w.double().T) * scales.double()[:, None] * ws.double()
+    # the sum's, the scales' product's and the result's rounding, and bf16's
+    assert ((wide[:, :outer].double() - want).abs() <= (4 * U32 + (2.0 ** -8 if t == BF16 else 0.0)) * want.abs()).all()
+
+
 def test_int8_beyond_32_bit_offsets(tctx):
     stride = 2**30 + 16  # row 2 of the weights starts past 2^31 bytes
     memory = torch.zeros(2 * stride + 64, device="cuda", dtype=torch.int8)
