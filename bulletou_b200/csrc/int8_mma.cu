@@ -18,7 +18,7 @@
 // them and five stages: 8192 x 1024 x 4096 with bf16 results 33 us and f32 43, where
 // four warps that staged f32 and stored it themselves took 43 and 47 (lanes
 // that store their own rows 44 and 74).  Six stages and four such warps take 35
-// and 47; with k = 4096 they are equal.
+// and 47; for many tiles of long k they are ahead by 4 %.
 //
 // int8_tile_kernel, where there are too few 256 x 256 tiles for the SMs: one
 // 128 x 64 tile for each CTA, with k cut over a cluster of up to four CTAs where
@@ -630,7 +630,7 @@ int launch_typed(BulletOuCudaCppContext* ctx, const ProductArgs& a, bool early, 
     const int64_t pairs = static_cast<int64_t>((a.m + 255) / 256) * ((a.n + 255) / 256);
     const int64_t singles = static_cast<int64_t>((a.m + 127) / 128) * ((a.n + 63) / 64);
     if (a.n > 64 && singles > 2 * ctx->sm_count && pairs <= INT32_MAX)
-        // 16384 x 4096 x 4096 takes 202 us with six stages, 206 with five; 4096 x 8192 x
+        // 16384 x 4096 x 4096 takes 197 us with six stages, 206 with five; 4096 x 8192 x
         // 2048 (two tiles for each pair) 67 and 66, 8192 x 1024 x 4096 44 and 41
         return a.k >= 2048 && pairs >= 4 * ctx->sm_count / 2 ? launch_pairs<true, Out>(ctx, a, static_cast<int>(pairs), vector_ok, early)
                                                              : launch_pairs<false, Out>(ctx, a, static_cast<int>(pairs), vector_ok, early);
