@@ -626,10 +626,11 @@ int launch_typed(BulletOuCudaCppContext* ctx, const ProductArgs& a, bool early, 
     // Single tiles while they all run at once, two on an SM: 512 x 4096 x 4096 (256 of
     // them) takes 15 us, in pairs 18; 8192 x 640 x 256 (256) 6.0 and 9.0.  Beyond,
     // pairs, unless most of their columns are empty: 16384 x 2560 x 256 (512) takes
-    // 13 us in pairs, 17 singly, but 65536 x 640 x 64 16 and 10.
+    // 13 us in pairs, 17 singly, but 65536 x 640 x 64 16 and 10.  Without inner columns
+    // there is no MMA whose end a pair could wait for; a single tile takes its sums as zeros.
     const int64_t pairs = static_cast<int64_t>((a.m + 255) / 256) * ((a.n + 255) / 256);
     const int64_t singles = static_cast<int64_t>((a.m + 127) / 128) * ((a.n + 63) / 64);
-    if (a.n > 64 && singles > 2 * ctx->sm_count && pairs <= INT32_MAX)
+    if (a.k > 0 && a.n > 64 && singles > 2 * ctx->sm_count && pairs <= INT32_MAX)
         // 16384 x 4096 x 4096 takes 197 us with six stages, 206 with five; 4096 x 8192 x
         // 2048 (two tiles for each pair) 67 and 66, 8192 x 1024 x 4096 44 and 41
         return a.k >= 2048 && pairs >= 4 * ctx->sm_count / 2 ? launch_pairs<true, Out>(ctx, a, static_cast<int>(pairs), vector_ok, early)
