@@ -19,11 +19,14 @@
 
 namespace bou {
 
-// Grow-only device scratch owned by a context.  Never shrinks during a run, so
-// buffers handed to an enqueued kernel stay valid until the context dies.
+// Grow-only device scratch owned by a context.  A block that a larger call
+// outgrows is freed once the stream is done with it, unless a graph was captured
+// with it: the graph's kernels hold its address, so it stays until the context
+// dies.
 struct Scratch {
     void* ptr = nullptr;
     size_t bytes = 0;
+    bool captured = false;  // handed out while the stream was capturing
 };
 
 }  // namespace bou
@@ -35,6 +38,7 @@ struct BulletOuCudaCppContext {
     int sm_count = 148;
     // Named scratch slots; see scratch_slot in runtime.cu.
     bou::Scratch scratch[32];
+    std::vector<bou::Scratch> outgrown;  // blocks that captured graphs hold
     // Dense QAT mode between bulletou_dense_qat_begin / _end (the reference's
     // context flags, cu:9356-9382): integer L1 / L2 / L3 in the SFNN entries.
     bool dense_qat = false;

@@ -6,6 +6,7 @@
 #include <cstring>
 #include <cfloat>
 #include <algorithm>
+#include <new>
 
 #include "common.cuh"
 
@@ -90,8 +91,22 @@ int scratch_slot(BulletOuCudaCppContext* ctx, int slot, size_t bytes, void** out
         return fail_message("internal: scratch slot out of range");
     Scratch& s = ctx->scratch[slot];
     if (bytes == 0) bytes = 256;
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(ctx->stream, &status) != cudaSuccess) {
+        cudaGetLastError();  // the default stream while another one captures
+        status = cudaStreamCaptureStatusNone;
+    }
+    const bool capturing = status != cudaStreamCaptureStatusNone;
     if (s.bytes < bytes) {
         cudaError_t st;
+        if (s.ptr != nullptr && (s.captured || capturing)) {
+            try {
+                ctx->outgrown.push_back(s);
+            } catch (const std::bad_alloc&) {
+                return fail_messagef("%s: out of host memory", label);
+            }
+            s = Scratch{};
+        }
         if (s.ptr != nullptr) {
             st = cudaStreamSynchronize(ctx->stream);
             if (st != cudaSuccess) return fail(label, st);
@@ -108,6 +123,7 @@ int scratch_slot(BulletOuCudaCppContext* ctx, int slot, size_t bytes, void** out
         }
         s.bytes = rounded;
     }
+    s.captured = s.captured || capturing;
     *out = s.ptr;
     return 0;
 }
@@ -347,14 +363,16 @@ int bulletou_cuda_cpp_context_destroy(BulletOuCudaCppContext* ctx) {
     }
     if (ctx->stream != nullptr) cudaStreamSynchronize(ctx->stream);
     int rc = 0;
-    for (auto& s : ctx->scratch) {
+    auto release = [&](Scratch& s) {
         if (s.ptr != nullptr) {
             st = cudaFree(s.ptr);
             if (st != cudaSuccess && rc == 0) rc = fail("cudaFree context scratch", st);
             s.ptr = nullptr;
             s.bytes = 0;
         }
-    }
+    };
+    for (auto& s : ctx->scratch) release(s);
+    for (auto& s : ctx->outgrown) release(s);
     for (auto e : ctx->prof_events) cudaEventDestroy(e);
     ctx->prof_events.clear();
     if (ctx->owns_stream && ctx->stream != nullptr) {
@@ -429,6 +447,7 @@ int bulletou_b200_context_scratch_bytes(const BulletOuCudaCppContext* ctx, size_
     if (out == nullptr) return fail_message("context_scratch_bytes: output must not be null");
     size_t total = 0;
     for (const Scratch& s : ctx->scratch) total += s.bytes;
+    for (const Scratch& s : ctx->outgrown) total += s.bytes;
     *out = total;
     return ok();
 }

@@ -99,7 +99,9 @@ int bulletou_b200_profile_end(BulletOuCudaCppContext* ctx, float* ms_out, size_t
 
 /* Device bytes the context currently holds in its grow-only scratch slots
  * (no counterpart in the reference; diagnostics).  The slots are allocated on
- * first use by the entries that need scratch and freed at context destroy. */
+ * first use by the entries that need scratch and freed at context destroy; a
+ * slot that has grown counts once, and once more for each outgrown block that a
+ * captured graph holds. */
 int bulletou_b200_context_scratch_bytes(const BulletOuCudaCppContext* ctx, size_t* out);
 
 /* Data-parallel overlap (no counterpart in the reference): the next SFNN
@@ -572,7 +574,10 @@ int bulletou_b200_hcpe_to_psv_device(BulletOuCudaCppContext* ctx, const BulletOu
  * balance loss, and the 8-bit product that evaluates a dense layer.  They work
  * on matrices in device memory of the context's device, on the context's
  * stream, and allocate nothing but context scratch, which only grows (so a
- * call whose sizes were seen before can be captured in a graph).  All sums are
+ * call whose sizes were seen before can be captured in a graph).  A graph keeps
+ * the scratch that it was captured with until the context is destroyed, however
+ * large later calls are; it shares that scratch with them, so it is launched on
+ * the context that it was captured on, and not after its end.  All sums are
  * held in f32 or in integers; for the same inputs the results are the same
  * bits from call to call. */
 #define BULLETOU_B200_TYPE_F32 0

@@ -40,3 +40,68 @@ def test_int8_of_no_inner_columns_is_the_bias(tctx, rows, outer, t, bias):
     out.fill_(9.0)
     bo.int8_matmul(tctx, torch.empty(rows, 0, device="cuda", dtype=torch.int8), scales, w, ws, out, bias=b)
     assert torch.equal(out, want)
+
+
+# --------------------------------------------------------------------------- graphs
+def scratch_bytes(ctx):
+    import ctypes
+
+    n = ctypes.c_size_t(0)
+    ctx.lib.call("bulletou_b200_context_scratch_bytes", ctx.as_ptr(), ctypes.byref(n))
+    return n.value
+
+
+class Calls:
+    """The three operators that use scratch, on tensors for up to `n` tokens."""
+
+    def __init__(self, n, seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        self.n, self.g = n, g
+        self.tokens = torch.randint(-1, 700, (n,), generator=g, device="cuda", dtype=torch.int32)
+        self.grad = torch.randn(n, 40, generator=g, device="cuda")
+        self.logits = torch.randn(n, 9, generator=g, device="cuda")
+        self.weights = torch.randint(-127, 128, (70, 40), generator=g, device="cuda", dtype=torch.int8)
+        self.scales = torch.rand(70, generator=g, device="cuda")
+        self.out = {"table": torch.zeros(700, 40, device="cuda"), "experts": torch.zeros(n, 2, device="cuda", dtype=torch.int32),
+                    "gates": torch.zeros(n, 2, device="cuda"), "counts": torch.zeros(10, device="cuda", dtype=torch.int32),
+                    "mean": torch.zeros(9, device="cuda"), "loss": torch.zeros(1, device="cuda"), "y": torch.zeros(n, 70, device="cuda")}
+
+    def run(self, ctx):
+        o = self.out
+        bo.embedding_backward(ctx, self.tokens, self.grad, o["table"])
+        bo.router_forward(ctx, self.logits, o["experts"], o["gates"], o["counts"], o["mean"], o["loss"], balance=0.1)
+        bo.int8_linear(ctx, self.grad, self.weights, self.scales, o["y"])
+
+
+def test_graph_replays_after_larger_calls():
+    """Scratch that a graph was captured with stays its own when larger calls outgrow it."""
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        ctx, plain = (bo.Context(0, stream=stream.cuda_stream) for _ in range(2))
+        small, sizes = Calls(6000, 1), (20000, 90000)
+        small.run(ctx)
+        held = scratch_bytes(ctx)
+        bo.GraphExec.begin_capture(ctx)
+        small.run(ctx)
+        graph = bo.GraphExec.end_capture(ctx)
+        for n in sizes:
+            large = Calls(n, n)
+            large.run(ctx)
+            large.run(plain)
+            # the captured blocks are kept once; those of the first larger size are not
+            assert scratch_bytes(ctx) == scratch_bytes(plain) + held
+            junk = torch.full((1 << 26,), float("nan"), device="cuda")  # whatever was freed holds something else by now
+            small.tokens.copy_(torch.randint(-1, 700, (6000,), generator=small.g, device="cuda", dtype=torch.int32))
+            small.grad.normal_(generator=small.g)
+            small.logits.normal_(generator=small.g)
+            small.run(ctx)
+            want = {k: v.clone() for k, v in small.out.items()}
+            for v in small.out.values():
+                v.fill_(3)
+            graph.launch(ctx)
+            stream.synchronize()
+            assert all(torch.equal(want[k], small.out[k]) for k in want)
+            del junk
+        graph.close()
+        ctx.close()
+        plain.close()
