@@ -240,7 +240,9 @@ __global__ void __launch_bounds__(kThreads, 4) quantize_kernel(const QuantizeArg
 // takes 3.8 us, which is the launch and one chain of latencies; two rows of 4096
 // x 4096 8.2 us against 9.2 on the tensor cores, four were 16 against 9.
 constexpr int kFewRows = 2;
-constexpr size_t kFewRowsBytes = 48 * 1024;  // shared memory for the rows
+// Shared memory for the rows: what a launch has without asking for more, less the
+// kernel's own row maxima.
+constexpr size_t kFewRowsBytes = 48 * 1024 - kWarps * kFewRows * sizeof(float);
 
 struct FewRowsArgs {
     ProductArgs p;

@@ -42,6 +42,27 @@ def test_int8_of_no_inner_columns_is_the_bias(tctx, rows, outer, t, bias):
     assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("rows", [1, 2, 3])
+@pytest.mark.parametrize("inner", [24543, 24544, 24545, 24560, 24561, 24576, 24577, 49152, 49153])
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_int8_around_the_shared_memory_of_few_rows(tctx, rows, inner, t):
+    """Two rows fill a launch's 48 KB of shared memory, with the kernel's own 64 bytes, at 24544 columns."""
+    rng = np.random.default_rng(inner + rows)
+    x = cuda(rng.standard_normal((rows, inner)).astype(np.float32))
+    w = rng.integers(-128, 128, (11, inner)).astype(np.int8)
+    ws = (0.01 * (0.5 + rng.random(11))).astype(np.float32)
+    want_q, want_s = quantize_rows(x.cpu().numpy())
+    want, size = int8_product(want_q, want_s, w, ws, None)
+    # the scales' product, its product with the sum, the sum's conversion and the last operation; bf16's
+    bound = 4 * U32 * (size + np.abs(want)) + (UBF if t == torch.bfloat16 else 0.0) * np.abs(want)
+    out = torch.full((rows, 11), 9.0, device="cuda", dtype=t)
+    bo.int8_linear(tctx, x, cuda(w), cuda(ws), out)
+    assert (np.abs(out.double().cpu().numpy() - want) <= bound).all()
+    out.fill_(9.0)
+    bo.int8_matmul(tctx, cuda(want_q), cuda(want_s), cuda(w), cuda(ws), out)
+    assert (np.abs(out.double().cpu().numpy() - want) <= bound).all()
+
+
 # --------------------------------------------------------------------------- graphs
 def scratch_bytes(ctx):
     import ctypes
