@@ -135,7 +135,7 @@ struct Group {
                 if (offset & (4 * step)) w[i] = w[i + step];
 #pragma unroll
         for (int i = 0; i < 4 * kUnits; ++i) {
-            const int left = (cols - c) * static_cast<int>(sizeof(T)) - 4 * i;  // bytes of the row from here on
+            const int left = min(cols - c, kGroup) * static_cast<int>(sizeof(T)) - 4 * i;  // bytes of the row from here on, in this group
             const uint32_t word = sizeof(T) == 2 ? __funnelshift_r(w[i], w[i + 1], (offset & 2) * 8) : w[i];
             reinterpret_cast<uint32_t*>(raw)[i] = left >= 4 ? word : left > 0 ? word & 0xffffu : 0;
         }

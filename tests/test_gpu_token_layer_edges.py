@@ -63,6 +63,21 @@ def test_int8_around_the_shared_memory_of_few_rows(tctx, rows, inner, t):
     assert (np.abs(out.double().cpu().numpy() - want) <= bound).all()
 
 
+@pytest.mark.parametrize("t,cols", [(torch.float32, 2**29 + 9), (torch.bfloat16, 2**30 + 9)])
+@pytest.mark.parametrize("shift", [0, 1])  # a row on 16 bytes and off them
+def test_quantise_rows_of_more_than_31_bits_of_bytes(tctx, t, cols, shift):
+    memory = torch.zeros(cols + shift, device="cuda", dtype=t)
+    x = memory[shift:].view(1, cols)
+    at = torch.tensor([0, 1, 17, 4095, 4096, 8191, 2**20 + 3, 2**28 + 1, cols - 2**20, cols - 17, cols - 1], device="cuda")
+    x[0, at] = torch.linspace(-1.0, 2.0, 11, device="cuda").to(t)
+    q, s = torch.full((1, cols), 5, device="cuda", dtype=torch.int8), torch.zeros(1, device="cuda")
+    bo.int8_quantize_rows(tctx, x, q, s)
+    want_q, want_s = quantize_rows(x[:, at].float().cpu().numpy())  # they hold the largest; the rest are zeros
+    assert np.array_equal(q[:, at].cpu().numpy(), want_q) and s.item() == want_s[0]
+    q[0, at] = 0
+    assert not q.view(-1)[: cols // 8 * 8].view(torch.int64).any() and not q[0, cols // 8 * 8 :].any()
+
+
 # --------------------------------------------------------------------------- graphs
 def scratch_bytes(ctx):
     import ctypes
