@@ -83,6 +83,7 @@ __global__ void __launch_bounds__(kThreads) repack_kernel(const RepackArgs a) { 
 // ------------------------------------------------------------------ quantisation
 struct QuantizeArgs {
     const void* x;
+    const void* x_end;  // past the last row's last element
     size_t x_stride;
     int8_t* q;
     size_t q_stride;
@@ -100,6 +101,11 @@ constexpr int kGroup = 16;  // columns that a thread takes together: a 16-byte s
 template <typename T>
 struct Group {
     uint4 raw[kGroup * sizeof(T) / 16];
+    __device__ __forceinline__ void load_elements(const T* x, int c, int cols) {
+        T* e = reinterpret_cast<T*>(raw);
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) e[i] = c + i < cols ? x[c + i] : from_f32<T>(0.0f);
+    }
     // A row that starts on 16 bytes.
     __device__ __forceinline__ void load(const T* x, int c, int cols) {
         constexpr int kUnits = kGroup * sizeof(T) / 16;
@@ -107,20 +113,23 @@ struct Group {
 #pragma unroll
             for (int i = 0; i < kUnits; ++i) raw[i] = __ldcs(reinterpret_cast<const uint4*>(x + c) + i);
         } else {
-            T* e = reinterpret_cast<T*>(raw);
-#pragma unroll
-            for (int i = 0; i < kGroup; ++i) e[i] = c + i < cols ? x[c + i] : from_f32<T>(0.0f);
+            load_elements(x, c, cols);
         }
     }
     // The same of a row at any alignment: the aligned units that hold the values,
-    // shifted into place; units without a value of the row are not read.  (Loads of
-    // single elements took 31 us for 3373 rows of 5445 bf16, these 23.)
-    __device__ __forceinline__ void load_shifted(const T* x, int c, int cols) {
+    // shifted into place; units without a value of the row are not read.  Where they
+    // begin before the matrix or end after it the values are loaded one by one.
+    // (That took 31 us everywhere for 3373 rows of 5445 bf16, these 23.)
+    __device__ __forceinline__ void load_shifted(const QuantizeArgs& a, const T* x, int c, int cols) {
         constexpr int kUnits = kGroup * sizeof(T) / 16;
         const char* const at = reinterpret_cast<const char*>(x + c);
         const unsigned offset = static_cast<unsigned>(reinterpret_cast<uintptr_t>(at)) & 15;
         const uint4* const from = reinterpret_cast<const uint4*>(at - offset);
         const uint4* const end = reinterpret_cast<const uint4*>(x + cols);
+        if (static_cast<const void*>(from) < a.x || static_cast<const void*>(from + kUnits + 1) > a.x_end) {
+            load_elements(x, c, cols);
+            return;
+        }
         uint32_t w[4 * kUnits + 4];
 #pragma unroll
         for (int i = 0; i <= kUnits; ++i) {
@@ -190,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 4) quantize_kernel(const QuantizeArg
     Group<T> held[kHeld];
     auto load = [&](Group<T>& g, int c, int cols) {
         if constexpr (kAligned) g.load(x, c, cols);
-        else g.load_shifted(x, c, cols);
+        else g.load_shifted(a, x, c, cols);
     };
     float top = 0.0f;
 #pragma unroll
@@ -375,6 +384,7 @@ int quantize(BulletOuCudaCppContext* ctx, const BulletOuB200Matrix& x, int8_t* q
              float* scales, const RepackArgs& weights) {
     QuantizeArgs a{};
     a.x = x.data;
+    a.x_end = static_cast<const char*>(x.data) + (x.cols > 0 ? (x.rows - 1) * (x.rows > 1 ? x.row_stride : 0) + x.cols : 0) * type_bytes(x.type);
     a.x_stride = x.row_stride;
     a.q = q;
     a.q_stride = q_stride;

@@ -63,6 +63,21 @@ def test_int8_around_the_shared_memory_of_few_rows(tctx, rows, inner, t):
     assert (np.abs(out.double().cpu().numpy() - want) <= bound).all()
 
 
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols,gap", [(1, 1, 0), (1, 15, 0), (1, 16, 0), (1, 33, 0), (3, 7, 0), (3, 40, 1), (2, 255, 9), (4, 1031, 3)])
+def test_quantise_rows_that_begin_and_end_inside_16_bytes(tctx, t, rows, cols, gap):
+    """At every alignment, from the first element of the memory to its last; what lies beside the rows is not looked at."""
+    rng = np.random.default_rng(cols)
+    for shift in range(8):
+        memory = torch.full((shift + rows * (cols + gap) - gap,), float("nan"), device="cuda", dtype=t)
+        x = torch.as_strided(memory, (rows, cols), (cols + gap, 1), shift)
+        x.copy_(cuda(rng.standard_normal((rows, cols)).astype(np.float32)))
+        q, s = torch.full((rows, cols), 5, device="cuda", dtype=torch.int8), torch.zeros(rows, device="cuda")
+        bo.int8_quantize_rows(tctx, x, q, s)
+        want_q, want_s = quantize_rows(x.float().cpu().numpy())
+        assert np.array_equal(q.cpu().numpy(), want_q) and np.array_equal(s.cpu().numpy(), want_s)
+
+
 @pytest.mark.parametrize("t,cols", [(torch.float32, 2**29 + 9), (torch.bfloat16, 2**30 + 9)])
 @pytest.mark.parametrize("shift", [0, 1])  # a row on 16 bytes and off them
 def test_quantise_rows_of_more_than_31_bits_of_bytes(tctx, t, cols, shift):
