@@ -62,6 +62,7 @@ class StackRouter:
         self.gate_gradients = F32Buffer(ctx, b * top_k)
         self.counts, self.mean_probabilities = I32Buffer(ctx, stacks + 1), F32Buffer(ctx, stacks)
         self.loss, self.expected_cost, self.one = F32Buffer(ctx, 1), F32Buffer(ctx, 1), F32Buffer.from_host(ctx, [1.0])
+        self.choice_loss = F32Buffer(ctx, 1)  # the balance loss of a choice
         self.weights8, self.weight_scales = I32Buffer(ctx, (stacks * inner + 3) // 4), F32Buffer(ctx, stacks)
         self.choice_gates = F32Buffer(ctx, b)
         self._m = {
@@ -152,12 +153,12 @@ class StackRouter:
         self._lookup(tokens)
         int8_linear(self.ctx, m["hidden"], m["weights8"], self.weight_scales, m["logits"])
         router_forward(self.ctx, m["logits"], DeviceMatrix(buckets, self.batch_size, 1), m["choice_gates"], self.counts,
-                       self.mean_probabilities, self.loss, balance=self.balance)
+                       self.mean_probabilities, self.choice_loss, balance=self.balance)
 
     def read_counts(self) -> np.ndarray:
         """Choices of each stack in the last step or choice (a device-to-host read)."""
         return self.counts.download()[:-1]
 
     def read_losses(self) -> tuple:
-        """(expected cost, balance loss) of the last step."""
+        """(expected cost, balance loss) of the last step; a choice leaves them."""
         return float(self.expected_cost.download()[0]), float(self.loss.download()[0])

@@ -156,3 +156,35 @@ def test_graph_replays_after_larger_calls():
         graph.close()
         ctx.close()
         plain.close()
+
+
+# --------------------------------------------------------------------------- the router model
+VOCAB, ACTIVE, WIDTH, STACKS, BATCH = 50, 6, 8, 5, 40
+
+
+@pytest.fixture
+def model():
+    ctx = bo.Context(0)
+    rng = np.random.default_rng(11)
+    r = bo.StackRouter(ctx, VOCAB, ACTIVE, WIDTH, STACKS, BATCH, top_k=2, balance=0.05, drop_probability=0.2, seed=5)
+    tokens = rng.integers(-1, VOCAB, (BATCH, ACTIVE)).astype(np.int32)
+    costs = bo.F32Buffer.from_host(ctx, rng.random((BATCH, STACKS)).astype(np.float32))
+    yield ctx, r, tokens, bo.I32Buffer.from_host(ctx, tokens), costs, bo.I32Buffer(ctx, BATCH)
+    ctx.close()
+
+
+def eight_bit_choices(r, tokens):
+    """The choices of the parameters that the model holds now, and whether a position's two best logits are apart."""
+    table, weights = r.table.download().reshape(VOCAB, WIDTH), r.weights.download().reshape(STACKS, -1)
+    hidden = (np.float32(r.scale) * np.where(tokens.reshape(-1, 1) >= 0, table[tokens.reshape(-1)], np.float32(0))).reshape(BATCH, -1)
+    z, size = int8_product(*quantize_rows(hidden), *quantize_rows(weights), None)
+    order = np.sort(z, 1)
+    return z.argmax(1), order[:, -1] - order[:, -2] > 8 * U32 * size.max()
+
+
+def test_choice_leaves_the_last_steps_losses(model):
+    ctx, r, tokens, on_device, costs, buckets = model
+    r.gradients(on_device, costs)
+    losses = r.read_losses()
+    r.choose(on_device, buckets)
+    assert r.read_losses() == losses
