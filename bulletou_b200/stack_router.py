@@ -139,15 +139,18 @@ class StackRouter:
         self.quantized = False
 
     def quantize(self) -> None:
-        """The weights as 8-bit rows with a scale for each stack; ``choose`` calls it after a step."""
+        """The weights as 8-bit rows with a scale for each stack."""
         int8_quantize_rows(self.ctx, self._m["weights"], self._m["weights8"], self.weight_scales)
         self.quantized = True
 
-    def choose(self, tokens: I32Buffer, buckets: I32Buffer) -> None:
-        """buckets [batch] = the best stack of each position (a position without tokens: the first among equals)."""
+    def choose(self, tokens: I32Buffer, buckets: I32Buffer, *, keep_weights: bool = False) -> None:
+        """buckets [batch] = the best stack of each position (a position without tokens: the first among equals).
+
+        The weights are quantised as the buffer holds them now.  A program that serves fixed weights sets
+        `keep_weights`: those of the last ``quantize`` or choice are then taken, unless ``update`` has run since."""
         if len(buckets) != self.batch_size:
             raise CudaCppError(f"buckets have {len(buckets)} values, expected {self.batch_size}")
-        if not self.quantized:
+        if not (keep_weights and self.quantized):
             self.quantize()
         m = self._m
         self._lookup(tokens)

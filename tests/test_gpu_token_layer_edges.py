@@ -188,3 +188,32 @@ def test_choice_leaves_the_last_steps_losses(model):
     losses = r.read_losses()
     r.choose(on_device, buckets)
     assert r.read_losses() == losses
+
+
+def test_choices_follow_the_weights(model):
+    """After a step and after new values in the parameters' buffers; weights are kept from before only where that is asked."""
+    ctx, r, tokens, on_device, costs, buckets = model
+
+    def check():
+        want, apart = eight_bit_choices(r, tokens)
+        assert apart.any() and np.array_equal(buckets.download()[apart], want[apart])
+        return want
+
+    r.choose(on_device, buckets)
+    first = check()
+    r.train_step(bo.RangerUpdateParams(radam=bo.RAdamUpdateParams(step=1, learning_rate=0.5)), on_device, costs)
+    r.choose(on_device, buckets, keep_weights=True)  # kept weights end with an update
+    check()
+    rng = np.random.default_rng(13)
+    r.table.upload(rng.standard_normal((VOCAB, WIDTH)).astype(np.float32))
+    r.weights.upload(rng.standard_normal((STACKS, ACTIVE * WIDTH)).astype(np.float32))
+    r.choose(on_device, buckets)
+    assert not np.array_equal(check(), first)
+    r.choose(on_device, buckets, keep_weights=True)
+    check()
+    r.weights.upload(-r.weights.download())
+    before = buckets.download()
+    r.choose(on_device, buckets, keep_weights=True)
+    assert np.array_equal(buckets.download(), before)
+    r.choose(on_device, buckets)
+    check()
