@@ -144,7 +144,9 @@ class StackRouter:
         self.quantized = True
 
     def choose(self, tokens: I32Buffer, buckets: I32Buffer, *, keep_weights: bool = False) -> None:
-        """buckets [batch] = the best stack of each position (a position without tokens: the first among equals).
+        """buckets [batch] = the best stack of each position (a position without tokens: the first among equals).  A
+        position whose logits are not finite (its rows hold NaN or infinities) gets -1, a bucket that an SFNN step gives
+        to no stack; ``read_counts`` then adds up to fewer than the batch.
 
         The weights are quantised as the buffer holds them now.  A program that serves fixed weights sets
         `keep_weights`: those of the last ``quantize`` or choice are then taken, unless ``update`` has run since."""

@@ -217,3 +217,19 @@ def test_choices_follow_the_weights(model):
     assert np.array_equal(buckets.download(), before)
     r.choose(on_device, buckets)
     check()
+
+
+def test_position_that_is_not_finite_has_no_choice(model):
+    """-1, a bucket that belongs to no stack; the others choose as before."""
+    ctx, r, tokens, on_device, costs, buckets = model
+    r.choose(on_device, buckets)
+    before = buckets.download()
+    table = r.table.download().reshape(VOCAB, WIDTH)
+    broken = int(tokens[0][tokens[0] >= 0][0])
+    table[broken, 3] = np.nan
+    r.table.upload(table)
+    r.choose(on_device, buckets)
+    hit = (tokens == broken).any(1)
+    got = buckets.download()
+    assert (got[hit] == -1).all() and np.array_equal(got[~hit], before[~hit])
+    assert r.read_counts().sum() == BATCH - hit.sum()
