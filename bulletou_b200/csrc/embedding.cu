@@ -10,6 +10,7 @@
 // out_gradients read once and every row of the table written once.
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <utility>
 
 #include "device_matrix.cuh"
@@ -111,7 +112,10 @@ struct LookupArgs {
 // units of each row in flight in a lane, 155642 rows of 257 f32 46 us instead of
 // 66, 600000 of 63 bf16 37 instead of 55.  Aligned 16-byte blocks shifted into
 // place took 79 us there: all lanes go through the rows' ends element by element.
-template <typename In, typename Out, int kUnit, int kCols>
+//
+// kAnyScale: a scale that is not finite, which would not leave a padded token's
+// zeros as they are (a select of every row's scale cost finite ones up to 7 %).
+template <typename In, typename Out, int kUnit, int kCols, bool kAnyScale = false>
 __global__ void __launch_bounds__(kThreads, kLookupCtas) lookup_kernel(const LookupArgs a, int any_group, int span) {
     constexpr int kRows = 4;
     const int group = kCols > 1 ? 32 : any_group;  // with a group known only at run time the columns' offsets cost 100 bytes of spills
@@ -145,12 +149,13 @@ __global__ void __launch_bounds__(kThreads, kLookupCtas) lookup_kernel(const Loo
 #pragma unroll
                 for (int i = 0; i < kRows; ++i) {
                     if (i0 + i >= rows) break;
+                    const float scale = kAnyScale && token[i] >= a.tokens.vocab ? 0.0f : a.scale;
                     Out* const row = out + (i0 + i) * a.out_stride + u * kUnit;
 #pragma unroll
                     for (int k = 0; k < kCols; ++k) {
                         Raw<Out, kUnit> y;
 #pragma unroll
-                        for (int j = 0; j < kUnit; ++j) y.set(j, v[i][k].get(j) * a.scale);
+                        for (int j = 0; j < kUnit; ++j) y.set(j, v[i][k].get(j) * scale);
                         if (k == 0 || u + k * group < units) y.store(row + k * group * kUnit);
                     }
                 }
@@ -771,7 +776,7 @@ bool rows_of_units(const BulletOuB200Matrix& a, const BulletOuB200Matrix& b) {
            rows_aligned(b, std::min<size_t>(16, kUnit * sizeof(B)));
 }
 
-template <typename In, typename Out, int kUnit, int kCols>
+template <typename In, typename Out, int kUnit, int kCols, bool kAnyScale = false>
 int launch_lookup(BulletOuCudaCppContext* ctx, const LookupArgs& a) {
     const int units = a.width / kUnit;
     int group = 1;
@@ -784,11 +789,12 @@ int launch_lookup(BulletOuCudaCppContext* ctx, const LookupArgs& a) {
     const int64_t blocks = ((static_cast<int64_t>(a.tokens.n) + span - 1) / span * group + kThreads - 1) / kThreads;
     const unsigned x = static_cast<unsigned>(std::min(blocks, resident));
     const unsigned y = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(units / 64, resident / x)));
-    return launch_kernel(ctx, "embedding lookup launch", lookup_kernel<In, Out, kUnit, kCols>, LaunchShape{dim3(x, y), kThreads}, a, group, span);
+    return launch_kernel(ctx, "embedding lookup launch", lookup_kernel<In, Out, kUnit, kCols, kAnyScale>, LaunchShape{dim3(x, y), kThreads}, a, group, span);
 }
 
 template <typename In, typename Out>
 int lookup(BulletOuCudaCppContext* ctx, const LookupArgs& a, const BulletOuB200Matrix& table, const BulletOuB200Matrix& out) {
+    if (!std::isfinite(a.scale)) return launch_lookup<In, Out, 1, 1, true>(ctx, a);
     if (rows_of_units<In, Out, kVectorUnit<In, Out>>(table, out)) return launch_lookup<In, Out, kVectorUnit<In, Out>, 1>(ctx, a);
     if (rows_of_units<In, Out, 2>(table, out))
         return a.width > 64 ? launch_lookup<In, Out, 2, 2>(ctx, a) : launch_lookup<In, Out, 2, 1>(ctx, a);

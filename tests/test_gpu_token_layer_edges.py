@@ -23,6 +23,19 @@ def cuda(a):
     return torch.from_numpy(np.ascontiguousarray(a)).cuda()
 
 
+# --------------------------------------------------------------------------- lookup
+@pytest.mark.parametrize("width,pad", [(8, 0), (256, 0), (257, 0), (63, 1)])
+@pytest.mark.parametrize("scale", [float("inf"), float("nan"), -2.0])
+def test_padded_tokens_are_zeros_at_any_scale(tctx, width, pad, scale):
+    table = torch.ones(5, width + pad, device="cuda")[:, :width]
+    tokens = torch.tensor([-1, 4, 5, 0, -1, 2, 2**31 - 1], device="cuda", dtype=torch.int32)
+    for t in (torch.float32, torch.bfloat16):
+        out = torch.full((7, width), 9.0, device="cuda", dtype=t)
+        bo.embedding_forward(tctx, table, tokens, out, scale=scale)
+        inside = torch.tensor([False, True, False, True, False, True, False], device="cuda")
+        assert not out[~inside].any() and torch.equal(out[inside].nan_to_num(7.0), torch.full((3, width), scale, device="cuda", dtype=t).nan_to_num(7.0))
+
+
 # --------------------------------------------------------------------------- 8-bit product
 @pytest.mark.parametrize("rows,outer", [(1, 5), (2, 300), (40, 70), (300, 20000), (4096, 4096), (4700, 1100), (70000, 65)])
 @pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
