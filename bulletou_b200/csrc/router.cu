@@ -62,7 +62,7 @@ struct RouterArgs {
     size_t logit_grad_stride;
 };
 
-// 2^x and 1 / x to about two units in the last place, and a maximum that keeps NaN.
+// 2^x to about two units in the last place, and a maximum that keeps NaN.
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -78,13 +78,20 @@ __device__ __forceinline__ float max_nan(float a, float2 b) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b.x), "f"(b.y));
     return y;
 }
-__device__ __forceinline__ float reciprocal_approx(float x) {
+// 1 / x of a row's sums: the approximation and a step of Newton's iteration, half a
+// unit in the last place.  CUDA's division, whose special cases do not occur here,
+// takes 3 us more forward and 2 backward for 262144 x 81.
+__device__ __forceinline__ float reciprocal(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
+    return __fmaf_rn(y, __fmaf_rn(-x, y, 1.0f), y);
 }
-// A gate's part of its row's; exactly one where it is the only one.
-__device__ __forceinline__ float share_of(float p, float total) { return p == total ? 1.0f : p * reciprocal_approx(total); }
+// A gate's part of its row's, corrected by its remainder; exactly one where it is
+// the only one.
+__device__ __forceinline__ float share_of(float p, float total) {
+    const float inverse = reciprocal(total), q = p * inverse;
+    return p == total ? 1.0f : __fmaf_rn(__fmaf_rn(-q, total, p), inverse, q);
+}
 constexpr float kLog2E = 1.4426950408889634f;
 
 // Over the kGroup lanes that share a row.
@@ -155,7 +162,7 @@ struct Row {
         }
         const float total = group_sum<kGroup>(sum.x + sum.y);
         // a masked row's exponentials are zeros; a broken row is NaN
-        inverse = alive ? reciprocal_approx(total) : top == -INFINITY ? 0.0f : NAN;
+        inverse = alive ? reciprocal(total) : top == -INFINITY ? 0.0f : NAN;
     }
 };
 

@@ -246,3 +246,16 @@ def test_position_that_is_not_finite_has_no_choice(model):
     got = buckets.download()
     assert (got[hit] == -1).all() and np.array_equal(got[~hit], before[~hit])
     assert r.read_counts().sum() == BATCH - hit.sum()
+
+
+# --------------------------------------------------------------------------- router
+def test_gates_of_equal_logits_are_rounded_once(tctx):
+    """One of n alike: the exponentials and their sum are exact, so the gate is 1 / n to half a unit in its last place
+    (and 2^-45 for the iteration behind it)."""
+    for n in range(1, 513):
+        z = torch.full((1, n), -3.25, device="cuda")
+        experts, gates = torch.zeros(1, 1, device="cuda", dtype=torch.int32), torch.zeros(1, 1, device="cuda")
+        counts, mean, loss = torch.zeros(n + 1, device="cuda", dtype=torch.int32), torch.zeros(n, device="cuda"), torch.zeros(1, device="cuda")
+        bo.router_forward(tctx, z, experts, gates, counts, mean, loss, balance=1.0)
+        half_unit = 2.0 ** (np.floor(np.log2(1 / n)) - 24)
+        assert abs(gates.item() - 1 / n) <= half_unit + 2.0 ** -45 / n, n
