@@ -21,6 +21,8 @@ from bulletou_b200.sfnn import HALFKA_HM2_DIMENSIONS, PIECE_INPUTS  # noqa: E402
 
 
 def main(steps: int = 200, batch: int = 4096, width: int = 16, stacks: int = 9) -> dict:
+    if steps < 1:
+        raise SystemExit("at least one step is needed")
     ctx = bo.Context(0)
     config = bo.TeacherBatchConfig(feature_set="halfka_hm2", lambda_=1.0, win_rate_model=True)
     producer = bo.TeacherBatchProducer(ctx, config, batch, pinned=False)
