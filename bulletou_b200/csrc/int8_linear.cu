@@ -97,6 +97,20 @@ struct QuantizeArgs {
 
 constexpr int kGroup = 16;  // columns that a thread takes together: a 16-byte store of q
 
+// Which of the aligned 16-byte units around a row lie inside its matrix; the row's
+// values in the others are loaded one by one.
+struct RowUnits {
+    bool first_out, last_out;
+    const uint4* past;  // the units that may be read end here
+};
+
+template <typename T>
+__device__ __forceinline__ RowUnits row_units(const QuantizeArgs& a, const T* x, int cols) {
+    auto down = [](const void* p) { return reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(15); };
+    const uintptr_t past = down(reinterpret_cast<const char*>(x + cols) + 15), end = down(a.x_end);
+    return {down(x) < reinterpret_cast<uintptr_t>(a.x), past > end, reinterpret_cast<const uint4*>(min(past, end))};
+}
+
 // kGroup values of a row as they are in memory.
 template <typename T>
 struct Group {
@@ -117,23 +131,18 @@ struct Group {
         }
     }
     // The same of a row at any alignment: the aligned units that hold the values,
-    // shifted into place; units without a value of the row are not read.  Where they
-    // begin before the matrix or end after it the values are loaded one by one.
-    // (That took 31 us everywhere for 3373 rows of 5445 bf16, these 23.)
-    __device__ __forceinline__ void load_shifted(const QuantizeArgs& a, const T* x, int c, int cols) {
+    // shifted into place; units without a value of the row are not read, nor those
+    // that stick out of the matrix.  (Loads of single elements took 31 us for 3373
+    // rows of 5445 bf16, these 24.)
+    __device__ __forceinline__ void load_shifted(const T* x, int c, int cols, const RowUnits& units) {
         constexpr int kUnits = kGroup * sizeof(T) / 16;
         const char* const at = reinterpret_cast<const char*>(x + c);
         const unsigned offset = static_cast<unsigned>(reinterpret_cast<uintptr_t>(at)) & 15;
         const uint4* const from = reinterpret_cast<const uint4*>(at - offset);
-        const uint4* const end = reinterpret_cast<const uint4*>(x + cols);
-        if (static_cast<const void*>(from) < a.x || static_cast<const void*>(from + kUnits + 1) > a.x_end) {
-            load_elements(x, c, cols);
-            return;
-        }
         uint32_t w[4 * kUnits + 4];
 #pragma unroll
         for (int i = 0; i <= kUnits; ++i) {
-            const bool some = c < cols && from + i < end && (i < kUnits || offset != 0);
+            const bool some = c < cols && from + i < units.past && (i > 0 || c > 0 || !units.first_out) && (i < kUnits || offset != 0);
             const uint4 u = some ? __ldcs(from + i) : make_uint4(0, 0, 0, 0);
             w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
         }
@@ -148,6 +157,11 @@ struct Group {
             const uint32_t word = sizeof(T) == 2 ? __funnelshift_r(w[i], w[i + 1], (offset & 2) * 8) : w[i];
             reinterpret_cast<uint32_t*>(raw)[i] = left >= 4 ? word : left > 0 ? word & 0xffffu : 0;
         }
+    }
+    // The values in units that stick out.
+    __device__ __forceinline__ void load_rest(const T* x, int c, int cols, const RowUnits& units) {
+        const void* const past = x + min(c + kGroup, cols);
+        if (c < cols && ((c == 0 && units.first_out) || past > units.past)) load_elements(x, c, cols);
     }
     __device__ __forceinline__ float get(int i) const { return to_f32(reinterpret_cast<const T*>(raw)[i]); }
     // max |x|; NaN becomes +inf
@@ -196,22 +210,27 @@ __global__ void __launch_bounds__(kThreads, 4) quantize_kernel(const QuantizeArg
     const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / kRowThreads) + threadIdx.x / kRowThreads;
     const bool live = row < a.rows;
     const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.x_stride;
+    const int cols = live ? a.cols : 0;
+    const RowUnits units = row_units(a, x, cols);
     Group<T> held[kHeld];
-    auto load = [&](Group<T>& g, int c, int cols) {
+    auto load = [&](Group<T>& g, int c) {
         if constexpr (kAligned) g.load(x, c, cols);
-        else g.load_shifted(a, x, c, cols);
+        else g.load_shifted(x, c, cols, units);
+    };
+    auto load_rest = [&](Group<T>& g, int c) {
+        if (!kAligned && (units.first_out || units.last_out)) g.load_rest(x, c, cols, units);
     };
     float top = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-        const int c = (in_row + j * kRowThreads) * kGroup;
-        load(held[j], c, live ? a.cols : 0);
-    }
+    for (int j = 0; j < kHeld; ++j) load(held[j], (in_row + j * kRowThreads) * kGroup);
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) load_rest(held[j], (in_row + j * kRowThreads) * kGroup);
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) top = fmaxf(top, held[j].top());
-    for (int c = (in_row + kHeld * kRowThreads) * kGroup; live && c < a.cols; c += kRowThreads * kGroup) {
+    for (int c = (in_row + kHeld * kRowThreads) * kGroup; c < cols; c += kRowThreads * kGroup) {
         Group<T> g;
-        load(g, c, a.cols);
+        load(g, c);
+        load_rest(g, c);
         top = fmaxf(top, g.top());
     }
 #pragma unroll
@@ -234,7 +253,8 @@ __global__ void __launch_bounds__(kThreads, 4) quantize_kernel(const QuantizeArg
     }
     for (int c = (in_row + kHeld * kRowThreads) * kGroup; c < a.padded_cols; c += kRowThreads * kGroup) {
         Group<T> g;
-        load(g, c, a.cols);
+        load(g, c);
+        load_rest(g, c);
         g.store(a, q, c, factor, some);
     }
     if (in_row == 0) a.scales[row] = top == INFINITY ? NAN : some ? row_scale(top) : 0.0f;
