@@ -92,9 +92,9 @@ int scratch_slot(BulletOuCudaCppContext* ctx, int slot, size_t bytes, void** out
     Scratch& s = ctx->scratch[slot];
     if (bytes == 0) bytes = 256;
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(ctx->stream, &status) != cudaSuccess) {
-        cudaGetLastError();  // the default stream while another one captures
-        status = cudaStreamCaptureStatusNone;
+    if (ctx->stream != nullptr && ctx->stream != cudaStreamLegacy) {  // the default stream cannot be captured
+        const cudaError_t st = cudaStreamIsCapturing(ctx->stream, &status);
+        if (st != cudaSuccess) return fail(label, st);
     }
     const bool capturing = status != cudaStreamCaptureStatusNone;
     if (s.bytes < bytes) {
