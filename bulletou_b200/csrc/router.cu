@@ -18,6 +18,7 @@
 // 4.7 TB/s).  A lane for each row, the rows in shared memory, took 38 and 57 us:
 // 20 warps fit an SM, and the shared memory's bandwidth bounds them.
 #include <algorithm>
+#include <cstring>
 #include <type_traits>
 
 #include "device_matrix.cuh"
@@ -114,6 +115,33 @@ __device__ __forceinline__ int group_min(int v) {
     return v;
 }
 
+// Two f32 operations in one instruction, each rounded as by itself.  (By CUDA's
+// __fadd2_rn and its like 262144 x 81 f32 takes 40 us backward, so 37.)
+__device__ __forceinline__ uint64_t packed(float2 v) {
+    uint64_t u;
+    memcpy(&u, &v, sizeof(u));
+    return u;
+}
+__device__ __forceinline__ float2 unpacked(uint64_t u) {
+    float2 v;
+    memcpy(&v, &u, sizeof(v));
+    return v;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t y;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(packed(a)), "l"(packed(b)));
+    return unpacked(y);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t y;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(packed(a)), "l"(packed(b)));
+    return unpacked(y);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t y;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(packed(a)), "l"(packed(b)), "l"(packed(c)));
+    return unpacked(y);
+}
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // A row's logits and their exponentials: expert e in lane e % kGroup, place
@@ -156,9 +184,9 @@ struct Row {
         float2 sum = both(0.0f);
 #pragma unroll
         for (int i = 0; i < kPlaces / 2; ++i) {
-            const float2 x = __fmul2_rn(__fadd2_rn(z[i], both(-shift)), both(kLog2E));
+            const float2 x = mul2(add2(z[i], both(-shift)), both(kLog2E));
             e[i] = make_float2(exp2_approx(x.x), exp2_approx(x.y));
-            sum = __fadd2_rn(sum, e[i]);
+            sum = add2(sum, e[i]);
         }
         const float total = group_sum<kGroup>(sum.x + sum.y);
         // a masked row's exponentials are zeros; a broken row is NaN
@@ -234,7 +262,7 @@ __global__ void __launch_bounds__(kForwardThreads<kGroup, kPlaces>, 1) router_fo
         r.template load<T>(src, t < a.rows ? places : 0);
         r.normalise();
 #pragma unroll
-        for (int i = 0; i < kPlaces / 2; ++i) acc[i] = __ffma2_rn(r.e[i], both(r.inverse), acc[i]);
+        for (int i = 0; i < kPlaces / 2; ++i) acc[i] = fma2(r.e[i], both(r.inverse), acc[i]);
         alive += r.alive && lane == 0;
         float total = 0.0f, own = 0.0f;  // lane j keeps the j-th choice
         int pick = -1;
@@ -392,8 +420,8 @@ __global__ void __launch_bounds__(kThreads, kCtas<kPlaces>) router_backward_kern
         float2 dots = both(0.0f);
 #pragma unroll
         for (int i = 0; i < kPlaces / 2; ++i) {
-            r.e[i] = __fmul2_rn(r.e[i], both(r.inverse));
-            dots = __ffma2_rn(r.e[i], h[i], dots);
+            r.e[i] = mul2(r.e[i], both(r.inverse));
+            dots = fma2(r.e[i], h[i], dots);
         }
         float dot = group_sum<kGroup>(dots.x + dots.y);
         float direct = 0.0f;  // what the choice's gate adds to its logit's gradient
@@ -411,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<kPlaces>) router_backward_kern
         }
 #pragma unroll
         for (int i = 0; i < kPlaces / 2; ++i) {
-            const float2 g = __fmul2_rn(r.e[i], __fadd2_rn(h[i], both(-dot)));
+            const float2 g = mul2(r.e[i], add2(h[i], both(-dot)));
             if (2 * i < kPlaces - 2 ? mine > 0 : 2 * i < mine) dst[kGroup * 2 * i] = from_f32<T>(g.x);
             if (2 * i < kPlaces - 2 ? mine > 0 : 2 * i + 1 < mine) dst[kGroup * (2 * i + 1)] = from_f32<T>(g.y);
         }
