@@ -9,9 +9,11 @@
 // is used, and f = 2^16 / (2^16 - T), so E[y] = x holds exactly.
 //
 // Aligned rows are bound by memory: 655360 x 256 bf16 with a residual take 152 to
-// 164 us, 6.2 to 6.6 TB/s (a copy: 6.5).  Unaligned ones by the integer pipe, which runs
-// the logic and comparisons at half rate: 20011 x 769 f32 out of rows of 800 take
-// 31 us, 3.9 TB/s, 228 instructions for each piece of up to 224 elements.
+// 164 us, 6.2 to 6.6 TB/s (a copy: 6.5).  Unaligned ones by instructions: 20011 x 769
+// f32 out of rows of 800 take 31 us, 3.9 TB/s, 228 instructions for each piece of up
+// to 224 elements.  The generator is the smaller part of them (aligned rows go
+// through twice the elements in a time with the same rounds); the rest are
+// ballots, selects, and a load and a store for each element of a lane.
 #include <algorithm>
 #include <cmath>
 

@@ -195,7 +195,7 @@ struct Group {
 // the maximum and the rounding: x is read once.  Rows longer than 2 * kGroup *
 // kRowThreads (only with kRowThreads == kThreads) read the rest again, from L2.
 // 16384 x 4096 bf16: 38 us, 5.2 TB/s, bound by memory and the conversions together
-// (54 % of the issue slots); with the values held as f32, 92 registers and 16
+// (61 % of the issue slots); with the values held as f32, 92 registers and 16
 // warps on an SM it took 67 us.
 template <typename T, int kRowThreads, bool kAligned>
 __global__ void __launch_bounds__(kThreads, 4) quantize_kernel(const QuantizeArgs a) {

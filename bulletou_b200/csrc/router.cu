@@ -13,9 +13,10 @@
 // lane, warp and CTA and joined in a fixed order, so no result depends on
 // timing.  Counts are integers.
 //
-// 262144 rows of 81 with their top 2: forward 27 us (bound by the comparisons of
-// the maximum and the choices, which run at half rate), backward 36 us (170 MB,
-// 4.7 TB/s).  A lane for each row, the rows in shared memory, took 38 and 57 us:
+// 262144 rows of 81 with their top 2: forward 32 us with the join's launch (the 16
+// warps that fit an SM wait for their loads; the comparisons of the maximum and
+// the choices, which run at half rate, take 48 % of their pipe), backward 35 us (170
+// MB, 4.8 TB/s).  A lane for each row, the rows in shared memory, took 38 and 57 us:
 // 20 warps fit an SM, and the shared memory's bandwidth bounds them.
 #include <algorithm>
 #include <cstring>
